@@ -312,12 +312,13 @@ def _quantise(x: torch.Tensor, kind: str):
     """x [..., block, D] float32 -> (codes as float32, scale [..., 1, 1]): one scale for the block."""
     finite = torch.where(torch.isfinite(x), x, torch.zeros_like(x))
     amax = finite.abs().amax(dim=(-1, -2), keepdim=True)
+    most = torch.full_like(amax, 127.0 if kind == "int8" else 448.0)  # a tensor: by a number torch multiplies with the reciprocal
     if kind == "int8":
-        scale = (amax / 127.0).clamp(min=2.0**-100)
+        scale = (amax / most).clamp(min=2.0**-100)
         # the quotient in 64 bits: next to the border between two codes 32 are too few
         q = torch.round((torch.nan_to_num(x, nan=0.0).double() / scale.double())).clamp(-127, 127).float()
         return q, scale
-    mantissa, exponent = torch.frexp(amax / 448.0)
+    mantissa, exponent = torch.frexp(amax / most)
     exponent = torch.where(mantissa == 0.5, exponent - 1, exponent)  # ceil(log2(.))
     scale = torch.exp2(torch.where(amax > 0, exponent, torch.full_like(exponent, -100)).clamp(min=-100).double()).float()
     q = (torch.nan_to_num(x, nan=0.0) / scale).clamp(-448, 448).to(torch.float8_e4m3fn).float()
@@ -478,11 +479,12 @@ def _exact_stored(x: torch.Tensor, kind: str, block: int) -> torch.Tensor:
     for t0 in range(0, x.shape[0] - block + 1, block):
         rows = x[t0 : t0 + block]
         most = rows.abs().amax(dim=(0, 2))  # per head
+        share = most / torch.full_like(most, 127.0 if kind == "int8" else 448.0)  # (a quotient, not a product with 1 / 127)
         if kind == "int8":
-            step = torch.maximum((most.float() / 127.0).double(), torch.full_like(most, 2.0**-100))[None, :, None]
+            step = share.float().double().clamp(min=2.0**-100)[None, :, None]
             out[t0 : t0 + block] = (rows / step).round().clamp(-127, 127) * step
         else:
-            step = torch.exp2(torch.log2(most / 448.0).ceil().clamp(min=-100))[None, :, None]
+            step = torch.exp2(torch.log2(share).ceil().clamp(min=-100))[None, :, None]
             y = rows / step
             size = torch.floor(torch.log2(y.abs().clamp(min=2.0**-20))).clamp(min=-6)  # e4m3: 3 bits behind the first, exponents down to -6
             grid = torch.exp2(size - 3)

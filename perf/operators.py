@@ -334,35 +334,37 @@ class _PlainCache:
         code = torch.int8 if self.kind == "int8" else torch.float8_e4m3fn
         self.codes = [torch.zeros((b, kv, cap, d), dtype=code, device="cuda") for _ in range(2)]
         self.scales = [torch.zeros((b, kv, cap // block), dtype=torch.float32, device="cuda") for _ in range(2)]
-        self.tails = [torch.zeros((b, kv, block, d), dtype=torch.bfloat16, device="cuda") for _ in range(2)]
-        self.held = [0] * b
+        # two places for open blocks: the one that was open before a call stays as it is when the call opens another
+        self.tails = [torch.zeros((b, kv, 2, block, d), dtype=torch.bfloat16, device="cuda") for _ in range(2)]
+        self.held, self.side = [0] * b, [0] * b
 
     def append(self, i: int, k: torch.Tensor, v: torch.Tensor, move: bool = True):
         """Tokens k, v [n, kv, D] behind what sequence i holds; with `move` it holds them from now on."""
-        first, block, n = self.held[i], self.block, k.shape[0]
+        first, block, n, side = self.held[i], self.block, k.shape[0], self.side[i]
         part = first % block
         for x, codes, scales, tails in zip((k, v), self.codes, self.scales, self.tails):
-            rows = torch.cat([tails[i, :, :part], x.transpose(0, 1)], dim=1)  # [kv, part + n, D]
+            rows = torch.cat([tails[i, :, side, :part], x.transpose(0, 1)], dim=1)  # [kv, part + n, D]
             full = rows.shape[1] // block
+            tails[i, :, side, part : part + n] = rows[:, part:block]
             if full:
                 whole = rows[:, : full * block].float().reshape(rows.shape[0], full, block, -1)
                 q, scale = _quantise(whole, self.kind)
                 at = first - part
                 codes[i, :, at : at + full * block] = q.reshape(rows.shape[0], full * block, -1).to(codes.dtype)
                 scales[i, :, at // block : at // block + full] = scale[..., 0, 0]
-                tails[i, :, : rows.shape[1] - full * block] = rows[:, full * block :]
-            else:
-                tails[i, :, part : part + n] = x.transpose(0, 1)
+                tails[i, :, 1 - side, : rows.shape[1] - full * block] = rows[:, full * block :]
         if move:
             self.held[i] += n
+            self.side[i] ^= self.held[i] // block != first // block
 
     def rows(self, i: int, n: int) -> list:
         """The first n tokens of sequence i as the cache holds them: K, V [kv, n, D] float32."""
         full = n // self.block * self.block
+        side = self.side[i] ^ (n // self.block != self.held[i] // self.block)
         out = []
         for codes, scales, tails in zip(self.codes, self.scales, self.tails):
             whole = codes[i, :, :full].float() * scales[i, :, : full // self.block].repeat_interleave(self.block, dim=1)[..., None]
-            out.append(torch.cat([whole, tails[i, :, : n - full].float()], dim=1))
+            out.append(torch.cat([whole, tails[i, :, side, : n - full].float()], dim=1))
         return out
 
 
@@ -557,16 +559,19 @@ def exact(case, seed: int):
                 whole[i, :, : case["new"]] = _exact_stored(x[i], case["kind"], case["block"]).transpose(0, 1)
             dense.append(whole)
         return dense
-    if sum(_held(case)) * case["kv"] * case["dim"] > 300_000_000:
+    if sum(_held(case)) * case["kv"] * case["dim"] > 600_000_000:
         return None
     out = torch.empty(s["q"].shape, dtype=torch.float64, device="cuda")
-    tails = [torch.full((case["batch"], case["kv"], case["block"], case["dim"]), 0.0, dtype=torch.float64, device="cuda") for _ in range(2)]
+    block = case["block"]
+    tails = [torch.zeros((case["batch"], case["kv"], 2, block, case["dim"]), dtype=torch.float64, device="cuda") for _ in range(2)]
     for i, (pk, pv) in enumerate(s["past"]):
         k, v = torch.cat([pk, s["k"][i]]), torch.cat([pv, s["v"][i]])
-        stored = [_exact_stored(x, case["kind"], case["block"]) for x in (k, v)]
+        stored = [_exact_stored(x, case["kind"], block) for x in (k, v)]
         out[i] = _exact_rows(s["q"][i], stored[0], stored[1], pk.shape[0], 0, case)
-        # rows behind the last token of the incomplete block hold what an earlier block left there
-        n = k.shape[0] // case["block"] * case["block"]
+        # two open blocks are kept: the first that the past began with, and, if it filled up, the one open now
+        now = k.shape[0] // block
         for tail, x in zip(tails, (k, v)):
-            tail[i, :, : x.shape[0] - n] = x[n:].double().transpose(0, 1)
+            tail[i, :, 0, : min(block, x.shape[0])] = x[:block].double().transpose(0, 1)
+            if now:
+                tail[i, :, 1, : x.shape[0] - now * block] = x[now * block :].double().transpose(0, 1)
     return [out, *tails] if case["op"] == "decode" else [out]

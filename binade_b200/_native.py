@@ -21,6 +21,24 @@ class R4Struct(C.Structure):
     _fields_ = [(n, _vp) for n in ("raw", "codes", "flags", "esc", "table", "row_esc")] + [("n_esc", _u64), ("esc_cols", _vp), ("col_esc", _vp)]
 
 
+class Scores(C.Structure):
+    """bn_scores: what turns q.k into a score, and which keys a query sees."""
+
+    _fields_ = [("scale", C.c_float), ("softcap", C.c_float), ("window", _i64), ("slopes", _vp), ("causal", _int)]
+
+
+class KV8Struct(C.Structure):
+    """bn_kv8: device pointers and sizes of one layer's 8-bit key/value cache."""
+
+    _fields_ = [(n, _vp) for n in ("k", "v", "k_scale", "v_scale", "k_tail", "v_tail", "length", "side")] + [(n, _i64) for n in ("batch", "kv_heads", "rows", "D", "max_seq")] + [("block", _int), ("kind", _int)]
+
+
+class LogitRules(C.Structure):
+    """bn_logit_rules: penalties, bias and mask of a batch of logits."""
+
+    _fields_ = [("seen", _vp), ("counts", _vp), ("seen_row", _i64), ("counts_row", _i64)] + [(n, _vp) for n in ("repetition", "presence", "frequency")] + [(n, C.c_float) for n in ("repetition_all", "presence_all", "frequency_all")] + [("bias", _vp), ("bias_row", _i64), ("mask", _vp), ("mask_row", _i64)]
+
+
 _SIGNATURES = {
     "cuda": {
         "bn_abi_version": [],
@@ -47,6 +65,14 @@ _SIGNATURES = {
         "bn_r4_gather_grouped": [_vp, C.POINTER(R4Struct), _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _vp],
         "bn_moe_route": [_vp, _int, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _vp],
         "bn_swiglu": [_vp, _vp, _i64, _vp, _vp],
+        "bn_attention": [_vp, _i64, _i64] * 3 + [_i64] * 4 + [_vp, _i64, _vp, C.POINTER(Scores), _vp, _i64, _i64, _int, _vp],
+        "bn_kv8_append": [C.POINTER(KV8Struct), _vp, _i64, _i64, _i64, _vp, _i64, _i64, _i64, _i64, _vp, _vp],
+        "bn_kv8_workspace": [C.POINTER(KV8Struct), _i64, _i64],
+        "bn_kv8_attend": [C.POINTER(KV8Struct), _vp, _i64, _i64, _i64, _i64, _i64, _vp, _vp, C.POINTER(Scores), _vp, _i64, _i64, _i64, _int, _vp, _u64, _vp],
+        "bn_kv8_advance": [C.POINTER(KV8Struct), _i64, _vp, _vp],
+        "bn_kv8_dense": [C.POINTER(KV8Struct), _vp, _vp, _vp],
+        "bn_token_counts": [_vp, _int, _i64, _i64, _i64, _vp, _i64, _int, _vp, _i64, _vp, _i64, _vp],
+        "bn_logits": [_vp, _int, _i64, _i64, _i64, C.POINTER(LogitRules), _vp, _i64, _vp, _vp],
         "bn_push_gather": [_vp, _vp, _int, _vp, _u64, _vp, _int, _int, _vp, _vp],
         "bn_push_gather_beside": [_vp, _vp, _int, _vp, _u64, _vp, _int, _int, _vp, _vp],
         "bn_r4_mma": [_vp, _i64, C.POINTER(R4Struct), _i64, _i64, _i64, _vp, _i64, _vp],
@@ -83,7 +109,7 @@ def load(which: str) -> C.CDLL:
         lib = C.CDLL(str(path))
         for name, args in _SIGNATURES[which].items():
             fn = getattr(lib, name)
-            fn.argtypes, fn.restype = args, _int
+            fn.argtypes, fn.restype = args, _u64 if name == "bn_kv8_workspace" else _int
         getattr(lib, _ERRFN[which]).restype = C.c_char_p
         _libs[which] = lib
     return _libs[which]

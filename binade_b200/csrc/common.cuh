@@ -60,6 +60,8 @@ int mma_rows(const bn_r4 *w, const uint16_t *x, int64_t x_stride, int64_t M, int
 int mma_status(int *status);
 int exchange_status(int *status);  // exchange.cu
 int exchange_status_reset();
+int kv8_status(int *status);  // kv8.cu
+int kv8_status_reset();
 int mma_status_reset();
 int stream_status_reset();
 int oct_status_reset();

@@ -1,0 +1,206 @@
+// Writing and reading back the 8-bit key/value cache (bn_kv8).
+#include <stdio.h>
+
+#include "kv8.cuh"
+
+namespace bn {
+
+__device__ int g_kv8_error;  // 1: tokens were brought that the cache has no room for
+
+namespace {
+
+// The nearest code to x / scale, ties to the even one, for finite x; 0 for NaN, the largest code for an infinity.
+__device__ __forceinline__ uint32_t int8_code(float x, float scale) {
+  float t = __fdiv_rn(x, scale), q = rintf(t);
+  if (fabsf(t - q) == 0.5f) {  // the rounded quotient lies between two codes: the real one may lie to either side
+    const float r = fmaf(-t, scale, x);
+    if (r > 0.0f) q = ceilf(t);
+    if (r < 0.0f) q = floorf(t);
+  }
+  q = fminf(fmaxf(q, -127.0f), 127.0f);
+  return x == x ? (uint32_t)(int)q & 0xFFu : 0u;
+}
+
+// Least power of two, at least 2^-100, times which 448 (the largest e4m3 value) is not below amax.
+__device__ __forceinline__ float e4m3_scale(float amax) {
+  const uint32_t u = __float_as_uint(amax);
+  const int e = (int)(u >> 23) - 127 - 8 + ((u & 0x7FFFFFu) > 0x600000u);
+  return __uint_as_float((uint32_t)(max(e, -100) + 127) << 23);
+}
+
+__device__ __forceinline__ float finite_size(float x) {
+  const float s = fabsf(x);
+  return s <= 3.4028235e38f ? s : 0.0f;
+}
+
+struct AppendArgs {
+  bn_kv8 c;
+  const uint16_t *k, *v;
+  int64_t k_seq, k_token, k_head, v_seq, v_token, v_head;  // elements
+  const int32_t *counts;
+  int tokens, rel;  // tokens a sequence brings at most; blocks of the cache that those can touch
+};
+
+// One block of tokens of one sequence and head, keys or values, by 128 threads: a full block is scaled, coded
+// and stored; the tokens of the blocks that were open or stay open go to the tail in BF16. CHUNKS: 16-byte
+// pieces of the block that a thread has. The read of the new rows and the write of the codes bound it; a block
+// stays in registers between its maximum and its codes.
+template <int CHUNKS>
+__global__ void __launch_bounds__(128) append_kernel(const __grid_constant__ AppendArgs a) {
+  const bn_kv8 &c = a.c;
+  __shared__ float part_max[4];
+  uint32_t at = blockIdx.x;
+  const bool values = at & 1;
+  at >>= 1;
+  const int rel = (int)(at % a.rel);
+  at /= a.rel;
+  const int h = (int)(at % (uint32_t)c.kv_heads);
+  const int64_t b = at / (uint32_t)c.kv_heads, unit = b * c.kv_heads + h;
+  int held, brought;
+  kv8_tokens(c, a.counts, a.tokens, b, held, brought);
+  if (rel == 0 && h == 0 && !values && threadIdx.x == 0) {
+    const int asked = a.counts ? min(max(a.counts[b], 0), a.tokens) : a.tokens;
+    if (asked > brought) atomicExch(&g_kv8_error, 1);
+  }
+  if (brought == 0) return;
+  const int block = c.block, first = held / block, end = held + brought, last = (end - 1) / block;
+  const int D = (int)c.D, per_row = D / 8;
+  const uint16_t *const in = values ? a.v + b * a.v_seq + h * a.v_head : a.k + b * a.k_seq + h * a.k_head;
+  const int64_t step = values ? a.v_token : a.k_token;
+  uint16_t *const tails = (values ? c.v_tail : c.k_tail) + unit * 2 * block * D;
+  const int j = first + rel;
+  if (j > last) return;
+  {
+    const bool full = (j + 1) * (int64_t)block <= end, open = j == first || !full;  // the first block goes to its slot, full or not
+    uint16_t *const tail = tails + (open ? kv8_slot(c, b, held, j) : 0) * block * D;
+    uint4 x[CHUNKS];
+    float amax = 0.0f;
+#pragma unroll
+    for (int i = 0; i < CHUNKS; i++) {
+      const int chunk = (int)threadIdx.x + 128 * i, row = chunk / per_row, col = chunk % per_row, p = j * block + row;
+      x[i] = make_uint4(0, 0, 0, 0);
+      if (p < end && (full || p >= held)) x[i] = *reinterpret_cast<const uint4 *>(p < held ? tail + row * D + col * 8 : in + (int64_t)(p - held) * step + col * 8);
+      if (open && p >= held && p < end) *reinterpret_cast<uint4 *>(tail + row * D + col * 8) = x[i];
+      const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+#pragma unroll
+      for (int e = 0; e < 4; e++) amax = fmaxf(amax, fmaxf(finite_size(__uint_as_float(w[e] << 16)), finite_size(__uint_as_float(w[e] & 0xFFFF0000u))));
+    }
+    if (!full) return;
+#pragma unroll
+    for (int d = 16; d; d >>= 1) amax = fmaxf(amax, __shfl_xor_sync(BN_FULL, amax, d));
+    if (lane_id() == 0) part_max[threadIdx.x >> 5] = amax;
+    __syncthreads();
+    amax = fmaxf(fmaxf(part_max[0], part_max[1]), fmaxf(part_max[2], part_max[3]));
+    const float scale = c.kind == KV8_INT8 ? fmaxf(__fdiv_rn(amax, 127.0f), 7.888609052210118e-31f) : e4m3_scale(amax);
+    const float inv = __frcp_rn(scale);  // of a power of two: exact
+    uint8_t *const codes = (values ? c.v : c.k) + (unit * c.rows + (int64_t)j * block) * D;
+    if (threadIdx.x == 0) (values ? c.v_scale : c.k_scale)[unit * (c.rows / block) + j] = scale;
+#pragma unroll
+    for (int i = 0; i < CHUNKS; i++) {
+      const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+      uint32_t out[2];
+#pragma unroll
+      for (int e = 0; e < 2; e++) {
+        float f[4] = {__uint_as_float(w[2 * e] << 16), __uint_as_float(w[2 * e] & 0xFFFF0000u), __uint_as_float(w[2 * e + 1] << 16), __uint_as_float(w[2 * e + 1] & 0xFFFF0000u)};
+        if (c.kind == KV8_INT8) {
+          out[e] = int8_code(f[0], scale) | int8_code(f[1], scale) << 8 | int8_code(f[2], scale) << 16 | int8_code(f[3], scale) << 24;
+        } else {
+#pragma unroll
+          for (int n = 0; n < 4; n++) f[n] = f[n] == f[n] ? f[n] * inv : 0.0f;
+          out[e] = (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(f[0], f[1]), __NV_SATFINITE, __NV_E4M3) | (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(f[2], f[3]), __NV_SATFINITE, __NV_E4M3) << 16;
+        }
+      }
+      *reinterpret_cast<uint2 *>(codes + ((int64_t)threadIdx.x + 128 * i) * 8) = make_uint2(out[0], out[1]);
+    }
+  }
+}
+
+__global__ void __launch_bounds__(256) advance_kernel(const __grid_constant__ bn_kv8 c, int n, const int32_t *__restrict__ counts) {
+  const int64_t b = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (b >= c.batch) return;
+  const int held = min(max(c.length[b], 0), (int)c.max_seq);
+  const int now = (int)min(max((int64_t)held + (counts ? counts[b] : n), (int64_t)0), c.max_seq);
+  c.length[b] = now;
+  if (now / c.block != held / c.block) c.side[b] ^= 1;
+}
+
+// Eight values of a token a thread, of keys and of values; tokens that the cache does not hold as zeros.
+template <int KIND>
+__global__ void __launch_bounds__(256) dense_kernel(const __grid_constant__ bn_kv8 c, float *__restrict__ k, float *__restrict__ v) {
+  const int per_row = (int)c.D / 8;
+  const int64_t n = c.batch * c.kv_heads * c.max_seq * per_row, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= n) return;
+  const int col = (int)(i % per_row);
+  const int64_t row = i / per_row, unit = row / c.max_seq;
+  const int p = (int)(row % c.max_seq), length = min(max(c.length[unit / c.kv_heads], 0), (int)c.max_seq), full = length / c.block * c.block;
+#pragma unroll
+  for (int side = 0; side < 2; side++) {
+    float x[8] = {};
+    if (p < full) {
+      const float scale = (side ? c.v_scale : c.k_scale)[unit * (c.rows / c.block) + p / c.block];
+      const uint2 w = *reinterpret_cast<const uint2 *>((side ? c.v : c.k) + (unit * c.rows + p) * c.D + col * 8);
+#pragma unroll
+      for (int e = 0; e < 8; e++) x[e] = kv8_code<KIND>(((e < 4 ? w.x : w.y) >> (8 * (e & 3))) & 0xFFu) * scale;
+    } else if (p < length) {
+      const uint4 w = *reinterpret_cast<const uint4 *>((side ? c.v_tail : c.k_tail) + ((unit * 2 + (c.side[unit / c.kv_heads] & 1)) * c.block + p - full) * c.D + col * 8);
+      const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+      for (int e = 0; e < 8; e++) x[e] = e & 1 ? __uint_as_float(u[e >> 1] & 0xFFFF0000u) : __uint_as_float(u[e >> 1] << 16);
+    }
+    float4 *const out = reinterpret_cast<float4 *>((side ? v : k) + i * 8);
+    out[0] = make_float4(x[0], x[1], x[2], x[3]), out[1] = make_float4(x[4], x[5], x[6], x[7]);
+  }
+}
+
+}  // namespace
+
+int kv8_status(int *status) {
+  BN_CUDA(cudaMemcpyFromSymbol(status, g_kv8_error, sizeof(int)));
+  return BN_OK;
+}
+
+int kv8_status_reset() {
+  const int zero = 0;
+  BN_CUDA(cudaMemcpyToSymbol(g_kv8_error, &zero, sizeof(int)));
+  return BN_OK;
+}
+
+int refuse(const char *who, const char *why) {
+  char msg[256];
+  snprintf(msg, sizeof msg, "%s: %s", who, why);
+  return fail(BN_ERR_ARG, msg);
+}
+
+}  // namespace bn
+
+extern "C" int bn_kv8_append(const bn_kv8 *c, const uint16_t *k, int64_t k_seq, int64_t k_token, int64_t k_head, const uint16_t *v, int64_t v_seq, int64_t v_token, int64_t v_head, int64_t tokens, const int32_t *counts, void *stream) {
+  if (const char *why = bn::kv8_refusal(c)) return bn::refuse("bn_kv8_append", why);
+  if (tokens < 0 || tokens > 0x3FFFFFFF || (tokens && (!k || !v))) return bn::fail(BN_ERR_ARG, "bn_kv8_append: null pointer or bad number of tokens");
+  if (((uintptr_t)k | (uintptr_t)v) & 15 || (k_seq | k_token | k_head | v_seq | v_token | v_head) & 7) return bn::fail(BN_ERR_ARG, "bn_kv8_append: rows have to start on 16 bytes");
+  if (tokens == 0) return BN_OK;
+  bn::AppendArgs a{*c, k, v, k_seq, k_token, k_head, v_seq, v_token, v_head, counts, (int)tokens, 0};
+  a.rel = (int)((tokens + c->block - 1) / c->block) + 1;  // a run of tokens that starts inside a block touches one more
+  const int64_t blocks = c->batch * c->kv_heads * a.rel * 2;
+  if (blocks > 0x7FFFFFFF) return bn::fail(BN_ERR_ARG, "bn_kv8_append: too many tokens for one call");
+  const int chunks = (int)(c->block * c->D / 1024);
+  auto kern = chunks == 1 ? bn::append_kernel<1> : chunks == 2 ? bn::append_kernel<2> : chunks == 4 ? bn::append_kernel<4> : chunks == 8 ? bn::append_kernel<8> : bn::append_kernel<16>;
+  kern<<<(unsigned)blocks, 128, 0, (cudaStream_t)stream>>>(a);
+  return bn::launched("append_kernel");
+}
+
+extern "C" int bn_kv8_advance(const bn_kv8 *c, int64_t n, const int32_t *counts, void *stream) {
+  if (const char *why = bn::kv8_refusal(c)) return bn::refuse("bn_kv8_advance", why);
+  if (n < -0x3FFFFFFF || n > 0x3FFFFFFF) return bn::fail(BN_ERR_ARG, "bn_kv8_advance: bad number of tokens");
+  bn::advance_kernel<<<(unsigned)((c->batch + 255) / 256), 256, 0, (cudaStream_t)stream>>>(*c, (int)n, counts);
+  return bn::launched("advance_kernel");
+}
+
+extern "C" int bn_kv8_dense(const bn_kv8 *c, float *k, float *v, void *stream) {
+  if (const char *why = bn::kv8_refusal(c)) return bn::refuse("bn_kv8_dense", why);
+  if (!k || !v || ((uintptr_t)k | (uintptr_t)v) & 15) return bn::fail(BN_ERR_ARG, "bn_kv8_dense: outputs have to start on 16 bytes");
+  const int64_t blocks = (c->batch * c->kv_heads * c->max_seq * (c->D / 8) + 255) / 256;
+  if (blocks > 0x7FFFFFFF) return bn::fail(BN_ERR_ARG, "bn_kv8_dense: the cache is too large for one call");
+  if (c->kind == BN_KV8_INT8) bn::dense_kernel<BN_KV8_INT8><<<(unsigned)blocks, 256, 0, (cudaStream_t)stream>>>(*c, k, v);
+  else bn::dense_kernel<BN_KV8_E4M3><<<(unsigned)blocks, 256, 0, (cudaStream_t)stream>>>(*c, k, v);
+  return bn::launched("dense_kernel");
+}

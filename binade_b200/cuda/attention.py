@@ -1,0 +1,228 @@
+"""Attention beside the R4 linear layers: of prompts, and of new tokens over a cache held in 8 bits.
+
+  attention(q, k, v, offsets)      packed prompts: every query over the keys of its own document
+  KV8Cache(layers, batch, ...)     keys and values of a batch of sequences as 8-bit codes with a scale for
+                                   each block of tokens and head; append, attend, advance, dense
+
+Scores take the options that models put on them: softcap (s = cap tanh(s / cap)), slopes (a bias
+-slope |i - j| for each query head), window (keys at a distance below it), prefix (the first keys of a document,
+seen from everywhere in it) and causal. Kernels, no gradients: tensors that ask for one are refused.
+"""
+
+from __future__ import annotations
+
+import ctypes
+import math
+
+import torch
+
+from .. import _native
+from . import kernels as ck
+
+HEAD_DIMS = (64, 128, 256)
+BLOCKS = (16, 32, 64)
+KINDS = {"int8": 0, "e4m3": 1}  # BN_KV8_INT8, BN_KV8_E4M3
+
+
+def _rows(t: torch.Tensor, name: str, dims: int, device) -> torch.Tensor:
+    """Checks a BF16 tensor of rows (its last dimension a head's) and gives it with rows that the kernels
+    can read: neighbouring elements, every row on 16 bytes."""
+    if not isinstance(t, torch.Tensor) or t.dtype != torch.bfloat16 or t.dim() != dims:
+        raise ValueError(f"{name} has to be a bfloat16 tensor of {dims} dimensions")
+    if t.device != device:
+        raise ValueError(f"{name} is on {t.device}, the call on {device}")
+    if t.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{name} asks for a gradient: attention here has none (use torch.no_grad)")
+    if t.stride(-1) != 1 or t.data_ptr() % 16 or any(s % 8 for s, n in zip(t.stride()[:-1], t.shape[:-1]) if n > 1):
+        t = t.contiguous()
+        if t.data_ptr() % 16:
+            t = t.clone()
+    return t
+
+
+def _steps(t: torch.Tensor):
+    """Strides of the leading dimensions; of one that is not stepped, 0."""
+    return [s if n > 1 else 0 for s, n in zip(t.stride()[:-1], t.shape[:-1])]
+
+
+def _numbers(t, name: str, n: int, device, dtype=torch.int32) -> torch.Tensor | None:
+    if t is None:
+        return None
+    if not isinstance(t, torch.Tensor) or t.device != device or t.dim() != 1 or t.numel() != n or (dtype == torch.int32 and t.is_floating_point()):
+        raise ValueError(f"{name} has to be a tensor of {n} {'whole ' if dtype == torch.int32 else ''}numbers on {device}")
+    return t.to(dtype).contiguous()
+
+
+def extent(t: torch.Tensor):
+    """First and last byte address (the latter exclusive) that a tensor's elements lie in."""
+    last = sum((n - 1) * s for n, s in zip(t.shape, t.stride())) if t.numel() else -1
+    return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+
+
+def overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    (a0, a1), (b0, b1) = extent(a), extent(b)
+    return a0 < b1 and b0 < a1
+
+
+def _out(out, like: torch.Tensor, device, *inputs) -> torch.Tensor:
+    if out is None:
+        return torch.empty(like.shape, dtype=torch.bfloat16, device=device)
+    if not isinstance(out, torch.Tensor) or out.dtype != torch.bfloat16 or out.shape != like.shape or out.device != device or out.requires_grad:
+        raise ValueError("out has to be a bfloat16 tensor of q's shape on its device")
+    if out.stride(-1) != 1 or out.data_ptr() % 16 or any(s % 8 or s == 0 for s, n in zip(out.stride()[:-1], out.shape[:-1]) if n > 1):
+        raise ValueError("out's rows have to lie apart, each of neighbouring elements from a 16-byte boundary on")
+    if any(t is not None and overlap(out, t) for t in inputs):
+        raise ValueError("out may not lie among the inputs")
+    return out
+
+
+def _scores(dim: int, heads: int, device, scale, softcap, window, slopes, causal):
+    """The bn_scores of a call, and the slopes that it points at."""
+    if softcap is not None and not (softcap > 0 and math.isfinite(softcap)):
+        raise ValueError("softcap has to be a positive number")
+    if window is not None and not 1 <= window < 1 << 30:
+        raise ValueError("window has to be at least 1")
+    if scale is not None and not math.isfinite(scale):
+        raise ValueError("scale has to be a finite number")
+    slopes = _numbers(slopes, "slopes", heads, device, torch.float32)
+    return _native.Scores(1.0 / math.sqrt(dim) if scale is None else scale, softcap or 0.0, window or 0, ck._p(slopes), int(bool(causal))), slopes
+
+
+def _device(t) -> torch.device:
+    dev = ck.require_cuda()
+    if not isinstance(t, torch.Tensor) or t.device != dev:
+        raise ValueError(f"q has to be a tensor on the current device, {dev}")
+    return dev
+
+
+def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets: torch.Tensor | None = None, *, causal: bool = True, scale: float | None = None, softcap: float | None = None, window: int | None = None, slopes: torch.Tensor | None = None, prefix: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Softmax attention of packed prompts: q [T, heads, D], k and v [T, kv_heads, D] bfloat16 (views of a fused
+    projection's output are read in place), D 64, 128 or 256, heads a multiple of kv_heads -> [T, heads, D].
+
+    offsets: rising whole numbers [documents + 1] on the device: tokens offsets[n] .. offsets[n + 1] - 1 are
+    document n, and queries see keys of their own document only (None: one document). Rows of tokens in no
+    document come back as zeros, or, with `out` given, stay as they are. causal: a query sees no key behind
+    it, but for the first prefix[n] of its document n. window: only keys at a distance below it. scale
+    defaults to 1 / sqrt(D). Nothing is read on the host: the call can be captured in a graph."""
+    dev = _device(q)
+    q = _rows(q, "q", 3, dev)
+    T, heads, D = q.shape
+    k, v = _rows(k, "k", 3, dev), _rows(v, "v", 3, dev)
+    kv = k.shape[1]
+    if D not in HEAD_DIMS or k.shape != (T, kv, D) or v.shape != k.shape or kv < 1 or heads < 1 or heads % kv:
+        raise ValueError(f"q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}: heads of 64, 128 or 256, query heads a multiple of key heads, the same tokens")
+    docs = 1
+    if offsets is not None:
+        if not isinstance(offsets, torch.Tensor) or offsets.numel() < 1:
+            raise ValueError("offsets has to be a tensor of documents + 1 whole numbers")
+        docs = offsets.numel() - 1
+        offsets = _numbers(offsets, "offsets", docs + 1, dev)
+    prefix = _numbers(prefix, "prefix", docs, dev)
+    scores, slopes = _scores(D, heads, dev, scale, softcap, window, slopes, causal)
+    y = _out(out, q, dev, q, k, v)
+    if T:
+        ck._call("bn_attention", ck._p(q), *_steps(q), ck._p(k), *_steps(k), ck._p(v), *_steps(v), T, heads, kv, D, ck._p(offsets), docs, ck._p(prefix), ctypes.byref(scores), ck._p(y), *_steps(y), int(out is None))
+    return y
+
+
+class KV8Cache:
+    """Keys and values of `batch` sequences in `layers` layers, 8 bits a value: codes with one fp32 scale for each
+    block of `block` tokens and head ("int8": amax / 127; "e4m3": a power of two). The tokens of a block that is
+    not full yet stay in BF16 until it is, so what is held does not depend on how the tokens came.
+    NaN is stored as 0 and an infinity as the largest code.
+
+    A step of a model: for every layer `attend(layer, q, k, v)` (or `append` and later `attend`), then
+    one `advance`. `length` (int32 [batch], on the device) is what each sequence holds; setting a sequence's to 0
+    frees its place. Calls on one cache are ordered by the stream that they share."""
+
+    def __init__(self, layers: int, batch: int, kv_heads: int, head_dim: int, max_seq: int, kind: str = "int8", block: int = 32, device=None):
+        if min(layers, batch, kv_heads, max_seq) < 1 or batch > 65535 or kv_heads > 65535 or max_seq >= 1 << 30:
+            raise ValueError("layers, batch, kv_heads and max_seq have to be positive (batch and kv_heads below 65536, max_seq below 2^30)")
+        if head_dim not in HEAD_DIMS or block not in BLOCKS or kind not in KINDS:
+            raise ValueError(f"head_dim {head_dim} (64, 128, 256), block {block} (16, 32, 64), kind {kind!r} (int8, e4m3)")
+        dev = ck.require_cuda() if device is None else torch.device(device)
+        if dev.type != "cuda":
+            raise ValueError(f"the cache lives on a CUDA device, not {dev}")
+        self.device = dev if dev.index is not None else ck.require_cuda()
+        self.layers, self.batch, self.kv_heads, self.head_dim, self.max_seq, self.kind, self.block = layers, batch, kv_heads, head_dim, max_seq, kind, block
+        rows = -(-max_seq // 64) * 64
+        new = lambda *shape, dtype: torch.zeros((layers, batch, kv_heads, *shape), dtype=dtype, device=self.device)  # noqa: E731
+        self.k, self.v = new(rows, head_dim, dtype=torch.uint8), new(rows, head_dim, dtype=torch.uint8)
+        self.k_scale, self.v_scale = new(rows // block, dtype=torch.float32), new(rows // block, dtype=torch.float32)
+        self.k_tail, self.v_tail = new(2, block, head_dim, dtype=torch.bfloat16), new(2, block, head_dim, dtype=torch.bfloat16)
+        self.length, self._side = torch.zeros(batch, dtype=torch.int32, device=self.device), torch.zeros(batch, dtype=torch.int32, device=self.device)
+        self._structs = [_native.KV8Struct(*(t[i].data_ptr() for t in (self.k, self.v, self.k_scale, self.v_scale, self.k_tail, self.v_tail)), self.length.data_ptr(), self._side.data_ptr(), batch, kv_heads, rows, head_dim, max_seq, block, KINDS[kind]) for i in range(layers)]
+
+    def bytes(self) -> int:
+        """Device memory of the cache."""
+        return sum(t.numel() * t.element_size() for t in (self.k, self.v, self.k_scale, self.v_scale, self.k_tail, self.v_tail, self.length, self._side))
+
+    def _layer(self, layer: int):
+        if not 0 <= layer < self.layers:
+            raise ValueError(f"layer {layer} of {self.layers}")
+        if torch.cuda.current_device() != self.device.index:
+            raise ValueError(f"the cache is on {self.device}, the current device is another one")
+        return ctypes.byref(self._structs[layer])
+
+    def _new(self, t, name: str, heads: int | None = None) -> torch.Tensor:
+        t = _rows(t, name, 4, self.device)
+        if t.shape[0] != self.batch or t.shape[3] != self.head_dim or (heads is not None and t.shape[2] != heads):
+            raise ValueError(f"{name} {tuple(t.shape)}: [batch {self.batch}, tokens, {'heads' if heads is None else heads}, {self.head_dim}] expected")
+        return t
+
+    def append(self, layer: int, k: torch.Tensor, v: torch.Tensor, counts: torch.Tensor | None = None) -> None:
+        """New tokens k, v [batch, tokens, kv_heads, D] bfloat16 behind what the sequences hold; counts (whole
+        numbers [batch] on the device): how many of each sequence's are real, the first ones (None: all).
+        `length` stays until `advance`: until then a second append writes the same places again. Tokens
+        beyond max_seq are dropped, and bn_device_status tells (bits 24..27)."""
+        at = self._layer(layer)
+        k, v = self._new(k, "k", self.kv_heads), self._new(v, "v", self.kv_heads)
+        if k.shape != v.shape:
+            raise ValueError(f"k {tuple(k.shape)} and v {tuple(v.shape)} differ")
+        counts = _numbers(counts, "counts", self.batch, self.device)
+        if k.shape[1]:
+            ck._call("bn_kv8_append", at, ck._p(k), *_steps(k), ck._p(v), *_steps(v), k.shape[1], ck._p(counts))
+
+    def attend(self, layer: int, q: torch.Tensor, k: torch.Tensor | None = None, v: torch.Tensor | None = None, counts: torch.Tensor | None = None, *, causal: bool = True, scale: float | None = None, softcap: float | None = None, window: int | None = None, slopes: torch.Tensor | None = None, prefix: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+        """Attention of new tokens q [batch, tokens, heads, D] bfloat16 over what their sequences hold and
+        themselves -> [batch, tokens, heads, D]. With k and v the tokens are appended first; without, an `append`
+        before did it. Query t of sequence b has position length[b] + t and sees the keys up to itself (all
+        length[b] + counts[b] if not causal; options as in `attention`, prefix [batch]). Rows behind a sequence's
+        counts come back as zeros, or, with `out` given, stay as they are."""
+        at = self._layer(layer)
+        q = self._new(q, "q")
+        tokens, heads = q.shape[1], q.shape[2]
+        if heads < 1 or heads % self.kv_heads:
+            raise ValueError(f"{heads} query heads over {self.kv_heads} key heads")
+        if (k is None) != (v is None):
+            raise ValueError("k and v come together")
+        counts = _numbers(counts, "counts", self.batch, self.device)
+        prefix = _numbers(prefix, "prefix", self.batch, self.device)
+        scores, slopes = _scores(self.head_dim, heads, self.device, scale, softcap, window, slopes, causal)
+        y = _out(out, q, self.device, q, k, v)
+        if k is not None:
+            if k.dim() != 4 or k.shape[1] != tokens:
+                raise ValueError(f"k {tuple(k.shape)} for {tokens} tokens")
+            self.append(layer, k, v, counts)
+        if tokens:
+            need = _native.load("cuda").bn_kv8_workspace(at, tokens, heads)
+            work = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
+            ck._call("bn_kv8_attend", at, ck._p(q), *_steps(q), tokens, heads, ck._p(counts), ck._p(prefix), ctypes.byref(scores), ck._p(y), *_steps(y), int(out is None), ck._p(work), need)
+        return y
+
+    def advance(self, n) -> None:
+        """Moves `length` on by n tokens (a number, or whole numbers [batch] on the device), within 0 .. max_seq.
+        Fewer than were appended may be kept (a draft whose end is rejected), and a sequence may go back, as
+        long as the new length lies in the block that was open before, in the one that is open behind all
+        the tokens, or on a border of blocks."""
+        at = self._layer(0)
+        counts = _numbers(n, "n", self.batch, self.device) if isinstance(n, torch.Tensor) else None
+        ck._call("bn_kv8_advance", at, 0 if counts is not None else n, ck._p(counts))
+
+    def dense(self, layer: int):
+        """What the layer holds as the values that its codes stand for: (K, V) float32 [batch, kv_heads,
+        max_seq, D], zeros behind each sequence's length."""
+        at = self._layer(layer)
+        k, v = (torch.empty((self.batch, self.kv_heads, self.max_seq, self.head_dim), dtype=torch.float32, device=self.device) for _ in range(2))
+        ck._call("bn_kv8_dense", at, ck._p(k), ck._p(v))
+        return k, v

@@ -279,6 +279,109 @@ int bn_moe_route(const void *ids, int ids64, int64_t G, int64_t k, int64_t E, ui
  * fp32 with one rounding. */
 int bn_swiglu(const uint16_t *gate, const uint16_t *up, int64_t n, uint16_t *h, void *stream);
 
+/* ---- Attention. The reference leaves attention to its host framework: these have no counterpart there.
+ * A score is s = scale q.k, s = softcap tanh(s / softcap) if softcap > 0, s -= slopes[head] |i - j| if
+ * slopes; i and j are positions in the document (or sequence) of L keys. Query i sees the keys
+ *   max(0, i - window + 1) <= j < min(L, i + window, causal ? max(i + 1, prefix) : L)   (window 0: no limit)
+ * and its output is the softmax over their scores times their values. Sums are kept in fp32. */
+typedef struct bn_scores {
+  float scale;
+  float softcap;       /* 0: none */
+  int64_t window;      /* 0: none */
+  const float *slopes; /* [query heads] or NULL */
+  int causal;
+} bn_scores;
+
+/* Attention of packed prompts: q [T, heads, D], k and v [T, kv_heads, D], out [T, heads, D] in BF16, a row
+ * (token, head) at token * x_token + head * x_head elements (both multiples of 8, arrays on 16 bytes). Query
+ * head h reads key head h / (heads / kv_heads). D is 64, 128 or 256. Tokens offsets[n] .. offsets[n+1] - 1
+ * are document n of `docs` (offsets: docs + 1 rising int32; NULL: one document of T tokens), and no
+ * query sees another document's keys. prefix [docs] (or NULL): the first keys of each document, which its
+ * queries see wherever they are. Rows of tokens in no document are zeroed if zero_rest, else left as they are. */
+int bn_attention(const uint16_t *q, int64_t q_token, int64_t q_head, const uint16_t *k, int64_t k_token,
+                 int64_t k_head, const uint16_t *v, int64_t v_token, int64_t v_head, int64_t T, int64_t heads,
+                 int64_t kv_heads, int64_t D, const int32_t *offsets, int64_t docs, const int32_t *prefix,
+                 const bn_scores *scores, uint16_t *out, int64_t o_token, int64_t o_head, int zero_rest,
+                 void *stream);
+
+/* A key/value cache in 8 bits with a scale for each block of tokens and head:
+ *   k, v       [batch, kv_heads, rows, D] codes of the full blocks; rows: max_seq rounded up to 64
+ *   k_scale,   [batch, kv_heads, rows / block]: a value is its code times the scale of its block
+ *   v_scale
+ *   k_tail,    [batch, kv_heads, 2, block, D] BF16: the tokens of the block that is not full yet. What a
+ *   v_tail     cache holds does not depend on how the tokens came: a block is coded once, when full. Of the
+ *              two slots, `side` names the one of the block that is open at `length`; if new tokens
+ *              fill that block, the next open one goes to the other slot, and the first stays as it is
+ *   length,    [batch] tokens held, and the slot; bn_kv8_advance moves both on. Appending again before
+ *   side       that writes the same places again
+ * int8: scale = max(amax / 127, 2^-100), code = x / scale rounded to nearest even. e4m3: scale = the least
+ * power of two with amax <= 448 scale, at least 2^-100. amax is over the block's finite values; NaN is
+ * stored as 0 and an infinity as the largest code (the tail holds them as they are). block is 16, 32 or 64. */
+#define BN_KV8_INT8 0
+#define BN_KV8_E4M3 1
+typedef struct bn_kv8 {
+  uint8_t *k, *v;
+  float *k_scale, *v_scale;
+  uint16_t *k_tail, *v_tail;
+  int32_t *length, *side;
+  int64_t batch, kv_heads, rows, D, max_seq;
+  int block, kind;
+} bn_kv8;
+
+/* Up to `tokens` new tokens of every sequence, of which counts[b] are real (NULL: all), written behind the
+ * length[b] that it holds; rows k, v (sequence, token, head) in BF16. Tokens that do not fit in max_seq are dropped, and
+ * the device status says so (bits 24..30). */
+int bn_kv8_append(const bn_kv8 *c, const uint16_t *k, int64_t k_seq, int64_t k_token, int64_t k_head,
+                  const uint16_t *v, int64_t v_seq, int64_t v_token, int64_t v_head, int64_t tokens,
+                  const int32_t *counts, void *stream);
+
+/* Attention of those tokens over everything up to themselves, after they were appended and before `length`
+ * moves on: query t of sequence b has position length[b] + t, its keys are the length[b] + counts[b] first.
+ * prefix [batch] or NULL. Rows of tokens that are not real are zeroed if zero_rest, else left as they are.
+ * workspace: bn_kv8_workspace bytes on 16 bytes, for this call alone. */
+uint64_t bn_kv8_workspace(const bn_kv8 *c, int64_t tokens, int64_t heads);
+int bn_kv8_attend(const bn_kv8 *c, const uint16_t *q, int64_t q_seq, int64_t q_token, int64_t q_head,
+                  int64_t tokens, int64_t heads, const int32_t *counts, const int32_t *prefix,
+                  const bn_scores *scores, uint16_t *out, int64_t o_seq, int64_t o_token, int64_t o_head,
+                  int zero_rest, void *workspace, uint64_t workspace_bytes, void *stream);
+
+/* length moves on by n (counts NULL) or counts[b] tokens, within 0 .. max_seq: after the last layer of a step, by
+ * all the tokens that were appended, or by fewer (a draft whose end is rejected), as long as the new length lies in the block that
+ * was open before, in the one open behind all of them, or on a border of blocks. */
+int bn_kv8_advance(const bn_kv8 *c, int64_t n, const int32_t *counts, void *stream);
+
+/* What the cache holds, as the values that the codes stand for: k, v [batch, kv_heads, max_seq, D] fp32,
+ * zeros behind a sequence's length. */
+int bn_kv8_dense(const bn_kv8 *c, float *k, float *v, void *stream);
+
+/* ---- Logits. Tokens [batch, n] (int64 if tokens64, else int32; rows row_step apart; lengths [batch] real ones
+ * a row, or NULL) set their bits in seen [batch, ceil(V / 32)] and, unless prompt, add to counts [batch, V];
+ * a token outside 0 .. V-1 is passed over. seen_row and counts_row: elements between rows. */
+int bn_token_counts(const void *tokens, int tokens64, int64_t row_step, int64_t batch, int64_t n,
+                    const int32_t *lengths, int64_t V, int prompt, uint32_t *seen, int64_t seen_row,
+                    int32_t *counts, int64_t counts_row, void *stream);
+
+/* Per row: penalties of the tokens that were seen (repetition: x / r for x > 0, else x r; then, of those that
+ * were counted, x -= frequency count + presence), then the bias [V] (bias_row 0: one for all rows), then -inf
+ * where the mask's bit (ceil(V / 32) words a row; mask_row 0: one for all) is clear. Each operation rounds
+ * to fp32 in this order. A penalty is a device array [batch], or with NULL the value behind it. */
+typedef struct bn_logit_rules {
+  const uint32_t *seen; /* or NULL: no penalties */
+  const int32_t *counts;
+  int64_t seen_row, counts_row;
+  const float *repetition, *presence, *frequency;
+  float repetition_all, presence_all, frequency_all;
+  const float *bias;
+  int64_t bias_row;
+  const uint32_t *mask;
+  int64_t mask_row;
+} bn_logit_rules;
+
+/* x [batch, V] (fp32 or BF16) -> out [batch, V] fp32 under the rules, and token [batch]: the lowest index of
+ * the row's largest value, -1 if no value is above -inf (NaN is never chosen). out may be x (fp32). */
+int bn_logits(const void *x, int fp32, int64_t x_row, int64_t batch, int64_t V, const bn_logit_rules *rules,
+              float *out, int64_t out_row, int64_t *token, void *stream);
+
 /* All-gather of small slices over NVLink peer memory, one kernel per rank (multi-GPU form of the
  * hook; the reference is single-device, so there is no counterpart). Every rank calls it with
  * 1..4 segments (one per projection): `locals[g]` is this rank's slice of segment g, `bytes[g]`
@@ -308,7 +411,7 @@ int bn_push_gather_beside(const void *const *locals, const uint64_t *bytes, int 
 
 /* Device-side status of the calling thread's current device: 0, or non-zero once a kernel of
  * this library gave up a bounded wait or refused a launch whose shared-memory window did not
- * match (its output is then incomplete): bits 0..7 the batch-1 matvec kernels, bits 8..15 the tensor-core GEMM, bits 16..23 the peer exchange. Every wait inside the
+ * match (its output is then incomplete): bits 0..7 the batch-1 matvec kernels, bits 8..15 the tensor-core GEMM, bits 16..23 the peer exchange, bits 24..30 tokens that a key/value cache had no room for. Every wait inside the
  * kernels is bounded, so a lost copy or an absent peer ends in this status instead of a hang.
  * Synchronises with the device. No counterpart in the reference. */
 int bn_device_status(int *status);

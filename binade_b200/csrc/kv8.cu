@@ -18,7 +18,7 @@ __device__ __forceinline__ uint32_t int8_code(float x, float scale) {
     if (r < 0.0f) q = floorf(t);
   }
   q = fminf(fmaxf(q, -127.0f), 127.0f);
-  return x == x ? (uint32_t)(int)q & 0xFFu : 0u;
+  return x == x ? (uint32_t)((int)q + 128) : 128u;  // stored with 128 added
 }
 
 // Least power of two, at least 2^-100, times which 448 (the largest e4m3 value) is not below amax.

@@ -26,7 +26,7 @@ __device__ __forceinline__ int kv8_slot(const bn_kv8 &c, int64_t b, int held, in
 template <int KIND>
 __device__ __forceinline__ float kv8_code(uint32_t byte) {
   if constexpr (KIND == KV8_INT8) {
-    return (float)(int8_t)byte;
+    return (float)((int)byte - 128);
   } else {
     __nv_fp8_e4m3 f;
     f.__x = (__nv_fp8_storage_t)byte;

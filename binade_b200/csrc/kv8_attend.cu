@@ -1,8 +1,35 @@
-// Attention of new tokens over an 8-bit key/value cache (bn_kv8).
+// Attention of new tokens over an 8-bit key/value cache (bn_kv8): for the few query rows that share a key head
+// (a token or a short draft times the head's group), bound by reading the cache once.
+//
+// The rows are the M of mma.sync m16n8k16 (16 or 32 rows a block, f16 operands, fp32 sums): a
+// decode step has 1 to 32 of them, which tcgen05's tiles of 64 and 128 rows would leave empty, and
+// at one byte a value the legacy tensor path has the rate to spare.
+//   codes -> f16   exact (8 bits fit f16's 11): int8 codes, stored as code + 128, become 1024 + byte by one byte
+//                  permute and lose the 1152 by one subtraction; e4m3 converts in hardware
+//   queries        to f16 after a power of two per row that puts its largest value in [1, 2): exact down to
+//                  2^-24 of that value, below which a product does not show in an fp32 sum of scores
+//   scores         K's scale multiplies the sum; V's scale 2^v goes into the exponent: p' = 2^(s + v - m + 15), m
+//                  the running maximum of s + v, so p' fits f16 (rounded to 11 bits, 2^-12) however far apart
+//                  the blocks' scales lie, and the sum of weights takes p' / 2^v, in fp32
+//   order of k     a dot product may take its dimensions, and the sum over keys its keys, in any order: each
+//                  thread reads 16 neighbouring bytes of a key (of four keys for V) and calls them the
+//                  elements that the fragments want
+// A warp streams its own keys through a cp.async ring of its own: no barrier in the loop; the warps of a block
+// are joined at the end. The work is the tiles of all sequences and heads in a row, cut into equal
+// shares: sequences of unequal lengths load the SMs alike, and one long one spreads over all of them. A sequence and head
+// that is cut leaves partial sums, joined by a second kernel.
+//
+// Figures: at attend_launch.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
 #include "kv8.cuh"
 
 namespace bn {
 namespace {
+
+constexpr int WARPS = 4;
+constexpr float HEADROOM = 15.0f;  // weights reach 2^15: f16 holds them to 11 bits over 29 binades, and to 2^-39 of the largest below
 
 struct AttendArgs {
   bn_kv8 c;
@@ -11,84 +38,678 @@ struct AttendArgs {
   int64_t q_seq, q_token, q_head, o_seq, o_token, o_head;  // elements
   const int32_t *counts, *prefix;
   const float *slopes;
-  int tokens, heads;
+  int tokens, heads, group;  // group: query heads of a key head
   int window, causal, zero_rest;
   float scale, cap;
+  // workspace: tiles before each sequence [batch + 1], the share of a block; then partial results, two slots a block
+  int64_t *plan;
+  float *parts;
+  int row_groups;
+  int blocks;
 };
 
-// One query of one head by a warp, keys one after the other; a lane has E = D / 32 neighbouring dimensions.
-template <int D, int KIND>
-__global__ void __launch_bounds__(128) attend_rows_kernel(const __grid_constant__ AttendArgs a) {
-  constexpr int E = D / 32;
-  const bn_kv8 &c = a.c;
-  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-  if (row >= c.batch * a.tokens * a.heads) return;
-  const int head = (int)(row % a.heads), t = (int)(row / a.heads % a.tokens);
-  const int64_t b = row / a.heads / a.tokens;
-  const uint32_t lane = lane_id();
-  int held, brought;
-  kv8_tokens(c, a.counts, a.tokens, b, held, brought);
-  uint16_t *const out = a.out + b * a.o_seq + t * a.o_token + head * a.o_head + lane * E;
-  if (t >= brought) {
-    if (a.zero_rest)
-      for (int e = 0; e < E; e++) out[e] = 0;
+template <int D, int MT>
+struct Shape {
+  static constexpr int ROWS = 16 * MT;                 // query rows of a block
+  static constexpr int KS = D == 64 ? 32 : 16;         // keys of a warp's stage
+  static constexpr int TILE = KS * WARPS;              // keys of a block's step
+  static constexpr int STAGES = D == 256 ? 3 : 4;
+  static constexpr int STAGE_BYTES = 2 * KS * D;
+  static constexpr int NT = D / 8;                     // n8 tiles of the output
+  static constexpr int RING = WARPS * STAGES * STAGE_BYTES;
+  static constexpr int JOIN = WARPS * ROWS * (D + 4) * 4;
+  static constexpr int SMEM = RING > JOIN ? RING : JOIN;
+  static constexpr int PART = ROWS * (D + 2);          // floats of a partial result: sums, then maxima and weights
+};
+
+// Tiles of sequence b, its first key and full blocks' end. The last tile is the open block's, if it holds tokens.
+struct Span {
+  int held, brought, L, full, start, quant, tiles;
+};
+__device__ __forceinline__ Span span_of(const AttendArgs &a, int64_t b, int tile) {
+  Span s;
+  kv8_tokens(a.c, a.counts, a.tokens, b, s.held, s.brought);
+  s.L = s.held + s.brought, s.full = s.L / a.c.block * a.c.block, s.start = 0;
+  if (s.brought == 0) {
+    s.quant = s.tiles = 0;
+    return s;
+  }
+  if (a.window > 0) s.start = max(0, s.held - a.window + 1) & ~15;  // the first query looks back furthest
+  s.start = min(s.start, s.full);
+  s.quant = (s.full - s.start + tile - 1) / tile;
+  s.tiles = s.quant + (s.L > s.full);
+  return s;
+}
+
+__device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_bf16x(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+// Two codes, in the low or (HIGH) the high half of a word, as f16.
+template <int KIND, bool HIGH>
+__device__ __forceinline__ uint32_t codes_f16(uint32_t w) {
+  uint32_t r;
+  if constexpr (KIND == KV8_INT8) {
+    r = __byte_perm(w, 0x64646464u, HIGH ? 0x4342 : 0x4140);
+    asm("sub.rn.f16x2 %0, %0, %1;" : "+r"(r) : "r"(0x64806480u));  // 1152
+  } else if constexpr (HIGH) {
+    asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, hi;\n\t}" : "=r"(r) : "r"(w));
+  } else {
+    asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\t}" : "=r"(r) : "r"(w));
+  }
+  return r;
+}
+
+__device__ __forceinline__ void copy16(uint32_t dst, const void *src, bool real) {  // zeros where there is nothing
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copy4(uint32_t dst, const void *src) { asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory"); }
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copies_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ uint4 lds16(uint32_t at) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at));
+  return v;
+}
+__device__ __forceinline__ uint2 lds8(uint32_t at) {
+  uint2 v;
+  asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(at));
+  return v;
+}
+
+// Which 16-byte piece of a key's row in shared memory holds its piece `col`: chosen so that the eight lanes of a
+// 16-byte access meet no bank twice, neither where they read two keys' four pieces (K) nor four keys' two (V).
+template <int D>
+__device__ __forceinline__ uint32_t piece(uint32_t key, uint32_t col) {
+  return D == 64 ? col ^ ((key >> 1) & 3u) : col ^ (((key & 1u) << 2) | (((key >> 1) & 3u) << 1));
+}
+
+// What a warp has so far: sums, running maxima (of s + v, in powers of two) and weights of its lane's rows.
+template <int D, int MT>
+struct State {
+  float o[MT][Shape<D, MT>::NT][4];
+  float m[MT][2], l[MT][2];
+};
+
+// What a lane's rows need: positions, the visible run, the factor from a sum of products to a score.
+template <int MT>
+struct Rows {
+  int i[MT][2], lo[MT][2], hi[MT][2];
+  float factor[MT][2], slope[MT][2];
+};
+
+// The scores of a 16-key piece into weights: x holds the raw sums and gets p'. vlog, vinv: V's scale as a power of
+// two and inverted. Updates maxima and weights, rescales the sums where a maximum rose.
+template <int D, int MT>
+__device__ __forceinline__ void weigh(const AttendArgs &a, float (&x)[MT][2][4], const Rows<MT> &r, State<D, MT> &st, int key0, float kscale, float vlog, float vinv, bool masked, bool scaled_rows) {
+  const uint32_t c = lane_id() & 3u;
+#pragma unroll
+  for (int mt = 0; mt < MT; mt++) {
+    float top[2];
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+      top[h] = st.m[mt][h];
+      const float f = scaled_rows ? r.factor[mt][h] : a.cap > 0.0f ? a.scale * (2.0f * LOG2E / a.cap) : a.scale * LOG2E;
+#pragma unroll
+      for (int j = 0; j < 2; j++)
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+          float &v = x[mt][j][2 * h + e];
+          const int key = key0 + 8 * j + 2 * (int)c + e;
+          v = v * kscale * f;
+          if (a.cap > 0.0f) v = capped(v, a.cap * LOG2E);
+          if (a.slopes) v = fmaf(-r.slope[mt][h], (float)abs(r.i[mt][h] - key), v);
+          v += vlog;
+          if (masked && (key < r.lo[mt][h] || key >= r.hi[mt][h])) v = -CUDART_INF_F;
+          top[h] = fmaxf(top[h], v);
+        }
+      top[h] = fmaxf(top[h], __shfl_xor_sync(BN_FULL, top[h], 1));
+      top[h] = fmaxf(top[h], __shfl_xor_sync(BN_FULL, top[h], 2));
+    }
+    if (__any_sync(BN_FULL, top[0] > st.m[mt][0] || top[1] > st.m[mt][1])) {
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        const float keep = top[h] > st.m[mt][h] ? ex2(st.m[mt][h] - top[h]) : 1.0f;
+        st.m[mt][h] = top[h], st.l[mt][h] *= keep;
+#pragma unroll
+        for (int t = 0; t < Shape<D, MT>::NT; t++) st.o[mt][t][2 * h] *= keep, st.o[mt][t][2 * h + 1] *= keep;
+      }
+    }
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+      const float base = top[h] == -CUDART_INF_F ? 0.0f : top[h] - HEADROOM;  // nothing visible yet: weights of 0
+      float sum = 0.0f;
+#pragma unroll
+      for (int j = 0; j < 2; j++)
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+          float &v = x[mt][j][2 * h + e];
+          v = ex2(v - base);
+          sum += v;
+        }
+      st.l[mt][h] = fmaf(sum, vinv, st.l[mt][h]);
+    }
+  }
+}
+
+// The dimension of n8 tile t's column n.
+template <int D>
+__device__ __forceinline__ constexpr int dim_of(int t, int n) {
+  return D == 64 ? 8 * n + t : 128 * (t / 16) + 16 * n + t % 16;
+}
+
+// The open block's 16 tokens from `key0` on, in BF16. Weights go in two BF16 halves (hi + lo: 2^-17), values times 2^-23
+// with 2^23 in the weights' exponent, so that no sum of 63 of them passes fp32. Where a value is not finite, a
+// weight of zero must not touch it: those go one by one.
+template <int D, int MT>
+__device__ void open_block(const AttendArgs &a, const uint16_t *const (&qrow)[MT][2], const uint16_t *ktail, const uint16_t *vtail, int full, int L, int key0, const Rows<MT> &r, State<D, MT> &st) {
+  const uint32_t lane = lane_id(), n = lane >> 2, c = lane & 3u;
+  const int last = L - 1 - full, at = key0 - full;  // the last token's row, this piece's first
+  float x[MT][2][4] = {};
+  const uint16_t *k[2];
+#pragma unroll
+  for (int j = 0; j < 2; j++) k[j] = ktail + (int64_t)min(at + 8 * j + (int)n, last) * D + 16 * c;
+#pragma unroll 1
+  for (int g = 0; g < D / 64; g++)
+#pragma unroll
+    for (int w = 0; w < 4; w++) {
+      const uint2 k0 = *reinterpret_cast<const uint2 *>(k[0] + 64 * g + 4 * w), k1 = *reinterpret_cast<const uint2 *>(k[1] + 64 * g + 4 * w);
+#pragma unroll
+      for (int mt = 0; mt < MT; mt++) {
+        uint2 q[2] = {};
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+          if (qrow[mt][h]) q[h] = *reinterpret_cast<const uint2 *>(qrow[mt][h] + 64 * g + 16 * c + 4 * w);
+        const uint32_t f[4] = {q[0].x, q[1].x, q[0].y, q[1].y};
+        mma_bf16x(x[mt][0], f, k0.x, k0.y);
+        mma_bf16x(x[mt][1], f, k1.x, k1.y);
+      }
+    }
+  weigh<D, MT>(a, x, r, st, key0, 1.0f, 23.0f, 1.0f / (1 << 23), true, false);
+  uint32_t hi[MT][4], lo[MT][4];
+#pragma unroll
+  for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+    for (int f = 0; f < 4; f++) {
+      const float p0 = x[mt][f >> 1][2 * (f & 1)], p1 = x[mt][f >> 1][2 * (f & 1) + 1];
+      hi[mt][f] = pack_bf16(p0, p1);
+      lo[mt][f] = pack_bf16(p0 - __uint_as_float(hi[mt][f] << 16), p1 - __uint_as_float(hi[mt][f] & 0xFFFF0000u));
+    }
+  const uint16_t *v[4];
+  bool odd = false;
+#pragma unroll
+  for (int i = 0; i < 4; i++) v[i] = vtail + (int64_t)min(at + 8 * (i >> 1) + 2 * (int)c + (i & 1), last) * D;
+#pragma unroll
+  for (int t = 0; t < Shape<D, MT>::NT; t += 2) {
+    uint32_t w[4];  // dims dim_of(t, n) and the next
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      w[i] = *reinterpret_cast<const uint32_t *>(v[i] + dim_of<D>(t, (int)n));
+      odd |= (w[i] & 0x7F80u) == 0x7F80u || (w[i] & 0x7F800000u) == 0x7F800000u;
+    }
+  }
+  if (!__any_sync(BN_FULL, odd)) {
+#pragma unroll
+    for (int t = 0; t < Shape<D, MT>::NT; t += 2) {
+      uint32_t w[4];
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        w[i] = *reinterpret_cast<const uint32_t *>(v[i] + dim_of<D>(t, (int)n));
+        asm("mul.rn.bf16x2 %0, %0, %1;" : "+r"(w[i]) : "r"(0x34003400u));  // 2^-23
+      }
+#pragma unroll
+      for (int e = 0; e < 2; e++) {
+        const uint32_t b0 = __byte_perm(w[0], w[1], e ? 0x7632 : 0x5410), b1 = __byte_perm(w[2], w[3], e ? 0x7632 : 0x5410);
+#pragma unroll
+        for (int mt = 0; mt < MT; mt++) {
+          mma_bf16x(st.o[mt][t + e], hi[mt], b0, b1);
+          mma_bf16x(st.o[mt][t + e], lo[mt], b0, b1);
+        }
+      }
+    }
     return;
   }
-  const int L = held + brought, i = held + t, kv = head / (a.heads / (int)c.kv_heads), full = L / c.block * c.block;
-  const int64_t unit = b * c.kv_heads + kv;
-  const int slot = kv8_slot(c, b, held, L / c.block);
-  int lo, hi;
-  visible_keys(i, L, a.prefix ? a.prefix[b] : 0, a.window, a.causal, lo, hi);
-  float q[E], o[E] = {}, m = -CUDART_INF_F, l = 0.0f;
-  for (int e = 0; e < E; e++) q[e] = bf16_to_f32(a.q[b * a.q_seq + t * a.q_token + head * a.q_head + lane * E + e]);
-  const float slope = a.slopes ? a.slopes[head] * LOG2E : 0.0f;
-  auto value = [&](const uint8_t *codes, const float *scales, const uint16_t *tail, int j, int e) {
-    if (j < full) return kv8_code<KIND>(codes[(unit * c.rows + j) * D + lane * E + e]) * scales[unit * (c.rows / c.block) + j / c.block];
-    return bf16_to_f32(tail[((unit * 2 + slot) * c.block + j - full) * D + lane * E + e]);
-  };
-  auto score = [&](int j) {
-    float dot = 0.0f;
-    for (int e = 0; e < E; e++) dot = fmaf(q[e], value(c.k, c.k_scale, c.k_tail, j, e), dot);
 #pragma unroll
-    for (int d = 16; d; d >>= 1) dot += __shfl_xor_sync(BN_FULL, dot, d);
-    float s = dot * a.scale;
-    s = a.cap > 0.0f ? capped(s * (2.0f * LOG2E / a.cap), a.cap * LOG2E) : s * LOG2E;
-    return s - slope * (float)abs(i - j);
-  };
-  for (int j = lo; j < hi; j++) {
-    const float s = score(j), top = fmaxf(m, s);
-    l = fmaf(l, ex2(m - top), ex2(s - top));
-    m = top;
+  for (int key = 0; key < 16; key++) {
+    const uint16_t *const row = vtail + (int64_t)min(at + key, last) * D;
+    const uint32_t from = (lane & ~3u) | ((key & 7) >> 1);
+#pragma unroll
+    for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        const float p = __shfl_sync(BN_FULL, x[mt][key >> 3][2 * h + (key & 1)], from);
+        if (p != 0.0f)
+#pragma unroll
+          for (int t = 0; t < Shape<D, MT>::NT; t++)
+#pragma unroll
+            for (int e = 0; e < 2; e++) st.o[mt][t][2 * h + e] = fmaf(p, bf16_to_f32(row[dim_of<D>(t, 2 * (int)c + e)]) * (1.0f / (1 << 23)), st.o[mt][t][2 * h + e]);
+      }
   }
-  const float inv = 1.0f / l;
-  for (int j = lo; j < hi; j++) {
-    const float p = ex2(score(j) - m) * inv;
-    for (int e = 0; e < E; e++) o[e] = fmaf(p, value(c.v, c.v_scale, c.v_tail, j, e), o[e]);
-  }
-  for (int e = 0; e < E; e++) out[e] = f32_to_bf16_bits(o[e]);
 }
+
+template <int D, int KIND, int MT>
+__global__ void __launch_bounds__(WARPS * 32, (D == 64 && MT == 1) ? 4 : (MT * D <= 128) ? 3 : 2) attend_kernel(const __grid_constant__ AttendArgs a) {
+  using S = Shape<D, MT>;
+  constexpr int NT = S::NT;
+  extern __shared__ __align__(128) uint8_t attend_smem[];
+  __shared__ int64_t found[2];
+  __shared__ int64_t warp_tiles[WARPS];
+  __shared__ float join_m[WARPS][S::ROWS], join_l[WARPS][S::ROWS];
+  __shared__ float scales[WARPS][S::STAGES][2][S::KS / 16];
+  const uint32_t lane = lane_id(), warp = threadIdx.x >> 5, n = lane >> 2, c = lane & 3u;
+  const bn_kv8 &cache = a.c;
+  const int per_seq = (int)cache.kv_heads * a.row_groups;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+
+  // ---- this block's share of the tiles: every thread counts those of a run of sequences
+  const int per_thread = (int)((cache.batch + WARPS * 32 - 1) / (WARPS * 32));
+  const int64_t b_from = min((int64_t)threadIdx.x * per_thread, cache.batch), b_to = min(b_from + per_thread, cache.batch);
+  int64_t mine = 0;
+  for (int64_t b = b_from; b < b_to; b++) mine += span_of(a, b, S::TILE).tiles;
+  int64_t upto = mine;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int64_t o = __shfl_up_sync(BN_FULL, upto, d);
+    if (lane >= (uint32_t)d) upto += o;
+  }
+  if (lane == 31) warp_tiles[warp] = upto;
+  __syncthreads();
+  int64_t before = upto - mine, total = 0;
+#pragma unroll
+  for (int w = 0; w < WARPS; w++) {
+    if (w < (int)warp) before += warp_tiles[w];
+    total += warp_tiles[w];
+  }
+  const int64_t share = max((total * per_seq + a.blocks - 1) / a.blocks, (int64_t)1);
+  int64_t x = (int64_t)blockIdx.x * share;
+  const int64_t x_end = min(x + share, total * per_seq);
+  for (int64_t b = b_from, at = before; b < b_to; b++) {
+    const int tiles = span_of(a, b, S::TILE).tiles;
+    if (blockIdx.x == 0) a.plan[b] = at;
+    if (x >= at * per_seq && x < (at + tiles) * per_seq) found[0] = b, found[1] = at;
+    at += tiles;
+  }
+  if (blockIdx.x == 0 && threadIdx.x == 0) a.plan[cache.batch] = total, a.plan[cache.batch + 1] = share;
+  __syncthreads();
+  if (x >= x_end) return;
+  int64_t b = found[0];
+  Span s = span_of(a, b, S::TILE);
+  int hr, tile;  // head and row group, tile inside it
+  {
+    const int64_t rest = x - found[1] * per_seq;
+    hr = (int)(rest / s.tiles), tile = (int)(rest % s.tiles);
+  }
+  const uint32_t ring = smem_addr(attend_smem) + warp * (S::STAGES * S::STAGE_BYTES);
+  bool first = true;
+
+  while (true) {
+    const int kv = hr / a.row_groups, row0 = hr % a.row_groups * S::ROWS;
+    const int rows = min(S::ROWS, a.group * a.tokens - row0);
+    const int64_t unit = b * cache.kv_heads + kv;
+    const int tile_end = (int)min((int64_t)s.tiles, tile + (x_end - x));
+    const uint8_t *const codes[2] = {cache.k + unit * cache.rows * D, cache.v + unit * cache.rows * D};
+    const int64_t scale_at = unit * (cache.rows / cache.block);
+
+    auto issue = [&](int t, int slot) {  // this warp's keys of tile t
+      if (t < min(tile_end, s.quant)) {
+        const int key0 = s.start + t * S::TILE + (int)warp * S::KS;
+        const uint32_t to = ring + slot * S::STAGE_BYTES;
+#pragma unroll
+        for (int side = 0; side < 2; side++)
+#pragma unroll
+          for (int i = 0; i < S::KS * D / 512; i++) {
+            const uint32_t q = lane + 32 * i, key = q / (D / 16), col = q % (D / 16);
+            const bool real = key0 + (int)key < s.full;
+            copy16(to + side * (S::KS * D) + key * D + piece<D>(key, col) * 16, codes[side] + (real ? (int64_t)(key0 + (int)key) * D + col * 16 : 0), real);
+          }
+        if (lane < 2 * (S::KS / 16)) {
+          const int side = (int)lane / (S::KS / 16), sub = (int)lane % (S::KS / 16);
+          copy4(smem_addr(&scales[warp][slot][side][sub]), (side ? cache.v_scale : cache.k_scale) + scale_at + min(key0 + 16 * sub, s.full - 1) / cache.block);
+        }
+      }
+      copies_commit();
+    };
+#pragma unroll
+    for (int i = 0; i < S::STAGES - 1; i++) issue(tile + i, i);
+
+    // ---- the rows of this lane: n and n + 8 of each 16
+    const int t_first = row0 / a.group, t_last = min((row0 + rows - 1) / a.group, s.brought - 1);
+    const int prefix = a.prefix ? a.prefix[b] : 0;
+    int lo_most, hi_least, unused;
+    visible_keys(s.held + t_last, s.L, prefix, a.window, a.causal, lo_most, unused);
+    visible_keys(s.held + t_first, s.L, prefix, a.window, a.causal, unused, hi_least);
+    Rows<MT> r;
+    State<D, MT> st;
+    uint32_t q[MT][D / 16][4];
+    const uint16_t *qrow[MT][2];
+#pragma unroll
+    for (int mt = 0; mt < MT; mt++) {
+      uint4 raw[2][D / 64][2];
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        const int row = 16 * mt + 8 * h + (int)n, t = (row0 + row) / a.group, head = kv * a.group + (row0 + row) % a.group;
+        const bool real = row < rows && t < s.brought;
+        qrow[mt][h] = real ? a.q + b * a.q_seq + t * a.q_token + head * a.q_head : nullptr;
+        r.i[mt][h] = s.held + t, r.lo[mt][h] = r.hi[mt][h] = 0;
+        if (real) visible_keys(s.held + t, s.L, prefix, a.window, a.causal, r.lo[mt][h], r.hi[mt][h]);
+        r.slope[mt][h] = real && a.slopes ? a.slopes[head] * LOG2E : 0.0f;
+        st.m[mt][h] = -CUDART_INF_F, st.l[mt][h] = 0.0f;
+        uint32_t most = 0;
+#pragma unroll
+        for (int g = 0; g < D / 64; g++)
+#pragma unroll
+          for (int i = 0; i < 2; i++) {
+            raw[h][g][i] = real ? *reinterpret_cast<const uint4 *>(qrow[mt][h] + 64 * g + 16 * c + 8 * i) : make_uint4(0, 0, 0, 0);
+            const uint32_t u[4] = {raw[h][g][i].x, raw[h][g][i].y, raw[h][g][i].z, raw[h][g][i].w};
+#pragma unroll
+            for (int e = 0; e < 4; e++) most = max(most, max((u[e] << 16) & 0x7FFFFFFFu, u[e] & 0x7FFF0000u));
+          }
+        most = max(most, __shfl_xor_sync(BN_FULL, most, 1));
+        most = max(most, __shfl_xor_sync(BN_FULL, most, 2));
+        const int e = min(max((int)(most >> 23), 1), 253);  // exponent of the row's largest value
+        const float down = __uint_as_float((uint32_t)(254 - e) << 23), up = __uint_as_float((uint32_t)e << 23);
+        r.factor[mt][h] = (a.cap > 0.0f ? a.scale * (2.0f * LOG2E / a.cap) : a.scale * LOG2E) * up;
+#pragma unroll
+        for (int g = 0; g < D / 64; g++)
+#pragma unroll
+          for (int w = 0; w < 4; w++) {
+            const uint4 u = raw[h][g][w >> 1];
+            const uint32_t p0 = w & 1 ? u.z : u.x, p1 = w & 1 ? u.w : u.y;
+            q[mt][4 * g + w][h] = pack_f16(__uint_as_float(p0 << 16) * down, __uint_as_float(p0 & 0xFFFF0000u) * down);
+            q[mt][4 * g + w][2 + h] = pack_f16(__uint_as_float(p1 << 16) * down, __uint_as_float(p1 & 0xFFFF0000u) * down);
+          }
+      }
+#pragma unroll
+      for (int t = 0; t < NT; t++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) st.o[mt][t][e] = 0.0f;
+    }
+
+    // ---- full blocks
+    int slot = 0;
+    const int quant_end = min(tile_end, s.quant);
+    for (int t = tile; t < quant_end; t++) {
+      copies_wait<S::STAGES - 2>();
+      __syncwarp();  // this tile's copies of all lanes are there, and the slot of the tile before is read
+      issue(t + S::STAGES - 1, slot == 0 ? S::STAGES - 1 : slot - 1);
+      const uint32_t at = ring + slot * S::STAGE_BYTES;
+#pragma unroll
+      for (int sub = 0; sub < S::KS / 16; sub++) {
+        const int key0 = s.start + t * S::TILE + (int)warp * S::KS + 16 * sub;
+        if (key0 >= s.full) break;
+        const float kscale = scales[warp][slot][0][sub], vscale = scales[warp][slot][1][sub];
+        float x[MT][2][4] = {};
+#pragma unroll
+        for (int g = 0; g < D / 64; g++)
+#pragma unroll
+          for (int j = 0; j < 2; j++) {
+            const uint32_t key = 16 * sub + 8 * j + n;
+            const uint4 w4 = lds16(at + key * D + piece<D>(key, 4 * g + c) * 16);
+            const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+              const uint32_t b0 = codes_f16<KIND, false>(w[e]), b1 = codes_f16<KIND, true>(w[e]);
+#pragma unroll
+              for (int mt = 0; mt < MT; mt++) mma_f16(x[mt][j], q[mt][4 * g + e], b0, b1);
+            }
+          }
+        float vlog;
+        asm("lg2.approx.f32 %0, %1;" : "=f"(vlog) : "f"(vscale));
+        weigh<D, MT>(a, x, r, st, key0, kscale, vlog, __frcp_rn(vscale), key0 < lo_most || key0 + 16 > min(hi_least, s.full), true);
+        uint32_t p[MT][4];
+#pragma unroll
+        for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+          for (int f = 0; f < 4; f++) p[mt][f] = pack_f16(x[mt][f >> 1][2 * (f & 1)], x[mt][f >> 1][2 * (f & 1) + 1]);
+        const uint32_t vat = at + S::KS * D;
+#pragma unroll
+        for (int half = 0; half < (D + 127) / 128; half++) {
+          constexpr int WORDS = D == 64 ? 2 : 4;
+          uint32_t v[4][WORDS];
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            const uint32_t key = 16 * sub + 8 * (i >> 1) + 2 * c + (i & 1);
+            if constexpr (D == 64) {
+              const uint2 w = lds8(vat + key * D + piece<D>(key, n >> 1) * 16 + (n & 1) * 8);
+              v[i][0] = w.x, v[i][1] = w.y;
+            } else {
+              const uint4 w = lds16(vat + key * D + piece<D>(key, 8 * half + n) * 16);
+              v[i][0] = w.x, v[i][1] = w.y, v[i][2] = w.z, v[i][3] = w.w;
+            }
+          }
+#pragma unroll
+          for (int w = 0; w < WORDS; w++)
+#pragma unroll
+            for (int pair = 0; pair < 2; pair++) {
+              const uint32_t lo = __byte_perm(v[0][w], v[1][w], pair ? 0x7362 : 0x5140), hi = __byte_perm(v[2][w], v[3][w], pair ? 0x7362 : 0x5140);
+              const int t8 = 16 * half + 4 * w + 2 * pair;
+              const uint32_t b0 = codes_f16<KIND, false>(lo), b1 = codes_f16<KIND, false>(hi), b2 = codes_f16<KIND, true>(lo), b3 = codes_f16<KIND, true>(hi);
+#pragma unroll
+              for (int mt = 0; mt < MT; mt++) {
+                mma_f16(st.o[mt][t8], p[mt], b0, b1);
+                mma_f16(st.o[mt][t8 + 1], p[mt], b2, b3);
+              }
+            }
+        }
+      }
+      slot = slot + 1 == S::STAGES ? 0 : slot + 1;
+    }
+    // ---- the open block
+    if (tile_end == s.tiles && s.L > s.full) {
+      const int64_t tail_at = (unit * 2 + kv8_slot(cache, b, s.held, s.full / cache.block)) * cache.block * D;
+      for (int key0 = s.full + 16 * (int)warp; key0 < s.L; key0 += 16 * WARPS) open_block<D, MT>(a, qrow, cache.k_tail + tail_at, cache.v_tail + tail_at, s.full, s.L, key0, r, st);
+    }
+
+    // ---- the warps' results together
+    copies_wait<0>();
+    __syncthreads();
+    float *const join = reinterpret_cast<float *>(attend_smem);
+#pragma unroll
+    for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        float l = st.l[mt][h];
+        l += __shfl_xor_sync(BN_FULL, l, 1);
+        l += __shfl_xor_sync(BN_FULL, l, 2);
+        const int row = 16 * mt + 8 * h + (int)n;
+        if (c == 0) join_m[warp][row] = st.m[mt][h], join_l[warp][row] = l;
+        float *const to = join + (warp * S::ROWS + row) * (D + 4);
+        constexpr int RUN = D == 64 ? 8 : 16;  // neighbouring dimensions of a column
+#pragma unroll
+        for (int t = 0; t < NT; t += 4)
+#pragma unroll
+          for (int e = 0; e < 2; e++) *reinterpret_cast<float4 *>(to + (t / RUN) * 128 + (2 * c + e) * RUN + t % RUN) = make_float4(st.o[mt][t][2 * h + e], st.o[mt][t + 1][2 * h + e], st.o[mt][t + 2][2 * h + e], st.o[mt][t + 3][2 * h + e]);
+      }
+    __syncthreads();
+    const bool whole = tile == 0 && tile_end == s.tiles;
+    float *const part = a.parts + ((int64_t)blockIdx.x * 2 + (first ? 0 : 1)) * S::PART;
+    for (int i = (int)threadIdx.x; i < rows * (D / 4); i += WARPS * 32) {
+      const int row = i / (D / 4), col = i % (D / 4) * 4;
+      float m = join_m[0][row], l = 0.0f, o[4] = {};
+#pragma unroll
+      for (int w = 1; w < WARPS; w++) m = fmaxf(m, join_m[w][row]);
+#pragma unroll
+      for (int w = 0; w < WARPS; w++) {
+        const float f = m == -CUDART_INF_F ? 0.0f : ex2(join_m[w][row] - m);
+        const float4 v = *reinterpret_cast<const float4 *>(join + (w * S::ROWS + row) * (D + 4) + col);
+        l = fmaf(f, join_l[w][row], l);
+        o[0] = fmaf(f, v.x, o[0]), o[1] = fmaf(f, v.y, o[1]), o[2] = fmaf(f, v.z, o[2]), o[3] = fmaf(f, v.w, o[3]);
+      }
+      if (whole) {
+        const int t = (row0 + row) / a.group, head = kv * a.group + (row0 + row) % a.group;
+        if (t < s.brought) {
+          const float inv = 1.0f / l;
+          *reinterpret_cast<uint2 *>(a.out + b * a.o_seq + t * a.o_token + head * a.o_head + col) = make_uint2(pack_bf16(o[0] * inv, o[1] * inv), pack_bf16(o[2] * inv, o[3] * inv));
+        } else if (a.zero_rest) {
+          *reinterpret_cast<uint2 *>(a.out + b * a.o_seq + t * a.o_token + head * a.o_head + col) = make_uint2(0, 0);
+        }
+      } else {
+        *reinterpret_cast<float4 *>(part + row * D + col) = make_float4(o[0], o[1], o[2], o[3]);
+        if (col == 0) part[S::ROWS * D + row] = m, part[S::ROWS * D + S::ROWS + row] = l;
+      }
+    }
+    x += tile_end - tile;
+    if (x >= x_end) return;
+    __syncthreads();  // the join's shared memory is the ring's
+    first = false, tile = 0;
+    if (++hr == per_seq) {
+      hr = 0;
+      do s = span_of(a, ++b, S::TILE);
+      while (s.tiles == 0);
+    }
+  }
+}
+
+// Joins what blocks left of a sequence and head that was cut, and zeroes the rows of sequences that brought nothing.
+// A block per sequence, head and row group; its threads take the parts in groups, four dimensions each.
+template <int D, int MT>
+__global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ AttendArgs a) {
+  using S = Shape<D, MT>;
+  __shared__ float sums[256][4], weights[256], tops[256];
+  const int per_seq = (int)a.c.kv_heads * a.row_groups;
+  const int64_t b = blockIdx.x / per_seq;
+  const int hr = (int)(blockIdx.x % per_seq), kv = hr / a.row_groups, row0 = hr % a.row_groups * S::ROWS, rows = min(S::ROWS, a.group * a.tokens - row0);
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int64_t tiles = a.plan[b + 1] - a.plan[b], share = a.plan[a.c.batch + 1];
+  const int64_t from = a.plan[b] * per_seq + hr * tiles, to = from + tiles;
+  if (tiles && from / share == (to - 1) / share) return;  // one block's: it wrote the output
+  int held, brought;
+  kv8_tokens(a.c, a.counts, a.tokens, b, held, brought);
+  const int first = (int)(from / share), last = tiles ? (int)((to - 1) / share) : first - 1;
+  const int tasks = rows * (D / 4), groups = max(1, 256 / tasks);
+  for (int i0 = 0; i0 < tasks; i0 += 256) {
+    const int i = i0 + (groups > 1 ? (int)threadIdx.x % tasks : (int)threadIdx.x), g = groups > 1 ? (int)threadIdx.x / tasks : 0;
+    const int row = min(i, tasks - 1) / (D / 4), col = i % (D / 4) * 4;
+    float m = -CUDART_INF_F, l = 0.0f, o[4] = {};
+    if (g < groups && i < tasks)
+      for (int p = first + g; p <= last; p += groups) {
+        const float *const part = a.parts + ((int64_t)p * 2 + (p == first && from != p * share ? 1 : 0)) * S::PART;
+        const float pm = part[S::ROWS * D + row], pl = part[S::ROWS * D + S::ROWS + row];
+        const float4 v = *reinterpret_cast<const float4 *>(part + row * D + col);
+        const float top = fmaxf(m, pm);
+        if (top == -CUDART_INF_F && !(pl != pl)) continue;
+        const float f = ex2(m - top), pf = ex2(pm - top);
+        m = top, l = l * f + pl * pf;
+        o[0] = o[0] * f + v.x * pf, o[1] = o[1] * f + v.y * pf, o[2] = o[2] * f + v.z * pf, o[3] = o[3] * f + v.w * pf;
+      }
+    if (groups > 1) {
+      tops[threadIdx.x] = m, weights[threadIdx.x] = l;
+#pragma unroll
+      for (int e = 0; e < 4; e++) sums[threadIdx.x][e] = o[e];
+      __syncthreads();
+      if (g == 0)
+        for (int k = 1; k < groups; k++) {
+          const int at = (int)threadIdx.x + k * tasks;
+          const float top = fmaxf(m, tops[at]);
+          if (top == -CUDART_INF_F && !(weights[at] != weights[at])) continue;
+          const float f = ex2(m - top), pf = ex2(tops[at] - top);
+          m = top, l = l * f + weights[at] * pf;
+#pragma unroll
+          for (int e = 0; e < 4; e++) o[e] = o[e] * f + sums[at][e] * pf;
+        }
+    }
+    if (g == 0 && i < tasks) {
+      const int t = (row0 + row) / a.group, head = kv * a.group + (row0 + row) % a.group;
+      uint16_t *const out = a.out + b * a.o_seq + t * a.o_token + head * a.o_head + col;
+      const float inv = 1.0f / l;
+      if (t < brought) *reinterpret_cast<uint2 *>(out) = make_uint2(pack_bf16(o[0] * inv, o[1] * inv), pack_bf16(o[2] * inv, o[3] * inv));
+      else if (a.zero_rest) *reinterpret_cast<uint2 *>(out) = make_uint2(0, 0);
+    }
+  }
+}
+
+int sm_count() {
+  int dev = 0, n = 0;
+  cudaGetDevice(&dev);
+  cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
+  return n > 0 ? n : 148;
+}
+
+// Blocks of a launch, and bytes of its workspace.
+struct Plan {
+  int mt, row_groups, blocks;
+  uint64_t plan_bytes, bytes;
+};
+template <int D>
+Plan plan_of(const bn_kv8 *c, int64_t tokens, int64_t heads) {
+  Plan p;
+  const int64_t rows = heads / c->kv_heads * tokens;
+  p.mt = D < 256 && rows > 16 ? 2 : 1;
+  p.row_groups = (int)((rows + 16 * p.mt - 1) / (16 * p.mt));
+  const int resident = (D == 64 && p.mt == 1) ? 4 : (p.mt * D <= 128) ? 3 : 2;
+  const int tile = p.mt == 1 ? Shape<D, 1>::TILE : Shape<D, 2 - (D == 256)>::TILE;
+  const int64_t most = c->batch * c->kv_heads * p.row_groups * ((c->max_seq + tile - 1) / tile + 1);
+  const int64_t full = (int64_t)sm_count() * resident;
+  p.blocks = (int)(most < full ? most : full);
+  p.plan_bytes = ((uint64_t)(c->batch + 2) * 8 + 127) / 128 * 128;
+  p.bytes = p.plan_bytes + (uint64_t)p.blocks * 2 * (16 * p.mt * (D + 2)) * 4;
+  return p;
+}
+Plan plan_of(const bn_kv8 *c, int64_t tokens, int64_t heads) { return c->D == 64 ? plan_of<64>(c, tokens, heads) : c->D == 128 ? plan_of<128>(c, tokens, heads) : plan_of<256>(c, tokens, heads); }
+
+template <int D, int KIND, int MT>
+int attend_launch(const AttendArgs &a, cudaStream_t stream) {
+  using S = Shape<D, MT>;
+  cudaLaunchConfig_t cfg{};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.gridDim = dim3((unsigned)a.blocks), cfg.blockDim = dim3(WARPS * 32), cfg.dynamicSmemBytes = S::SMEM, cfg.stream = stream, cfg.attrs = attr, cfg.numAttrs = 1;
+  BN_CUDA(allow_smem(attend_kernel<D, KIND, MT>, S::SMEM));
+  BN_CUDA(cudaLaunchKernelEx(&cfg, attend_kernel<D, KIND, MT>, a));
+  cfg.gridDim = dim3((unsigned)(a.c.batch * a.c.kv_heads * a.row_groups)), cfg.blockDim = dim3(256), cfg.dynamicSmemBytes = 0;
+  BN_CUDA(cudaLaunchKernelEx(&cfg, join_kernel<D, MT>, a));
+  return launched("attend_kernel");
+}
+
+template <int KIND>
+int attend_kind(const AttendArgs &a, int mt, cudaStream_t s) {
+  if (a.c.D == 64) return mt == 1 ? attend_launch<64, KIND, 1>(a, s) : attend_launch<64, KIND, 2>(a, s);
+  if (a.c.D == 128) return mt == 1 ? attend_launch<128, KIND, 1>(a, s) : attend_launch<128, KIND, 2>(a, s);
+  return attend_launch<256, KIND, 1>(a, s);
+}
+
+bool attend_sizes(const bn_kv8 *c, int64_t tokens, int64_t heads) { return tokens >= 0 && tokens <= 0x3FFFFFFF && heads >= 1 && heads <= 4096 && heads % c->kv_heads == 0; }
 
 }  // namespace
 }  // namespace bn
 
-extern "C" uint64_t bn_kv8_workspace(const bn_kv8 *, int64_t, int64_t) { return 0; }
+extern "C" uint64_t bn_kv8_workspace(const bn_kv8 *c, int64_t tokens, int64_t heads) {
+  if (bn::kv8_refusal(c) || !bn::attend_sizes(c, tokens, heads) || tokens == 0) return 0;
+  return bn::plan_of(c, tokens, heads).bytes;
+}
 
 extern "C" int bn_kv8_attend(const bn_kv8 *c, const uint16_t *q, int64_t q_seq, int64_t q_token, int64_t q_head, int64_t tokens, int64_t heads, const int32_t *counts, const int32_t *prefix, const bn_scores *scores, uint16_t *out, int64_t o_seq, int64_t o_token, int64_t o_head, int zero_rest, void *workspace, uint64_t workspace_bytes, void *stream) {
   if (const char *why = bn::kv8_refusal(c)) return bn::refuse("bn_kv8_attend", why);
-  if (tokens < 0 || tokens > 0x3FFFFFFF || heads < 1 || heads > 4096 || heads % c->kv_heads) return bn::fail(BN_ERR_ARG, "bn_kv8_attend: bad size (query heads have to be a multiple of the cache's heads)");
+  if (!bn::attend_sizes(c, tokens, heads)) return bn::fail(BN_ERR_ARG, "bn_kv8_attend: bad size (query heads have to be a multiple of the cache's heads)");
   if (!scores || (tokens && (!q || !out))) return bn::fail(BN_ERR_ARG, "bn_kv8_attend: null pointer");
   if (((uintptr_t)q | (uintptr_t)out) & 15 || (q_seq | q_token | q_head | o_seq | o_token | o_head) & 7) return bn::fail(BN_ERR_ARG, "bn_kv8_attend: rows have to start on 16 bytes");
   if (scores->window < 0 || scores->window > 0x3FFFFFFF || !(scores->softcap >= 0.0f)) return bn::fail(BN_ERR_ARG, "bn_kv8_attend: negative window or cap");
-  (void)workspace, (void)workspace_bytes;
   if (tokens == 0) return BN_OK;
-  bn::AttendArgs a{*c, q, out, q_seq, q_token, q_head, o_seq, o_token, o_head, counts, prefix, scores->slopes, (int)tokens, (int)heads, (int)scores->window, scores->causal, zero_rest, scores->scale, scores->softcap};
-  const int64_t blocks = (c->batch * tokens * heads + 3) / 4;
-  if (blocks > 0x7FFFFFFF) return bn::fail(BN_ERR_ARG, "bn_kv8_attend: too many rows");
-  auto pick = [&](auto kind) {
-    constexpr int KIND = decltype(kind)::value;
-    return c->D == 64 ? bn::attend_rows_kernel<64, KIND> : c->D == 128 ? bn::attend_rows_kernel<128, KIND> : bn::attend_rows_kernel<256, KIND>;
-  };
-  auto kern = c->kind == BN_KV8_INT8 ? pick(std::integral_constant<int, BN_KV8_INT8>()) : pick(std::integral_constant<int, BN_KV8_E4M3>());
-  kern<<<(unsigned)blocks, 128, 0, (cudaStream_t)stream>>>(a);
-  return bn::launched("attend_rows_kernel");
+  const bn::Plan p = bn::plan_of(c, tokens, heads);
+  if (!workspace || (uintptr_t)workspace & 15 || workspace_bytes < p.bytes) return bn::fail(BN_ERR_CAPACITY, "bn_kv8_attend: the workspace is smaller than bn_kv8_workspace says, or not on 16 bytes");
+  if (c->batch * c->kv_heads * p.row_groups > 0x7FFFFFFF) return bn::fail(BN_ERR_ARG, "bn_kv8_attend: too many rows for one call");
+  bn::AttendArgs a{*c, q, out, q_seq, q_token, q_head, o_seq, o_token, o_head, counts, prefix, scores->slopes, (int)tokens, (int)heads, (int)(heads / c->kv_heads), (int)scores->window, scores->causal, zero_rest, scores->scale, scores->softcap, (int64_t *)workspace, (float *)((uint8_t *)workspace + p.plan_bytes), p.row_groups, p.blocks};
+  return c->kind == BN_KV8_INT8 ? bn::attend_kind<BN_KV8_INT8>(a, p.mt, (cudaStream_t)stream) : bn::attend_kind<BN_KV8_E4M3>(a, p.mt, (cudaStream_t)stream);
 }

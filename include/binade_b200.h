@@ -314,7 +314,7 @@ int bn_attention(const uint16_t *q, int64_t q_token, int64_t q_head, const uint1
  *              fill that block, the next open one goes to the other slot, and the first stays as it is
  *   length,    [batch] tokens held, and the slot; bn_kv8_advance moves both on. Appending again before
  *   side       that writes the same places again
- * int8: scale = max(amax / 127, 2^-100), code = x / scale rounded to nearest even. e4m3: scale = the least
+ * int8: scale = max(amax / 127, 2^-100), code = x / scale rounded to nearest even, stored as code + 128. e4m3: scale = the least
  * power of two with amax <= 448 scale, at least 2^-100. amax is over the block's finite values; NaN is
  * stored as 0 and an infinity as the largest code (the tail holds them as they are). block is 16, 32 or 64. */
 #define BN_KV8_INT8 0

@@ -42,8 +42,9 @@ struct AppendArgs {
 };
 
 // One block of tokens of one sequence and head, keys or values, by 128 threads: a full block is scaled, coded
-// and stored; the tokens of the blocks that were open or stay open go to the tail in BF16. CHUNKS: 16-byte
-// pieces of the block that a thread has. The read of the new rows and the write of the codes bound it; a block
+// and stored; the tokens of the blocks that were open or stay open go to the tail in BF16. CHUNKS: pieces of
+// eight values that a thread has: neighbours of one token, or for values two neighbours of four tokens, whose codes lie
+// together. The read of the new rows and the write of the codes bound it; a block
 // stays in registers between its maximum and its codes.
 template <int CHUNKS>
 __global__ void __launch_bounds__(128) append_kernel(const __grid_constant__ AppendArgs a) {
@@ -64,7 +65,7 @@ __global__ void __launch_bounds__(128) append_kernel(const __grid_constant__ App
   }
   if (brought == 0) return;
   const int block = c.block, first = held / block, end = held + brought, last = (end - 1) / block;
-  const int D = (int)c.D, per_row = D / 8;
+  const int D = (int)c.D;
   const uint16_t *const in = values ? a.v + b * a.v_seq + h * a.v_head : a.k + b * a.k_seq + h * a.k_head;
   const int64_t step = values ? a.v_token : a.k_token;
   uint16_t *const tails = (values ? c.v_tail : c.k_tail) + unit * 2 * block * D;
@@ -77,10 +78,24 @@ __global__ void __launch_bounds__(128) append_kernel(const __grid_constant__ App
     float amax = 0.0f;
 #pragma unroll
     for (int i = 0; i < CHUNKS; i++) {
-      const int chunk = (int)threadIdx.x + 128 * i, row = chunk / per_row, col = chunk % per_row, p = j * block + row;
-      x[i] = make_uint4(0, 0, 0, 0);
-      if (p < end && (full || p >= held)) x[i] = *reinterpret_cast<const uint4 *>(p < held ? tail + row * D + col * 8 : in + (int64_t)(p - held) * step + col * 8);
-      if (open && p >= held && p < end) *reinterpret_cast<uint4 *>(tail + row * D + col * 8) = x[i];
+      const int chunk = (int)threadIdx.x + 128 * i;
+      if (values) {
+        const int row = chunk / (D / 2) * 4, col = chunk % (D / 2) * 2;
+        uint32_t w[4] = {};
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          const int p = j * block + row + e;
+          if (p < end && (full || p >= held)) w[e] = *reinterpret_cast<const uint32_t *>(p < held ? tail + (row + e) * D + col : in + (int64_t)(p - held) * step + col);
+          if (open && p >= held && p < end) *reinterpret_cast<uint32_t *>(tail + (row + e) * D + col) = w[e];
+        }
+        // dimension by dimension: the order in which the codes lie
+        x[i] = make_uint4(__byte_perm(w[0], w[1], 0x5410), __byte_perm(w[2], w[3], 0x5410), __byte_perm(w[0], w[1], 0x7632), __byte_perm(w[2], w[3], 0x7632));
+      } else {
+        const int row = chunk / (D / 8), col = chunk % (D / 8) * 8, p = j * block + row;
+        x[i] = make_uint4(0, 0, 0, 0);
+        if (p < end && (full || p >= held)) x[i] = *reinterpret_cast<const uint4 *>(p < held ? tail + row * D + col : in + (int64_t)(p - held) * step + col);
+        if (open && p >= held && p < end) *reinterpret_cast<uint4 *>(tail + row * D + col) = x[i];
+      }
       const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
 #pragma unroll
       for (int e = 0; e < 4; e++) amax = fmaxf(amax, fmaxf(finite_size(__uint_as_float(w[e] << 16)), finite_size(__uint_as_float(w[e] & 0xFFFF0000u))));
@@ -124,30 +139,37 @@ __global__ void __launch_bounds__(256) advance_kernel(const __grid_constant__ bn
   if (now / c.block != held / c.block) c.side[b] ^= 1;
 }
 
-// Eight values of a token a thread, of keys and of values; tokens that the cache does not hold as zeros.
+// Eight values a thread, of keys eight of a token, of values two of four tokens, as the codes lie; tokens that the
+// cache does not hold as zeros.
 template <int KIND>
 __global__ void __launch_bounds__(256) dense_kernel(const __grid_constant__ bn_kv8 c, float *__restrict__ k, float *__restrict__ v) {
-  const int per_row = (int)c.D / 8;
-  const int64_t n = c.batch * c.kv_heads * c.max_seq * per_row, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= n) return;
-  const int col = (int)(i % per_row);
-  const int64_t row = i / per_row, unit = row / c.max_seq;
-  const int p = (int)(row % c.max_seq), length = min(max(c.length[unit / c.kv_heads], 0), (int)c.max_seq), full = length / c.block * c.block;
+  const bool values = blockIdx.y;
+  const int D = (int)c.D;
+  const int64_t per_unit = values ? (c.max_seq + 3) / 4 * (D / 2) : c.max_seq * (D / 8);
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, unit = i / per_unit;
+  if (unit >= c.batch * c.kv_heads) return;
+  const int64_t at = i % per_unit;
+  const int row = (int)(values ? at / (D / 2) * 4 : at / (D / 8)), col = (int)(values ? at % (D / 2) * 2 : at % (D / 8) * 8);
+  const int64_t b = unit / c.kv_heads;
+  const int length = min(max(c.length[b], 0), (int)c.max_seq), full = length / c.block * c.block;
+  float x[8] = {};
+  if (row < full) {  // (a block has whole rows of four)
+    const float scale = (values ? c.v_scale : c.k_scale)[unit * (c.rows / c.block) + row / c.block];
+    const uint2 w = *reinterpret_cast<const uint2 *>((values ? c.v : c.k) + (unit * c.rows + row) * D + (values ? 4 : 1) * col);
 #pragma unroll
-  for (int side = 0; side < 2; side++) {
-    float x[8] = {};
-    if (p < full) {
-      const float scale = (side ? c.v_scale : c.k_scale)[unit * (c.rows / c.block) + p / c.block];
-      const uint2 w = *reinterpret_cast<const uint2 *>((side ? c.v : c.k) + (unit * c.rows + p) * c.D + col * 8);
+    for (int e = 0; e < 8; e++) x[e] = kv8_code<KIND>(((e < 4 ? w.x : w.y) >> (8 * (e & 3))) & 0xFFu) * scale;
+  } else {
+    const uint16_t *const tail = (values ? c.v_tail : c.k_tail) + ((unit * 2 + (c.side[b] & 1)) * c.block + row - full) * D + col;
 #pragma unroll
-      for (int e = 0; e < 8; e++) x[e] = kv8_code<KIND>(((e < 4 ? w.x : w.y) >> (8 * (e & 3))) & 0xFFu) * scale;
-    } else if (p < length) {
-      const uint4 w = *reinterpret_cast<const uint4 *>((side ? c.v_tail : c.k_tail) + ((unit * 2 + (c.side[unit / c.kv_heads] & 1)) * c.block + p - full) * c.D + col * 8);
-      const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+    for (int e = 0; e < 8; e++)
+      if (row + (values ? e & 3 : 0) < length) x[e] = bf16_to_f32(tail[values ? (e & 3) * D + (e >> 2) : e]);
+  }
+  if (values) {
 #pragma unroll
-      for (int e = 0; e < 8; e++) x[e] = e & 1 ? __uint_as_float(u[e >> 1] & 0xFFFF0000u) : __uint_as_float(u[e >> 1] << 16);
-    }
-    float4 *const out = reinterpret_cast<float4 *>((side ? v : k) + i * 8);
+    for (int e = 0; e < 4; e++)
+      if (row + e < c.max_seq) *reinterpret_cast<float2 *>(v + (unit * c.max_seq + row + e) * D + col) = make_float2(x[e], x[4 + e]);
+  } else {
+    float4 *const out = reinterpret_cast<float4 *>(k + (unit * c.max_seq + row) * D + col);
     out[0] = make_float4(x[0], x[1], x[2], x[3]), out[1] = make_float4(x[4], x[5], x[6], x[7]);
   }
 }
@@ -198,9 +220,10 @@ extern "C" int bn_kv8_advance(const bn_kv8 *c, int64_t n, const int32_t *counts,
 extern "C" int bn_kv8_dense(const bn_kv8 *c, float *k, float *v, void *stream) {
   if (const char *why = bn::kv8_refusal(c)) return bn::refuse("bn_kv8_dense", why);
   if (!k || !v || ((uintptr_t)k | (uintptr_t)v) & 15) return bn::fail(BN_ERR_ARG, "bn_kv8_dense: outputs have to start on 16 bytes");
-  const int64_t blocks = (c->batch * c->kv_heads * c->max_seq * (c->D / 8) + 255) / 256;
+  const int64_t blocks = (c->batch * c->kv_heads * ((c->max_seq + 3) / 4 * 4) * (c->D / 8) + 255) / 256;
   if (blocks > 0x7FFFFFFF) return bn::fail(BN_ERR_ARG, "bn_kv8_dense: the cache is too large for one call");
-  if (c->kind == BN_KV8_INT8) bn::dense_kernel<BN_KV8_INT8><<<(unsigned)blocks, 256, 0, (cudaStream_t)stream>>>(*c, k, v);
-  else bn::dense_kernel<BN_KV8_E4M3><<<(unsigned)blocks, 256, 0, (cudaStream_t)stream>>>(*c, k, v);
+  const dim3 grid((unsigned)blocks, 2);
+  if (c->kind == BN_KV8_INT8) bn::dense_kernel<BN_KV8_INT8><<<grid, 256, 0, (cudaStream_t)stream>>>(*c, k, v);
+  else bn::dense_kernel<BN_KV8_E4M3><<<grid, 256, 0, (cudaStream_t)stream>>>(*c, k, v);
   return bn::launched("dense_kernel");
 }

@@ -8,12 +8,15 @@
 //                  permute and lose the 1152 by one subtraction; e4m3 converts in hardware
 //   queries        to f16 after a power of two per row that puts its largest value in [1, 2): exact down to
 //                  2^-24 of that value, below which a product does not show in an fp32 sum of scores
-//   scores         K's scale multiplies the sum; V's scale 2^v goes into the exponent: p' = 2^(s + v - m + 15), m
-//                  the running maximum of s + v, so p' fits f16 (rounded to 11 bits, 2^-12) however far apart
+//   scores         K's scale multiplies the sum; V's scale 2^v goes into the exponent: p' = 2^(s + v - m) with m
+//                  near the running maximum of s + v, so p' fits f16 (rounded to 11 bits, 2^-12) however far apart
 //                  the blocks' scales lie, and the sum of weights takes p' / 2^v, in fp32
 //   order of k     a dot product may take its dimensions, and the sum over keys its keys, in any order: each
-//                  thread reads 16 neighbouring bytes of a key (of four keys for V) and calls them the
-//                  elements that the fragments want
+//                  thread reads 16 neighbouring bytes of a key and calls them the elements that the
+//                  fragments want. V's codes lie four keys at a time, dimension by dimension, since its fragments pair
+//                  keys: a word is one dimension of the thread's four keys
+//   maximum        a row's m moves only when a score passes it by 2^15, the room that f16 leaves above 1: a
+//                  vote per 16 keys in place of shuffles and a rescaling of the sums
 // A warp streams its own keys through a cp.async ring of its own: no barrier in the loop; the warps of a block
 // are joined at the end. The work is the tiles of all sequences and heads in a row, cut into equal
 // shares: sequences of unequal lengths load the SMs alike, and one long one spreads over all of them. A sequence and head
@@ -29,7 +32,8 @@ namespace bn {
 namespace {
 
 constexpr int WARPS = 4;
-constexpr float HEADROOM = 15.0f;  // weights reach 2^15: f16 holds them to 11 bits over 29 binades, and to 2^-39 of the largest below
+constexpr float HEADROOM = 15.0f;  // weights may reach 2^15
+constexpr float NOTHING = -3.402823466e38f;  // a row's m while no key was visible: finite, so that a masked score less m stays -inf
 
 struct AttendArgs {
   bn_kv8 c;
@@ -116,9 +120,7 @@ __device__ __forceinline__ uint32_t codes_f16(uint32_t w) {
   return r;
 }
 
-__device__ __forceinline__ void copy16(uint32_t dst, const void *src, bool real) {  // zeros where there is nothing
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
-}
+__device__ __forceinline__ void copy16(uint32_t dst, const void *src) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory"); }
 __device__ __forceinline__ void copy4(uint32_t dst, const void *src) { asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory"); }
 __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -130,17 +132,16 @@ __device__ __forceinline__ uint4 lds16(uint32_t at) {
   asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at));
   return v;
 }
-__device__ __forceinline__ uint2 lds8(uint32_t at) {
-  uint2 v;
-  asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(at));
-  return v;
-}
-
-// Which 16-byte piece of a key's row in shared memory holds its piece `col`: chosen so that the eight lanes of a
-// 16-byte access meet no bank twice, neither where they read two keys' four pieces (K) nor four keys' two (V).
+// Which 16-byte piece of a key's row in shared memory holds its piece `col`, and the same for a row of four keys of V:
+// chosen so that the eight lanes of a 16-byte access meet no bank twice (K: four pieces of two neighbouring
+// keys; V: two pieces of four rows).
 template <int D>
-__device__ __forceinline__ uint32_t piece(uint32_t key, uint32_t col) {
-  return D == 64 ? col ^ ((key >> 1) & 3u) : col ^ (((key & 1u) << 2) | (((key >> 1) & 3u) << 1));
+__device__ __forceinline__ uint32_t k_piece(uint32_t key, uint32_t col) {
+  return D == 64 ? col : col ^ ((key & 1u) << 2);
+}
+template <int D>
+__device__ __forceinline__ uint32_t v_piece(uint32_t four, uint32_t col) {
+  return D == 64 ? col ^ ((four & 1u) | ((four & 2u) << 1)) : col ^ (four & 3u);
 }
 
 // What a warp has so far: sums, running maxima (of s + v, in powers of two) and weights of its lane's rows.
@@ -150,65 +151,94 @@ struct State {
   float m[MT][2], l[MT][2];
 };
 
-// What a lane's rows need: positions, the visible run, the factor from a sum of products to a score.
+// What a lane's rows need: positions (-1: no row), the factor from a sum of products to a score, the bias.
 template <int MT>
 struct Rows {
-  int i[MT][2], lo[MT][2], hi[MT][2];
+  int i[MT][2];
   float factor[MT][2], slope[MT][2];
+  int L, prefix;
 };
 
-// The scores of a 16-key piece into weights: x holds the raw sums and gets p'. vlog, vinv: V's scale as a power of
-// two and inverted. Updates maxima and weights, rescales the sums where a maximum rose.
-template <int D, int MT>
-__device__ __forceinline__ void weigh(const AttendArgs &a, float (&x)[MT][2][4], const Rows<MT> &r, State<D, MT> &st, int key0, float kscale, float vlog, float vinv, bool masked, bool scaled_rows) {
-  const uint32_t c = lane_id() & 3u;
+// The scores of a 16-key piece into weights: x holds the raw sums and gets p' (tile j, column 2c + e: key key0 + 4c
+// + 2j + e). scale, vlog, vinv: K's scale, V's as a power of two and inverted. Updates the weights' sum; where a score passes
+// a row's m by the headroom, moves m and rescales the sums.
+template <int D, int MT, bool PLAIN>
+__device__ __forceinline__ void weigh(const AttendArgs &a, float (&x)[MT][2][4], const Rows<MT> &r, State<D, MT> &st, int key0, float scale, float vlog, float vinv, bool masked) {
+  const int first = key0 + 4 * (int)(lane_id() & 3u);
 #pragma unroll
-  for (int mt = 0; mt < MT; mt++) {
-    float top[2];
+  for (int mt = 0; mt < MT; mt++)
 #pragma unroll
     for (int h = 0; h < 2; h++) {
-      top[h] = st.m[mt][h];
-      const float f = scaled_rows ? r.factor[mt][h] : a.cap > 0.0f ? a.scale * (2.0f * LOG2E / a.cap) : a.scale * LOG2E;
+      const float f = fminf(scale * r.factor[mt][h], 3.0e38f);
 #pragma unroll
       for (int j = 0; j < 2; j++)
 #pragma unroll
         for (int e = 0; e < 2; e++) {
           float &v = x[mt][j][2 * h + e];
-          const int key = key0 + 8 * j + 2 * (int)c + e;
-          v = v * kscale * f;
-          if (a.cap > 0.0f) v = capped(v, a.cap * LOG2E);
-          if (a.slopes) v = fmaf(-r.slope[mt][h], (float)abs(r.i[mt][h] - key), v);
-          v += vlog;
-          if (masked && (key < r.lo[mt][h] || key >= r.hi[mt][h])) v = -CUDART_INF_F;
-          top[h] = fmaxf(top[h], v);
+          if constexpr (PLAIN) {
+            v = fmaf(v, f, vlog);
+          } else {
+            v *= f;
+            if (a.cap > 0.0f) v = capped(v, a.cap * LOG2E);
+            v = fmaf(-r.slope[mt][h], (float)abs(r.i[mt][h] - (first + 2 * j + e)), v) + vlog;
+          }
         }
-      top[h] = fmaxf(top[h], __shfl_xor_sync(BN_FULL, top[h], 1));
-      top[h] = fmaxf(top[h], __shfl_xor_sync(BN_FULL, top[h], 2));
     }
-    if (__any_sync(BN_FULL, top[0] > st.m[mt][0] || top[1] > st.m[mt][1])) {
+  if (masked) {
+#pragma unroll
+    for (int mt = 0; mt < MT; mt++)
 #pragma unroll
       for (int h = 0; h < 2; h++) {
-        const float keep = top[h] > st.m[mt][h] ? ex2(st.m[mt][h] - top[h]) : 1.0f;
-        st.m[mt][h] = top[h], st.l[mt][h] *= keep;
+        int lo = 0, hi = 0;
+        if (r.i[mt][h] >= 0) visible_keys(r.i[mt][h], r.L, r.prefix, a.window, a.causal, lo, hi);
 #pragma unroll
-        for (int t = 0; t < Shape<D, MT>::NT; t++) st.o[mt][t][2 * h] *= keep, st.o[mt][t][2 * h + 1] *= keep;
+        for (int j = 0; j < 2; j++)
+#pragma unroll
+          for (int e = 0; e < 2; e++) {
+            const int key = first + 2 * j + e;
+            if (key < lo || key >= hi) x[mt][j][2 * h + e] = -CUDART_INF_F;
+          }
       }
-    }
+  }
+  float top[MT][2];
+  bool over = false;
+#pragma unroll
+  for (int mt = 0; mt < MT; mt++)
 #pragma unroll
     for (int h = 0; h < 2; h++) {
-      const float base = top[h] == -CUDART_INF_F ? 0.0f : top[h] - HEADROOM;  // nothing visible yet: weights of 0
+      top[mt][h] = fmaxf(fmaxf(x[mt][0][2 * h], x[mt][0][2 * h + 1]), fmaxf(x[mt][1][2 * h], x[mt][1][2 * h + 1]));
+      over |= top[mt][h] > st.m[mt][h] + HEADROOM;
+    }
+  if (__any_sync(BN_FULL, over)) {
+#pragma unroll
+    for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        float t = top[mt][h];
+        t = fmaxf(t, __shfl_xor_sync(BN_FULL, t, 1));
+        t = fmaxf(t, __shfl_xor_sync(BN_FULL, t, 2));
+        t = fmaxf(t, st.m[mt][h]);
+        const float keep = ex2(st.m[mt][h] - t);
+        st.m[mt][h] = t, st.l[mt][h] *= keep;
+#pragma unroll
+        for (int n = 0; n < Shape<D, MT>::NT; n++) st.o[mt][n][2 * h] *= keep, st.o[mt][n][2 * h + 1] *= keep;
+      }
+  }
+#pragma unroll
+  for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
       float sum = 0.0f;
 #pragma unroll
       for (int j = 0; j < 2; j++)
 #pragma unroll
         for (int e = 0; e < 2; e++) {
           float &v = x[mt][j][2 * h + e];
-          v = ex2(v - base);
+          v = ex2(v - st.m[mt][h]);
           sum += v;
         }
       st.l[mt][h] = fmaf(sum, vinv, st.l[mt][h]);
     }
-  }
 }
 
 // The dimension of n8 tile t's column n.
@@ -220,14 +250,14 @@ __device__ __forceinline__ constexpr int dim_of(int t, int n) {
 // The open block's 16 tokens from `key0` on, in BF16. Weights go in two BF16 halves (hi + lo: 2^-17), values times 2^-23
 // with 2^23 in the weights' exponent, so that no sum of 63 of them passes fp32. Where a value is not finite, a
 // weight of zero must not touch it: those go one by one.
-template <int D, int MT>
+template <int D, int MT, bool PLAIN>
 __device__ void open_block(const AttendArgs &a, const uint16_t *const (&qrow)[MT][2], const uint16_t *ktail, const uint16_t *vtail, int full, int L, int key0, const Rows<MT> &r, State<D, MT> &st) {
   const uint32_t lane = lane_id(), n = lane >> 2, c = lane & 3u;
   const int last = L - 1 - full, at = key0 - full;  // the last token's row, this piece's first
   float x[MT][2][4] = {};
   const uint16_t *k[2];
 #pragma unroll
-  for (int j = 0; j < 2; j++) k[j] = ktail + (int64_t)min(at + 8 * j + (int)n, last) * D + 16 * c;
+  for (int j = 0; j < 2; j++) k[j] = ktail + (int64_t)min(at + 4 * (int)(n >> 1) + 2 * j + (int)(n & 1), last) * D + 16 * c;
 #pragma unroll 1
   for (int g = 0; g < D / 64; g++)
 #pragma unroll
@@ -244,7 +274,10 @@ __device__ void open_block(const AttendArgs &a, const uint16_t *const (&qrow)[MT
         mma_bf16x(x[mt][1], f, k1.x, k1.y);
       }
     }
-  weigh<D, MT>(a, x, r, st, key0, 1.0f, 23.0f, 1.0f / (1 << 23), true, false);
+  Rows<MT> plain = r;  // the queries as they are: no power of two in the factor
+#pragma unroll
+  for (int mt = 0; mt < MT; mt++) plain.factor[mt][0] = plain.factor[mt][1] = a.cap > 0.0f ? a.scale * (2.0f * LOG2E / a.cap) : a.scale * LOG2E;
+  weigh<D, MT, PLAIN>(a, x, plain, st, key0, 1.0f, 23.0f, 1.0f / (1 << 23), true);
   uint32_t hi[MT][4], lo[MT][4];
 #pragma unroll
   for (int mt = 0; mt < MT; mt++)
@@ -257,7 +290,7 @@ __device__ void open_block(const AttendArgs &a, const uint16_t *const (&qrow)[MT
   const uint16_t *v[4];
   bool odd = false;
 #pragma unroll
-  for (int i = 0; i < 4; i++) v[i] = vtail + (int64_t)min(at + 8 * (i >> 1) + 2 * (int)c + (i & 1), last) * D;
+  for (int i = 0; i < 4; i++) v[i] = vtail + (int64_t)min(at + 4 * (int)c + i, last) * D;
 #pragma unroll
   for (int t = 0; t < Shape<D, MT>::NT; t += 2) {
     uint32_t w[4];  // dims dim_of(t, n) and the next
@@ -291,12 +324,12 @@ __device__ void open_block(const AttendArgs &a, const uint16_t *const (&qrow)[MT
 #pragma unroll
   for (int key = 0; key < 16; key++) {
     const uint16_t *const row = vtail + (int64_t)min(at + key, last) * D;
-    const uint32_t from = (lane & ~3u) | ((key & 7) >> 1);
+    const uint32_t from = (lane & ~3u) | (key >> 2);
 #pragma unroll
     for (int mt = 0; mt < MT; mt++)
 #pragma unroll
       for (int h = 0; h < 2; h++) {
-        const float p = __shfl_sync(BN_FULL, x[mt][key >> 3][2 * h + (key & 1)], from);
+        const float p = __shfl_sync(BN_FULL, x[mt][(key >> 1) & 1][2 * h + (key & 1)], from);
         if (p != 0.0f)
 #pragma unroll
           for (int t = 0; t < Shape<D, MT>::NT; t++)
@@ -306,7 +339,7 @@ __device__ void open_block(const AttendArgs &a, const uint16_t *const (&qrow)[MT
   }
 }
 
-template <int D, int KIND, int MT>
+template <int D, int KIND, int MT, bool PLAIN>
 __global__ void __launch_bounds__(WARPS * 32, (D == 64 && MT == 1) ? 4 : (MT * D <= 128) ? 3 : 2) attend_kernel(const __grid_constant__ AttendArgs a) {
   using S = Shape<D, MT>;
   constexpr int NT = S::NT;
@@ -360,6 +393,7 @@ __global__ void __launch_bounds__(WARPS * 32, (D == 64 && MT == 1) ? 4 : (MT * D
     hr = (int)(rest / s.tiles), tile = (int)(rest % s.tiles);
   }
   const uint32_t ring = smem_addr(attend_smem) + warp * (S::STAGES * S::STAGE_BYTES);
+  const int block_log2 = 31 - __clz(cache.block);
   bool first = true;
 
   while (true) {
@@ -370,21 +404,25 @@ __global__ void __launch_bounds__(WARPS * 32, (D == 64 && MT == 1) ? 4 : (MT * D
     const uint8_t *const codes[2] = {cache.k + unit * cache.rows * D, cache.v + unit * cache.rows * D};
     const int64_t scale_at = unit * (cache.rows / cache.block);
 
-    auto issue = [&](int t, int slot) {  // this warp's keys of tile t
+    // this warp's keys of tile t, 16 at a time: those of the full blocks come in whole pieces
+    auto issue = [&](int t, int slot) {
       if (t < min(tile_end, s.quant)) {
         const int key0 = s.start + t * S::TILE + (int)warp * S::KS;
         const uint32_t to = ring + slot * S::STAGE_BYTES;
 #pragma unroll
-        for (int side = 0; side < 2; side++)
+        for (int sub = 0; sub < S::KS / 16; sub++) {
+          if (key0 + 16 * sub >= s.full) break;
 #pragma unroll
-          for (int i = 0; i < S::KS * D / 512; i++) {
-            const uint32_t q = lane + 32 * i, key = q / (D / 16), col = q % (D / 16);
-            const bool real = key0 + (int)key < s.full;
-            copy16(to + side * (S::KS * D) + key * D + piece<D>(key, col) * 16, codes[side] + (real ? (int64_t)(key0 + (int)key) * D + col * 16 : 0), real);
+          for (int side = 0; side < 2; side++) {
+            const uint8_t *const from = codes[side] + (int64_t)(key0 + 16 * sub) * D + lane * 16;
+#pragma unroll
+            for (int i = 0; i < D / 32; i++) {
+              const uint32_t q = lane + 32 * i;
+              const uint32_t at = side ? q / (D / 4) * (4 * D) + v_piece<D>(q / (D / 4), q % (D / 4)) * 16 : q / (D / 16) * D + k_piece<D>(q / (D / 16), q % (D / 16)) * 16;
+              copy16(to + side * (S::KS * D) + sub * (16 * D) + at, from + i * 512);
+            }
           }
-        if (lane < 2 * (S::KS / 16)) {
-          const int side = (int)lane / (S::KS / 16), sub = (int)lane % (S::KS / 16);
-          copy4(smem_addr(&scales[warp][slot][side][sub]), (side ? cache.v_scale : cache.k_scale) + scale_at + min(key0 + 16 * sub, s.full - 1) / cache.block);
+          if (lane < 2) copy4(smem_addr(&scales[warp][slot][lane][sub]), (lane ? cache.v_scale : cache.k_scale) + scale_at + ((key0 + 16 * sub) >> block_log2));
         }
       }
       copies_commit();
@@ -399,6 +437,7 @@ __global__ void __launch_bounds__(WARPS * 32, (D == 64 && MT == 1) ? 4 : (MT * D
     visible_keys(s.held + t_last, s.L, prefix, a.window, a.causal, lo_most, unused);
     visible_keys(s.held + t_first, s.L, prefix, a.window, a.causal, unused, hi_least);
     Rows<MT> r;
+    r.L = s.L, r.prefix = prefix;
     State<D, MT> st;
     uint32_t q[MT][D / 16][4];
     const uint16_t *qrow[MT][2];
@@ -410,10 +449,9 @@ __global__ void __launch_bounds__(WARPS * 32, (D == 64 && MT == 1) ? 4 : (MT * D
         const int row = 16 * mt + 8 * h + (int)n, t = (row0 + row) / a.group, head = kv * a.group + (row0 + row) % a.group;
         const bool real = row < rows && t < s.brought;
         qrow[mt][h] = real ? a.q + b * a.q_seq + t * a.q_token + head * a.q_head : nullptr;
-        r.i[mt][h] = s.held + t, r.lo[mt][h] = r.hi[mt][h] = 0;
-        if (real) visible_keys(s.held + t, s.L, prefix, a.window, a.causal, r.lo[mt][h], r.hi[mt][h]);
+        r.i[mt][h] = real ? s.held + t : -1;
         r.slope[mt][h] = real && a.slopes ? a.slopes[head] * LOG2E : 0.0f;
-        st.m[mt][h] = -CUDART_INF_F, st.l[mt][h] = 0.0f;
+        st.m[mt][h] = NOTHING, st.l[mt][h] = 0.0f;
         uint32_t most = 0;
 #pragma unroll
         for (int g = 0; g < D / 64; g++)
@@ -463,8 +501,8 @@ __global__ void __launch_bounds__(WARPS * 32, (D == 64 && MT == 1) ? 4 : (MT * D
         for (int g = 0; g < D / 64; g++)
 #pragma unroll
           for (int j = 0; j < 2; j++) {
-            const uint32_t key = 16 * sub + 8 * j + n;
-            const uint4 w4 = lds16(at + key * D + piece<D>(key, 4 * g + c) * 16);
+            const uint32_t key = 16 * sub + 4 * (n >> 1) + 2 * j + (n & 1);
+            const uint4 w4 = lds16(at + key * D + k_piece<D>(key, 4 * g + c) * 16);
             const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
 #pragma unroll
             for (int e = 0; e < 4; e++) {
@@ -475,49 +513,33 @@ __global__ void __launch_bounds__(WARPS * 32, (D == 64 && MT == 1) ? 4 : (MT * D
           }
         float vlog;
         asm("lg2.approx.f32 %0, %1;" : "=f"(vlog) : "f"(vscale));
-        weigh<D, MT>(a, x, r, st, key0, kscale, vlog, __frcp_rn(vscale), key0 < lo_most || key0 + 16 > min(hi_least, s.full), true);
+        weigh<D, MT, PLAIN>(a, x, r, st, key0, kscale, vlog, __fdividef(1.0f, vscale), key0 < lo_most || key0 + 16 > hi_least);
         uint32_t p[MT][4];
 #pragma unroll
         for (int mt = 0; mt < MT; mt++)
 #pragma unroll
           for (int f = 0; f < 4; f++) p[mt][f] = pack_f16(x[mt][f >> 1][2 * (f & 1)], x[mt][f >> 1][2 * (f & 1) + 1]);
-        const uint32_t vat = at + S::KS * D;
+        const uint32_t vat = at + S::KS * D + (4 * sub + c) * (4 * D);
 #pragma unroll
-        for (int half = 0; half < (D + 127) / 128; half++) {
-          constexpr int WORDS = D == 64 ? 2 : 4;
-          uint32_t v[4][WORDS];
+        for (int half = 0; half < (D + 127) / 128; half++)
 #pragma unroll
-          for (int i = 0; i < 4; i++) {
-            const uint32_t key = 16 * sub + 8 * (i >> 1) + 2 * c + (i & 1);
-            if constexpr (D == 64) {
-              const uint2 w = lds8(vat + key * D + piece<D>(key, n >> 1) * 16 + (n & 1) * 8);
-              v[i][0] = w.x, v[i][1] = w.y;
-            } else {
-              const uint4 w = lds16(vat + key * D + piece<D>(key, 8 * half + n) * 16);
-              v[i][0] = w.x, v[i][1] = w.y, v[i][2] = w.z, v[i][3] = w.w;
+          for (int i = 0; i < (D == 64 ? 2 : 4); i++) {
+            const uint4 w4 = lds16(vat + v_piece<D>(c, 32 * half + (D == 64 ? 2 : 4) * n + i) * 16);
+            const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+              const uint32_t b0 = codes_f16<KIND, false>(w[e]), b1 = codes_f16<KIND, true>(w[e]);
+#pragma unroll
+              for (int mt = 0; mt < MT; mt++) mma_f16(st.o[mt][16 * half + 4 * i + e], p[mt], b0, b1);
             }
           }
-#pragma unroll
-          for (int w = 0; w < WORDS; w++)
-#pragma unroll
-            for (int pair = 0; pair < 2; pair++) {
-              const uint32_t lo = __byte_perm(v[0][w], v[1][w], pair ? 0x7362 : 0x5140), hi = __byte_perm(v[2][w], v[3][w], pair ? 0x7362 : 0x5140);
-              const int t8 = 16 * half + 4 * w + 2 * pair;
-              const uint32_t b0 = codes_f16<KIND, false>(lo), b1 = codes_f16<KIND, false>(hi), b2 = codes_f16<KIND, true>(lo), b3 = codes_f16<KIND, true>(hi);
-#pragma unroll
-              for (int mt = 0; mt < MT; mt++) {
-                mma_f16(st.o[mt][t8], p[mt], b0, b1);
-                mma_f16(st.o[mt][t8 + 1], p[mt], b2, b3);
-              }
-            }
-        }
       }
       slot = slot + 1 == S::STAGES ? 0 : slot + 1;
     }
     // ---- the open block
     if (tile_end == s.tiles && s.L > s.full) {
       const int64_t tail_at = (unit * 2 + kv8_slot(cache, b, s.held, s.full / cache.block)) * cache.block * D;
-      for (int key0 = s.full + 16 * (int)warp; key0 < s.L; key0 += 16 * WARPS) open_block<D, MT>(a, qrow, cache.k_tail + tail_at, cache.v_tail + tail_at, s.full, s.L, key0, r, st);
+      for (int key0 = s.full + 16 * (int)warp; key0 < s.L; key0 += 16 * WARPS) open_block<D, MT, PLAIN>(a, qrow, cache.k_tail + tail_at, cache.v_tail + tail_at, s.full, s.L, key0, r, st);
     }
 
     // ---- the warps' results together
@@ -550,7 +572,7 @@ __global__ void __launch_bounds__(WARPS * 32, (D == 64 && MT == 1) ? 4 : (MT * D
       for (int w = 1; w < WARPS; w++) m = fmaxf(m, join_m[w][row]);
 #pragma unroll
       for (int w = 0; w < WARPS; w++) {
-        const float f = m == -CUDART_INF_F ? 0.0f : ex2(join_m[w][row] - m);
+        const float f = ex2(join_m[w][row] - m);
         const float4 v = *reinterpret_cast<const float4 *>(join + (w * S::ROWS + row) * (D + 4) + col);
         l = fmaf(f, join_l[w][row], l);
         o[0] = fmaf(f, v.x, o[0]), o[1] = fmaf(f, v.y, o[1]), o[2] = fmaf(f, v.z, o[2]), o[3] = fmaf(f, v.w, o[3]);
@@ -581,11 +603,15 @@ __global__ void __launch_bounds__(WARPS * 32, (D == 64 && MT == 1) ? 4 : (MT * D
 }
 
 // Joins what blocks left of a sequence and head that was cut, and zeroes the rows of sequences that brought nothing.
-// A block per sequence, head and row group; its threads take the parts in groups, four dimensions each.
+// A block per sequence, head and row group: first the rows' maxima over the parts and the factors that go with them,
+// then the sums, four dimensions a thread, the parts in groups where there are few rows.
+constexpr int JOIN_THREADS = 256, JOIN_PARTS = 64;
+
 template <int D, int MT>
-__global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ AttendArgs a) {
+__global__ void __launch_bounds__(JOIN_THREADS) join_kernel(const __grid_constant__ AttendArgs a) {
   using S = Shape<D, MT>;
-  __shared__ float sums[256][4], weights[256], tops[256];
+  __shared__ float factor[JOIN_PARTS][S::ROWS], tops[S::ROWS], weights[S::ROWS];
+  __shared__ float4 sums[JOIN_THREADS];
   const int per_seq = (int)a.c.kv_heads * a.row_groups;
   const int64_t b = blockIdx.x / per_seq;
   const int hr = (int)(blockIdx.x % per_seq), kv = hr / a.row_groups, row0 = hr % a.row_groups * S::ROWS, rows = min(S::ROWS, a.group * a.tokens - row0);
@@ -596,45 +622,58 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Atten
   if (tiles && from / share == (to - 1) / share) return;  // one block's: it wrote the output
   int held, brought;
   kv8_tokens(a.c, a.counts, a.tokens, b, held, brought);
-  const int first = (int)(from / share), last = tiles ? (int)((to - 1) / share) : first - 1;
-  const int tasks = rows * (D / 4), groups = max(1, 256 / tasks);
-  for (int i0 = 0; i0 < tasks; i0 += 256) {
-    const int i = i0 + (groups > 1 ? (int)threadIdx.x % tasks : (int)threadIdx.x), g = groups > 1 ? (int)threadIdx.x / tasks : 0;
+  const int first = (int)(from / share), parts = tiles ? (int)((to - 1) / share) - first + 1 : 0;
+  auto part_of = [&](int p) { return a.parts + ((int64_t)(first + p) * 2 + (p == 0 && from != first * share ? 1 : 0)) * S::PART; };
+  const int warp = (int)(threadIdx.x >> 5), lane = (int)lane_id();
+  for (int row = warp; row < rows; row += JOIN_THREADS / 32) {
+    float m = NOTHING, l = 0.0f;
+    for (int p = lane; p < parts; p += 32) m = fmaxf(m, part_of(p)[S::ROWS * D + row]);
+#pragma unroll
+    for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(BN_FULL, m, d));
+    for (int p = lane; p < parts; p += 32) {
+      const float *const part = part_of(p);
+      l = fmaf(ex2(part[S::ROWS * D + row] - m), part[S::ROWS * D + S::ROWS + row], l);
+    }
+#pragma unroll
+    for (int d = 16; d; d >>= 1) l += __shfl_xor_sync(BN_FULL, l, d);
+    if (lane == 0) tops[row] = m, weights[row] = l;
+  }
+  const int tasks = rows * (D / 4), groups = max(1, JOIN_THREADS / tasks);
+  for (int i0 = 0; i0 < tasks; i0 += JOIN_THREADS) {
+    const int g = groups > 1 ? (int)threadIdx.x / tasks : 0, i = i0 + (groups > 1 ? (int)threadIdx.x % tasks : (int)threadIdx.x);
     const int row = min(i, tasks - 1) / (D / 4), col = i % (D / 4) * 4;
-    float m = -CUDART_INF_F, l = 0.0f, o[4] = {};
-    if (g < groups && i < tasks)
-      for (int p = first + g; p <= last; p += groups) {
-        const float *const part = a.parts + ((int64_t)p * 2 + (p == first && from != p * share ? 1 : 0)) * S::PART;
-        const float pm = part[S::ROWS * D + row], pl = part[S::ROWS * D + S::ROWS + row];
-        const float4 v = *reinterpret_cast<const float4 *>(part + row * D + col);
-        const float top = fmaxf(m, pm);
-        if (top == -CUDART_INF_F && !(pl != pl)) continue;
-        const float f = ex2(m - top), pf = ex2(pm - top);
-        m = top, l = l * f + pl * pf;
-        o[0] = o[0] * f + v.x * pf, o[1] = o[1] * f + v.y * pf, o[2] = o[2] * f + v.z * pf, o[3] = o[3] * f + v.w * pf;
-      }
-    if (groups > 1) {
-      tops[threadIdx.x] = m, weights[threadIdx.x] = l;
-#pragma unroll
-      for (int e = 0; e < 4; e++) sums[threadIdx.x][e] = o[e];
+    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int p0 = 0; p0 < parts; p0 += JOIN_PARTS) {
+      const int some = min(JOIN_PARTS, parts - p0);
       __syncthreads();
-      if (g == 0)
-        for (int k = 1; k < groups; k++) {
-          const int at = (int)threadIdx.x + k * tasks;
-          const float top = fmaxf(m, tops[at]);
-          if (top == -CUDART_INF_F && !(weights[at] != weights[at])) continue;
-          const float f = ex2(m - top), pf = ex2(tops[at] - top);
-          m = top, l = l * f + weights[at] * pf;
-#pragma unroll
-          for (int e = 0; e < 4; e++) o[e] = o[e] * f + sums[at][e] * pf;
+      for (int k = (int)threadIdx.x; k < some * rows; k += JOIN_THREADS) factor[k / rows][k % rows] = ex2(part_of(p0 + k / rows)[S::ROWS * D + k % rows] - tops[k % rows]);
+      __syncthreads();
+      if (g < groups && i < tasks) {
+#pragma unroll 8
+        for (int p = g; p < some; p += groups) {
+          const float f = factor[p][row];
+          const float4 v = *reinterpret_cast<const float4 *>(part_of(p0 + p) + row * D + col);
+          o.x = fmaf(f, v.x, o.x), o.y = fmaf(f, v.y, o.y), o.z = fmaf(f, v.z, o.z), o.w = fmaf(f, v.w, o.w);
         }
+      }
+    }
+    if (groups > 1) {
+      sums[threadIdx.x] = o;
+      __syncthreads();
+      for (int k = 1; g == 0 && k < groups; k++) {
+        const float4 v = sums[(int)threadIdx.x + k * tasks];
+        o.x += v.x, o.y += v.y, o.z += v.z, o.w += v.w;
+      }
     }
     if (g == 0 && i < tasks) {
       const int t = (row0 + row) / a.group, head = kv * a.group + (row0 + row) % a.group;
       uint16_t *const out = a.out + b * a.o_seq + t * a.o_token + head * a.o_head + col;
-      const float inv = 1.0f / l;
-      if (t < brought) *reinterpret_cast<uint2 *>(out) = make_uint2(pack_bf16(o[0] * inv, o[1] * inv), pack_bf16(o[2] * inv, o[3] * inv));
-      else if (a.zero_rest) *reinterpret_cast<uint2 *>(out) = make_uint2(0, 0);
+      if (t < brought) {
+        const float inv = 1.0f / weights[row];
+        *reinterpret_cast<uint2 *>(out) = make_uint2(pack_bf16(o.x * inv, o.y * inv), pack_bf16(o.z * inv, o.w * inv));
+      } else if (a.zero_rest) {
+        *reinterpret_cast<uint2 *>(out) = make_uint2(0, 0);
+      }
     }
   }
 }
@@ -668,7 +707,7 @@ Plan plan_of(const bn_kv8 *c, int64_t tokens, int64_t heads) {
 }
 Plan plan_of(const bn_kv8 *c, int64_t tokens, int64_t heads) { return c->D == 64 ? plan_of<64>(c, tokens, heads) : c->D == 128 ? plan_of<128>(c, tokens, heads) : plan_of<256>(c, tokens, heads); }
 
-template <int D, int KIND, int MT>
+template <int D, int KIND, int MT, bool PLAIN>
 int attend_launch(const AttendArgs &a, cudaStream_t stream) {
   using S = Shape<D, MT>;
   cudaLaunchConfig_t cfg{};
@@ -676,18 +715,18 @@ int attend_launch(const AttendArgs &a, cudaStream_t stream) {
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.gridDim = dim3((unsigned)a.blocks), cfg.blockDim = dim3(WARPS * 32), cfg.dynamicSmemBytes = S::SMEM, cfg.stream = stream, cfg.attrs = attr, cfg.numAttrs = 1;
-  BN_CUDA(allow_smem(attend_kernel<D, KIND, MT>, S::SMEM));
-  BN_CUDA(cudaLaunchKernelEx(&cfg, attend_kernel<D, KIND, MT>, a));
-  cfg.gridDim = dim3((unsigned)(a.c.batch * a.c.kv_heads * a.row_groups)), cfg.blockDim = dim3(256), cfg.dynamicSmemBytes = 0;
+  BN_CUDA(allow_smem(attend_kernel<D, KIND, MT, PLAIN>, S::SMEM));
+  BN_CUDA(cudaLaunchKernelEx(&cfg, attend_kernel<D, KIND, MT, PLAIN>, a));
+  cfg.gridDim = dim3((unsigned)(a.c.batch * a.c.kv_heads * a.row_groups)), cfg.blockDim = dim3(JOIN_THREADS), cfg.dynamicSmemBytes = 0;
   BN_CUDA(cudaLaunchKernelEx(&cfg, join_kernel<D, MT>, a));
   return launched("attend_kernel");
 }
 
-template <int KIND>
+template <int KIND, bool PLAIN>
 int attend_kind(const AttendArgs &a, int mt, cudaStream_t s) {
-  if (a.c.D == 64) return mt == 1 ? attend_launch<64, KIND, 1>(a, s) : attend_launch<64, KIND, 2>(a, s);
-  if (a.c.D == 128) return mt == 1 ? attend_launch<128, KIND, 1>(a, s) : attend_launch<128, KIND, 2>(a, s);
-  return attend_launch<256, KIND, 1>(a, s);
+  if (a.c.D == 64) return mt == 1 ? attend_launch<64, KIND, 1, PLAIN>(a, s) : attend_launch<64, KIND, 2, PLAIN>(a, s);
+  if (a.c.D == 128) return mt == 1 ? attend_launch<128, KIND, 1, PLAIN>(a, s) : attend_launch<128, KIND, 2, PLAIN>(a, s);
+  return attend_launch<256, KIND, 1, PLAIN>(a, s);
 }
 
 bool attend_sizes(const bn_kv8 *c, int64_t tokens, int64_t heads) { return tokens >= 0 && tokens <= 0x3FFFFFFF && heads >= 1 && heads <= 4096 && heads % c->kv_heads == 0; }
@@ -711,5 +750,7 @@ extern "C" int bn_kv8_attend(const bn_kv8 *c, const uint16_t *q, int64_t q_seq, 
   if (!workspace || (uintptr_t)workspace & 15 || workspace_bytes < p.bytes) return bn::fail(BN_ERR_CAPACITY, "bn_kv8_attend: the workspace is smaller than bn_kv8_workspace says, or not on 16 bytes");
   if (c->batch * c->kv_heads * p.row_groups > 0x7FFFFFFF) return bn::fail(BN_ERR_ARG, "bn_kv8_attend: too many rows for one call");
   bn::AttendArgs a{*c, q, out, q_seq, q_token, q_head, o_seq, o_token, o_head, counts, prefix, scores->slopes, (int)tokens, (int)heads, (int)(heads / c->kv_heads), (int)scores->window, scores->causal, zero_rest, scores->scale, scores->softcap, (int64_t *)workspace, (float *)((uint8_t *)workspace + p.plan_bytes), p.row_groups, p.blocks};
-  return c->kind == BN_KV8_INT8 ? bn::attend_kind<BN_KV8_INT8>(a, p.mt, (cudaStream_t)stream) : bn::attend_kind<BN_KV8_E4M3>(a, p.mt, (cudaStream_t)stream);
+  const cudaStream_t s = (cudaStream_t)stream;
+  if (scores->softcap == 0.0f && !scores->slopes) return c->kind == BN_KV8_INT8 ? bn::attend_kind<BN_KV8_INT8, true>(a, p.mt, s) : bn::attend_kind<BN_KV8_E4M3, true>(a, p.mt, s);
+  return c->kind == BN_KV8_INT8 ? bn::attend_kind<BN_KV8_INT8, false>(a, p.mt, s) : bn::attend_kind<BN_KV8_E4M3, false>(a, p.mt, s);
 }

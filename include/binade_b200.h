@@ -305,7 +305,8 @@ int bn_attention(const uint16_t *q, int64_t q_token, int64_t q_head, const uint1
                  void *stream);
 
 /* A key/value cache in 8 bits with a scale for each block of tokens and head:
- *   k, v       [batch, kv_heads, rows, D] codes of the full blocks; rows: max_seq rounded up to 64
+ *   k          [batch, kv_heads, rows, D] codes of the full blocks; rows: max_seq rounded up to 64
+ *   v          [batch, kv_heads, rows / 4, D, 4] the same with four tokens of a dimension side by side
  *   k_scale,   [batch, kv_heads, rows / block]: a value is its code times the scale of its block
  *   v_scale
  *   k_tail,    [batch, kv_heads, 2, block, D] BF16: the tokens of the block that is not full yet. What a

@@ -68,7 +68,7 @@ _SIGNATURES = {
         "bn_attention": [_vp, _i64, _i64] * 3 + [_i64] * 4 + [_vp, _i64, _vp, C.POINTER(Scores), _vp, _i64, _i64, _int, _vp],
         "bn_kv8_append": [C.POINTER(KV8Struct), _vp, _i64, _i64, _i64, _vp, _i64, _i64, _i64, _i64, _vp, _vp],
         "bn_kv8_workspace": [C.POINTER(KV8Struct), _i64, _i64],
-        "bn_kv8_attend": [C.POINTER(KV8Struct), _vp, _i64, _i64, _i64, _i64, _i64, _vp, _vp, C.POINTER(Scores), _vp, _i64, _i64, _i64, _int, _vp, _u64, _vp],
+        "bn_kv8_attend": [C.POINTER(KV8Struct), *[_vp, _i64, _i64, _i64] * 3, _i64, _i64, _vp, _vp, C.POINTER(Scores), _vp, _i64, _i64, _i64, _int, _vp, _u64, _vp],
         "bn_kv8_advance": [C.POINTER(KV8Struct), _i64, _vp, _vp],
         "bn_kv8_dense": [C.POINTER(KV8Struct), _vp, _vp, _vp],
         "bn_token_counts": [_vp, _int, _i64, _i64, _i64, _vp, _i64, _int, _vp, _i64, _vp, _i64, _vp],

@@ -10,15 +10,18 @@ __device__ int g_kv8_error;  // 1: tokens were brought that the cache has no roo
 namespace {
 
 // The nearest code to x / scale, ties to the even one, for finite x; 0 for NaN, the largest code for an infinity.
-__device__ __forceinline__ uint32_t int8_code(float x, float scale) {
-  float t = __fdiv_rn(x, scale), q = rintf(t);
-  if (fabsf(t - q) == 0.5f) {  // the rounded quotient lies between two codes: the real one may lie to either side
-    const float r = fmaf(-t, scale, x);
-    if (r > 0.0f) q = ceilf(t);
-    if (r < 0.0f) q = floorf(t);
+// As stored, with 128 added. x times the inverse is off by at most 2^-15 in a quotient of up to 127: only next to the
+// middle of two codes the real quotient decides, by the sign of x - middle * scale, which one rounding keeps.
+__device__ __forceinline__ uint32_t int8_code(float x, float scale, float inv) {
+  const float t = x * inv;
+  int q = __float2int_rn(t);  // NaN: 0
+  const float off = t - (float)q;
+  if (fabsf(fabsf(off) - 0.5f) < 0.0005f) {
+    const float middle = (float)q + (off > 0.0f ? 0.5f : -0.5f), side = fmaf(-middle, scale, x);
+    const int below = (int)floorf(middle);
+    q = side > 0.0f ? below + 1 : side < 0.0f ? below : below + (below & 1);
   }
-  q = fminf(fmaxf(q, -127.0f), 127.0f);
-  return x == x ? (uint32_t)((int)q + 128) : 128u;  // stored with 128 added
+  return (uint32_t)(min(max(q, -127), 127) + 128);
 }
 
 // Least power of two, at least 2^-100, times which 448 (the largest e4m3 value) is not below amax.
@@ -50,6 +53,8 @@ template <int CHUNKS>
 __global__ void __launch_bounds__(128) append_kernel(const __grid_constant__ AppendArgs a) {
   const bn_kv8 &c = a.c;
   __shared__ float part_max[4];
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // what made the tokens, and what read the cache before
   uint32_t at = blockIdx.x;
   const bool values = at & 1;
   at >>= 1;
@@ -107,7 +112,7 @@ __global__ void __launch_bounds__(128) append_kernel(const __grid_constant__ App
     __syncthreads();
     amax = fmaxf(fmaxf(part_max[0], part_max[1]), fmaxf(part_max[2], part_max[3]));
     const float scale = c.kind == KV8_INT8 ? fmaxf(__fdiv_rn(amax, 127.0f), 7.888609052210118e-31f) : e4m3_scale(amax);
-    const float inv = __frcp_rn(scale);  // of a power of two: exact
+    const float inv = __frcp_rn(scale);  // (of a power of two: exact)
     uint8_t *const codes = (values ? c.v : c.k) + (unit * c.rows + (int64_t)j * block) * D;
     if (threadIdx.x == 0) (values ? c.v_scale : c.k_scale)[unit * (c.rows / block) + j] = scale;
 #pragma unroll
@@ -118,7 +123,7 @@ __global__ void __launch_bounds__(128) append_kernel(const __grid_constant__ App
       for (int e = 0; e < 2; e++) {
         float f[4] = {__uint_as_float(w[2 * e] << 16), __uint_as_float(w[2 * e] & 0xFFFF0000u), __uint_as_float(w[2 * e + 1] << 16), __uint_as_float(w[2 * e + 1] & 0xFFFF0000u)};
         if (c.kind == KV8_INT8) {
-          out[e] = int8_code(f[0], scale) | int8_code(f[1], scale) << 8 | int8_code(f[2], scale) << 16 | int8_code(f[3], scale) << 24;
+          out[e] = int8_code(f[0], scale, inv) | int8_code(f[1], scale, inv) << 8 | int8_code(f[2], scale, inv) << 16 | int8_code(f[3], scale, inv) << 24;
         } else {
 #pragma unroll
           for (int n = 0; n < 4; n++) f[n] = f[n] == f[n] ? f[n] * inv : 0.0f;
@@ -140,38 +145,47 @@ __global__ void __launch_bounds__(256) advance_kernel(const __grid_constant__ bn
 }
 
 // Eight values a thread, of keys eight of a token, of values two of four tokens, as the codes lie; tokens that the
-// cache does not hold as zeros.
-template <int KIND>
+// cache does not hold as zeros. Blocks: pieces of a sequence and head, those, and keys or values.
+template <int KIND, int D>
 __global__ void __launch_bounds__(256) dense_kernel(const __grid_constant__ bn_kv8 c, float *__restrict__ k, float *__restrict__ v) {
-  const bool values = blockIdx.y;
-  const int D = (int)c.D;
-  const int64_t per_unit = values ? (c.max_seq + 3) / 4 * (D / 2) : c.max_seq * (D / 8);
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, unit = i / per_unit;
-  if (unit >= c.batch * c.kv_heads) return;
-  const int64_t at = i % per_unit;
+  const bool values = blockIdx.z;
+  const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x, units = c.batch * c.kv_heads;
   const int row = (int)(values ? at / (D / 2) * 4 : at / (D / 8)), col = (int)(values ? at % (D / 2) * 2 : at % (D / 8) * 8);
-  const int64_t b = unit / c.kv_heads;
-  const int length = min(max(c.length[b], 0), (int)c.max_seq), full = length / c.block * c.block;
-  float x[8] = {};
-  if (row < full) {  // (a block has whole rows of four)
-    const float scale = (values ? c.v_scale : c.k_scale)[unit * (c.rows / c.block) + row / c.block];
-    const uint2 w = *reinterpret_cast<const uint2 *>((values ? c.v : c.k) + (unit * c.rows + row) * D + (values ? 4 : 1) * col);
+  if (row >= c.max_seq) return;
+  const int block_log2 = 31 - __clz(c.block);
+  for (int64_t unit = blockIdx.y; unit < units; unit += gridDim.y) {
+    const int64_t b = (int)unit / (int)c.kv_heads;
+    const int length = min(max(c.length[b], 0), (int)c.max_seq), full = length >> block_log2 << block_log2;
+    float x[8] = {};
+    if (row < full) {  // (a block has whole rows of four)
+      const float scale = (values ? c.v_scale : c.k_scale)[unit * (c.rows >> block_log2) + (row >> block_log2)];
+      const uint2 w = *reinterpret_cast<const uint2 *>((values ? c.v : c.k) + (unit * c.rows + row) * D + (values ? 4 : 1) * col);
 #pragma unroll
-    for (int e = 0; e < 8; e++) x[e] = kv8_code<KIND>(((e < 4 ? w.x : w.y) >> (8 * (e & 3))) & 0xFFu) * scale;
-  } else {
-    const uint16_t *const tail = (values ? c.v_tail : c.k_tail) + ((unit * 2 + (c.side[b] & 1)) * c.block + row - full) * D + col;
+      for (int e = 0; e < 8; e++) x[e] = kv8_code<KIND>(((e < 4 ? w.x : w.y) >> (8 * (e & 3))) & 0xFFu) * scale;
+    } else if (row < length) {
+      const uint16_t *const tail = (values ? c.v_tail : c.k_tail) + ((unit * 2 + (c.side[b] & 1)) * c.block + row - full) * D + col;
 #pragma unroll
-    for (int e = 0; e < 8; e++)
-      if (row + (values ? e & 3 : 0) < length) x[e] = bf16_to_f32(tail[values ? (e & 3) * D + (e >> 2) : e]);
+      for (int e = 0; e < 8; e++)
+        if (row + (values ? e & 3 : 0) < length) x[e] = bf16_to_f32(tail[values ? (e & 3) * D + (e >> 2) : e]);
+    }
+    if (values) {
+#pragma unroll
+      for (int e = 0; e < 4; e++)
+        if (row + e < c.max_seq) *reinterpret_cast<float2 *>(v + (unit * c.max_seq + row + e) * D + col) = make_float2(x[e], x[4 + e]);
+    } else {
+      float4 *const out = reinterpret_cast<float4 *>(k + (unit * c.max_seq + row) * D + col);
+      out[0] = make_float4(x[0], x[1], x[2], x[3]), out[1] = make_float4(x[4], x[5], x[6], x[7]);
+    }
   }
-  if (values) {
-#pragma unroll
-    for (int e = 0; e < 4; e++)
-      if (row + e < c.max_seq) *reinterpret_cast<float2 *>(v + (unit * c.max_seq + row + e) * D + col) = make_float2(x[e], x[4 + e]);
-  } else {
-    float4 *const out = reinterpret_cast<float4 *>(k + (unit * c.max_seq + row) * D + col);
-    out[0] = make_float4(x[0], x[1], x[2], x[3]), out[1] = make_float4(x[4], x[5], x[6], x[7]);
-  }
+}
+
+template <int KIND>
+int dense_launch(const bn_kv8 &c, float *k, float *v, cudaStream_t s) {
+  const int64_t units = c.batch * c.kv_heads, pieces = ((c.max_seq + 3) / 4 * 4 * (c.D / 8) + 255) / 256;
+  const dim3 grid((unsigned)pieces, (unsigned)(units < 65535 ? units : 65535), 2);
+  auto kern = c.D == 64 ? dense_kernel<KIND, 64> : c.D == 128 ? dense_kernel<KIND, 128> : dense_kernel<KIND, 256>;
+  kern<<<grid, 256, 0, s>>>(c, k, v);
+  return launched("dense_kernel");
 }
 
 }  // namespace
@@ -206,7 +220,12 @@ extern "C" int bn_kv8_append(const bn_kv8 *c, const uint16_t *k, int64_t k_seq, 
   if (blocks > 0x7FFFFFFF) return bn::fail(BN_ERR_ARG, "bn_kv8_append: too many tokens for one call");
   const int chunks = (int)(c->block * c->D / 1024);
   auto kern = chunks == 1 ? bn::append_kernel<1> : chunks == 2 ? bn::append_kernel<2> : chunks == 4 ? bn::append_kernel<4> : chunks == 8 ? bn::append_kernel<8> : bn::append_kernel<16>;
-  kern<<<(unsigned)blocks, 128, 0, (cudaStream_t)stream>>>(a);
+  cudaLaunchConfig_t cfg{};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.gridDim = dim3((unsigned)blocks), cfg.blockDim = dim3(128), cfg.stream = (cudaStream_t)stream, cfg.attrs = attr, cfg.numAttrs = 1;
+  BN_CUDA(cudaLaunchKernelEx(&cfg, kern, a));
   return bn::launched("append_kernel");
 }
 
@@ -220,10 +239,6 @@ extern "C" int bn_kv8_advance(const bn_kv8 *c, int64_t n, const int32_t *counts,
 extern "C" int bn_kv8_dense(const bn_kv8 *c, float *k, float *v, void *stream) {
   if (const char *why = bn::kv8_refusal(c)) return bn::refuse("bn_kv8_dense", why);
   if (!k || !v || ((uintptr_t)k | (uintptr_t)v) & 15) return bn::fail(BN_ERR_ARG, "bn_kv8_dense: outputs have to start on 16 bytes");
-  const int64_t blocks = (c->batch * c->kv_heads * ((c->max_seq + 3) / 4 * 4) * (c->D / 8) + 255) / 256;
-  if (blocks > 0x7FFFFFFF) return bn::fail(BN_ERR_ARG, "bn_kv8_dense: the cache is too large for one call");
-  const dim3 grid((unsigned)blocks, 2);
-  if (c->kind == BN_KV8_INT8) bn::dense_kernel<BN_KV8_INT8><<<grid, 256, 0, (cudaStream_t)stream>>>(*c, k, v);
-  else bn::dense_kernel<BN_KV8_E4M3><<<grid, 256, 0, (cudaStream_t)stream>>>(*c, k, v);
-  return bn::launched("dense_kernel");
+  if (c->batch * c->kv_heads > 0x7FFFFFFF) return bn::fail(BN_ERR_ARG, "bn_kv8_dense: the cache is too large for one call");
+  return c->kind == BN_KV8_INT8 ? bn::dense_launch<BN_KV8_INT8>(*c, k, v, (cudaStream_t)stream) : bn::dense_launch<BN_KV8_E4M3>(*c, k, v, (cudaStream_t)stream);
 }

@@ -603,78 +603,73 @@ __global__ void __launch_bounds__(WARPS * 32, (D == 64 && MT == 1) ? 4 : (MT * D
 }
 
 // Joins what blocks left of a sequence and head that was cut, and zeroes the rows of sequences that brought nothing.
-// A block per sequence, head and row group: first the rows' maxima over the parts and the factors that go with them,
-// then the sums, four dimensions a thread, the parts in groups where there are few rows.
-constexpr int JOIN_THREADS = 256, JOIN_PARTS = 64;
+// A block per query row: a thread has four dimensions of every few parts.
+constexpr int JOIN_THREADS = 256;
 
 template <int D, int MT>
 __global__ void __launch_bounds__(JOIN_THREADS) join_kernel(const __grid_constant__ AttendArgs a) {
   using S = Shape<D, MT>;
-  __shared__ float factor[JOIN_PARTS][S::ROWS], tops[S::ROWS], weights[S::ROWS];
+  constexpr int COLS = D / 4, GROUPS = JOIN_THREADS / COLS;
+  __shared__ float tops[JOIN_THREADS / 32], weights[16];
   __shared__ float4 sums[JOIN_THREADS];
-  const int per_seq = (int)a.c.kv_heads * a.row_groups;
-  const int64_t b = blockIdx.x / per_seq;
-  const int hr = (int)(blockIdx.x % per_seq), kv = hr / a.row_groups, row0 = hr % a.row_groups * S::ROWS, rows = min(S::ROWS, a.group * a.tokens - row0);
+  const int all_rows = a.group * a.tokens, per_seq = (int)a.c.kv_heads * a.row_groups;
+  const int unit = (int)(blockIdx.x / (unsigned)all_rows), r = (int)(blockIdx.x % (unsigned)all_rows);
+  const int64_t b = unit / (int)a.c.kv_heads;
+  const int kv = unit % (int)a.c.kv_heads, hr = kv * a.row_groups + r / S::ROWS, row = r % S::ROWS;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int64_t tiles = a.plan[b + 1] - a.plan[b], share = a.plan[a.c.batch + 1];
-  const int64_t from = a.plan[b] * per_seq + hr * tiles, to = from + tiles;
-  if (tiles && from / share == (to - 1) / share) return;  // one block's: it wrote the output
+  const int64_t before = a.plan[b], tiles = a.plan[b + 1] - before, share = a.plan[a.c.batch + 1];
+  const int64_t from = before * per_seq + hr * tiles, to = from + tiles;
+  // (blocks and tiles of a launch both count to less than 2^53: doubles divide them, and the products check)
+  int64_t first = (int64_t)((double)from / (double)share);
+  if (first * share > from) first--;
+  if ((first + 1) * share <= from) first++;
+  const int t = r / a.group, head = kv * a.group + r % a.group;
+  uint16_t *const out = a.out + b * a.o_seq + t * a.o_token + head * a.o_head;
+  if (tiles == 0) {
+    if (a.zero_rest)
+      for (int i = (int)threadIdx.x; i < D / 8; i += JOIN_THREADS) *reinterpret_cast<uint4 *>(out + 8 * i) = make_uint4(0, 0, 0, 0);
+    return;
+  }
+  if ((first + 1) * share >= to) return;  // one block's: it wrote the output
+  int parts = 1;
+  while ((first + parts) * share < to) parts += max(1, (int)((to - (first + parts) * share) / share));
+  auto part_of = [&](int p) { return a.parts + ((first + p) * 2 + (p == 0 && from != first * share ? 1 : 0)) * S::PART; };
+  float m = NOTHING;
+  for (int p = (int)threadIdx.x; p < parts; p += JOIN_THREADS) m = fmaxf(m, part_of(p)[S::ROWS * D + row]);
+#pragma unroll
+  for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(BN_FULL, m, d));
+  if (lane_id() == 0) tops[threadIdx.x >> 5] = m;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < JOIN_THREADS / 32; w++) m = fmaxf(m, tops[w]);
+  const int g = (int)threadIdx.x / COLS, col = (int)threadIdx.x % COLS * 4;
+  float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  float l = 0.0f;
+#pragma unroll 4
+  for (int p = g; p < parts; p += GROUPS) {
+    const float *const part = part_of(p);
+    const float f = ex2(part[S::ROWS * D + row] - m);
+    const float4 v = *reinterpret_cast<const float4 *>(part + row * D + col);
+    l = fmaf(f, part[S::ROWS * D + S::ROWS + row], l);
+    o.x = fmaf(f, v.x, o.x), o.y = fmaf(f, v.y, o.y), o.z = fmaf(f, v.z, o.z), o.w = fmaf(f, v.w, o.w);
+  }
+  sums[threadIdx.x] = o;
+  if (col == 0) weights[g] = l;
+  static_assert(GROUPS <= 16, "");
+  __syncthreads();
+  if (g) return;
+  for (int k = 1; k < GROUPS; k++) {
+    const float4 v = sums[(int)threadIdx.x + k * COLS];
+    o.x += v.x, o.y += v.y, o.z += v.z, o.w += v.w, l += weights[k];
+  }
   int held, brought;
   kv8_tokens(a.c, a.counts, a.tokens, b, held, brought);
-  const int first = (int)(from / share), parts = tiles ? (int)((to - 1) / share) - first + 1 : 0;
-  auto part_of = [&](int p) { return a.parts + ((int64_t)(first + p) * 2 + (p == 0 && from != first * share ? 1 : 0)) * S::PART; };
-  const int warp = (int)(threadIdx.x >> 5), lane = (int)lane_id();
-  for (int row = warp; row < rows; row += JOIN_THREADS / 32) {
-    float m = NOTHING, l = 0.0f;
-    for (int p = lane; p < parts; p += 32) m = fmaxf(m, part_of(p)[S::ROWS * D + row]);
-#pragma unroll
-    for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(BN_FULL, m, d));
-    for (int p = lane; p < parts; p += 32) {
-      const float *const part = part_of(p);
-      l = fmaf(ex2(part[S::ROWS * D + row] - m), part[S::ROWS * D + S::ROWS + row], l);
-    }
-#pragma unroll
-    for (int d = 16; d; d >>= 1) l += __shfl_xor_sync(BN_FULL, l, d);
-    if (lane == 0) tops[row] = m, weights[row] = l;
-  }
-  const int tasks = rows * (D / 4), groups = max(1, JOIN_THREADS / tasks);
-  for (int i0 = 0; i0 < tasks; i0 += JOIN_THREADS) {
-    const int g = groups > 1 ? (int)threadIdx.x / tasks : 0, i = i0 + (groups > 1 ? (int)threadIdx.x % tasks : (int)threadIdx.x);
-    const int row = min(i, tasks - 1) / (D / 4), col = i % (D / 4) * 4;
-    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    for (int p0 = 0; p0 < parts; p0 += JOIN_PARTS) {
-      const int some = min(JOIN_PARTS, parts - p0);
-      __syncthreads();
-      for (int k = (int)threadIdx.x; k < some * rows; k += JOIN_THREADS) factor[k / rows][k % rows] = ex2(part_of(p0 + k / rows)[S::ROWS * D + k % rows] - tops[k % rows]);
-      __syncthreads();
-      if (g < groups && i < tasks) {
-#pragma unroll 8
-        for (int p = g; p < some; p += groups) {
-          const float f = factor[p][row];
-          const float4 v = *reinterpret_cast<const float4 *>(part_of(p0 + p) + row * D + col);
-          o.x = fmaf(f, v.x, o.x), o.y = fmaf(f, v.y, o.y), o.z = fmaf(f, v.z, o.z), o.w = fmaf(f, v.w, o.w);
-        }
-      }
-    }
-    if (groups > 1) {
-      sums[threadIdx.x] = o;
-      __syncthreads();
-      for (int k = 1; g == 0 && k < groups; k++) {
-        const float4 v = sums[(int)threadIdx.x + k * tasks];
-        o.x += v.x, o.y += v.y, o.z += v.z, o.w += v.w;
-      }
-    }
-    if (g == 0 && i < tasks) {
-      const int t = (row0 + row) / a.group, head = kv * a.group + (row0 + row) % a.group;
-      uint16_t *const out = a.out + b * a.o_seq + t * a.o_token + head * a.o_head + col;
-      if (t < brought) {
-        const float inv = 1.0f / weights[row];
-        *reinterpret_cast<uint2 *>(out) = make_uint2(pack_bf16(o.x * inv, o.y * inv), pack_bf16(o.z * inv, o.w * inv));
-      } else if (a.zero_rest) {
-        *reinterpret_cast<uint2 *>(out) = make_uint2(0, 0);
-      }
-    }
+  if (t < brought) {
+    const float inv = 1.0f / l;
+    *reinterpret_cast<uint2 *>(out + col) = make_uint2(pack_bf16(o.x * inv, o.y * inv), pack_bf16(o.z * inv, o.w * inv));
+  } else if (a.zero_rest) {
+    *reinterpret_cast<uint2 *>(out + col) = make_uint2(0, 0);
   }
 }
 
@@ -717,7 +712,7 @@ int attend_launch(const AttendArgs &a, cudaStream_t stream) {
   cfg.gridDim = dim3((unsigned)a.blocks), cfg.blockDim = dim3(WARPS * 32), cfg.dynamicSmemBytes = S::SMEM, cfg.stream = stream, cfg.attrs = attr, cfg.numAttrs = 1;
   BN_CUDA(allow_smem(attend_kernel<D, KIND, MT, PLAIN>, S::SMEM));
   BN_CUDA(cudaLaunchKernelEx(&cfg, attend_kernel<D, KIND, MT, PLAIN>, a));
-  cfg.gridDim = dim3((unsigned)(a.c.batch * a.c.kv_heads * a.row_groups)), cfg.blockDim = dim3(JOIN_THREADS), cfg.dynamicSmemBytes = 0;
+  cfg.gridDim = dim3((unsigned)(a.c.batch * a.heads * a.tokens)), cfg.blockDim = dim3(JOIN_THREADS), cfg.dynamicSmemBytes = 0;
   BN_CUDA(cudaLaunchKernelEx(&cfg, join_kernel<D, MT>, a));
   return launched("attend_kernel");
 }
@@ -739,16 +734,18 @@ extern "C" uint64_t bn_kv8_workspace(const bn_kv8 *c, int64_t tokens, int64_t he
   return bn::plan_of(c, tokens, heads).bytes;
 }
 
-extern "C" int bn_kv8_attend(const bn_kv8 *c, const uint16_t *q, int64_t q_seq, int64_t q_token, int64_t q_head, int64_t tokens, int64_t heads, const int32_t *counts, const int32_t *prefix, const bn_scores *scores, uint16_t *out, int64_t o_seq, int64_t o_token, int64_t o_head, int zero_rest, void *workspace, uint64_t workspace_bytes, void *stream) {
+extern "C" int bn_kv8_attend(const bn_kv8 *c, const uint16_t *q, int64_t q_seq, int64_t q_token, int64_t q_head, const uint16_t *k, int64_t k_seq, int64_t k_token, int64_t k_head, const uint16_t *v, int64_t v_seq, int64_t v_token, int64_t v_head, int64_t tokens, int64_t heads, const int32_t *counts, const int32_t *prefix, const bn_scores *scores, uint16_t *out, int64_t o_seq, int64_t o_token, int64_t o_head, int zero_rest, void *workspace, uint64_t workspace_bytes, void *stream) {
   if (const char *why = bn::kv8_refusal(c)) return bn::refuse("bn_kv8_attend", why);
   if (!bn::attend_sizes(c, tokens, heads)) return bn::fail(BN_ERR_ARG, "bn_kv8_attend: bad size (query heads have to be a multiple of the cache's heads)");
-  if (!scores || (tokens && (!q || !out))) return bn::fail(BN_ERR_ARG, "bn_kv8_attend: null pointer");
+  if (!scores || (tokens && (!q || !out)) || !k != !v) return bn::fail(BN_ERR_ARG, "bn_kv8_attend: null pointer");
   if (((uintptr_t)q | (uintptr_t)out) & 15 || (q_seq | q_token | q_head | o_seq | o_token | o_head) & 7) return bn::fail(BN_ERR_ARG, "bn_kv8_attend: rows have to start on 16 bytes");
   if (scores->window < 0 || scores->window > 0x3FFFFFFF || !(scores->softcap >= 0.0f)) return bn::fail(BN_ERR_ARG, "bn_kv8_attend: negative window or cap");
   if (tokens == 0) return BN_OK;
   const bn::Plan p = bn::plan_of(c, tokens, heads);
   if (!workspace || (uintptr_t)workspace & 15 || workspace_bytes < p.bytes) return bn::fail(BN_ERR_CAPACITY, "bn_kv8_attend: the workspace is smaller than bn_kv8_workspace says, or not on 16 bytes");
-  if (c->batch * c->kv_heads * p.row_groups > 0x7FFFFFFF) return bn::fail(BN_ERR_ARG, "bn_kv8_attend: too many rows for one call");
+  if (c->batch * heads * tokens > 0x7FFFFFFF) return bn::fail(BN_ERR_ARG, "bn_kv8_attend: too many rows for one call");
+  if (k)
+    if (const int e = bn_kv8_append(c, k, k_seq, k_token, k_head, v, v_seq, v_token, v_head, tokens, counts, stream)) return e;
   bn::AttendArgs a{*c, q, out, q_seq, q_token, q_head, o_seq, o_token, o_head, counts, prefix, scores->slopes, (int)tokens, (int)heads, (int)(heads / c->kv_heads), (int)scores->window, scores->causal, zero_rest, scores->scale, scores->softcap, (int64_t *)workspace, (float *)((uint8_t *)workspace + p.plan_bytes), p.row_groups, p.blocks};
   const cudaStream_t s = (cudaStream_t)stream;
   if (scores->softcap == 0.0f && !scores->slopes) return c->kind == BN_KV8_INT8 ? bn::attend_kind<BN_KV8_INT8, true>(a, p.mt, s) : bn::attend_kind<BN_KV8_E4M3, true>(a, p.mt, s);

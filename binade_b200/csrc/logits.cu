@@ -50,7 +50,7 @@ __device__ __forceinline__ uint32_t four_bits(const uint32_t *__restrict__ words
 // by the bytes of the logits for many rows, by the latency of a chain of loads for one. Quads start where the output row
 // has 16-byte boundaries (rows of an odd vocabulary start anywhere); the input is read in one piece
 // where its row has them at the same places. Counts are read only where a token was said.
-template <typename T, int THREADS>
+template <typename T, int THREADS, int U>
 __global__ void __launch_bounds__(THREADS) logits_kernel(const __grid_constant__ LogitsArgs a) {
   namespace cg = cooperative_groups;
   cg::cluster_group cluster = cg::this_cluster();
@@ -66,57 +66,80 @@ __global__ void __launch_bounds__(THREADS) logits_kernel(const __grid_constant__
   const bool whole_x = (((uintptr_t)(x - shift)) & (4 * sizeof(T) - 1)) == 0, whole_bias = bias && ((uintptr_t)(bias - shift) & 15) == 0;
   const int V = a.V, quads = (V + shift + 3) / 4;
   Best best{-CUDART_INF_F, -1};
-  for (int k = blockIdx.x * THREADS + threadIdx.x; k < quads; k += gridDim.x * THREADS) {
-    const int t = 4 * k - shift;
-    const bool inside = t >= 0 && t + 3 < V;
-    float y[4], add[4] = {};
-    if (inside && whole_x) {
-      if constexpr (sizeof(T) == 2) {
-        const uint2 w = *reinterpret_cast<const uint2 *>(x + t);
-        y[0] = __uint_as_float(w.x << 16), y[1] = __uint_as_float(w.x & 0xFFFF0000u), y[2] = __uint_as_float(w.y << 16), y[3] = __uint_as_float(w.y & 0xFFFF0000u);
+  // U quads a thread at a time, first all their loads, so that the few tokens that were said (whose counts are
+  // a second load behind the first) wait once
+  const int stride = (int)gridDim.x * THREADS;
+  for (int k0 = blockIdx.x * THREADS + threadIdx.x; k0 < quads; k0 += U * stride) {
+    float y[U][4], add[U][4];
+    uint32_t said[U], open[U];
+    int n[U][4];
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      const int t = 4 * (k0 + u * stride) - shift;
+      const bool inside = t >= 0 && t + 3 < V;
+      said[u] = 0, open[u] = 15;
+      if (k0 + u * stride >= quads) continue;
+      if (inside && whole_x) {
+        if constexpr (sizeof(T) == 2) {
+          const uint2 w = *reinterpret_cast<const uint2 *>(x + t);
+          y[u][0] = __uint_as_float(w.x << 16), y[u][1] = __uint_as_float(w.x & 0xFFFF0000u), y[u][2] = __uint_as_float(w.y << 16), y[u][3] = __uint_as_float(w.y & 0xFFFF0000u);
+        } else {
+          const float4 w = *reinterpret_cast<const float4 *>(x + t);
+          y[u][0] = w.x, y[u][1] = w.y, y[u][2] = w.z, y[u][3] = w.w;
+        }
       } else {
-        const float4 w = *reinterpret_cast<const float4 *>(x + t);
-        y[0] = w.x, y[1] = w.y, y[2] = w.z, y[3] = w.w;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          const int at = min(max(t + e, 0), V - 1);
+          if constexpr (sizeof(T) == 2) y[u][e] = __uint_as_float((uint32_t)x[at] << 16);
+          else y[u][e] = x[at];
+        }
       }
-    } else {
+      if (seen) said[u] = four_bits(seen, t, V) & 15u;
+      if (mask) open[u] = four_bits(mask, t, V) & 15u;
+      if (bias) {
+        if (inside && whole_bias) {
+          const float4 w = *reinterpret_cast<const float4 *>(bias + t);
+          add[u][0] = w.x, add[u][1] = w.y, add[u][2] = w.z, add[u][3] = w.w;
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; e++) add[u][e] = bias[min(max(t + e, 0), V - 1)];
+        }
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      const int t = 4 * (k0 + u * stride) - shift;
 #pragma unroll
       for (int e = 0; e < 4; e++) {
-        const int at = min(max(t + e, 0), V - 1);
-        if constexpr (sizeof(T) == 2) y[e] = __uint_as_float((uint32_t)x[at] << 16);
-        else y[e] = x[at];
+        if (t + e < 0 || t + e >= V) said[u] &= ~(1u << e);
+        n[u][e] = (said[u] >> e) & 1u ? counts[t + e] : 0;
       }
     }
-    const uint32_t said = seen ? four_bits(seen, t, V) & 15u : 0u, open = mask ? four_bits(mask, t, V) & 15u : 15u;
-    if (bias) {
-      if (inside && whole_bias) {
-        const float4 w = *reinterpret_cast<const float4 *>(bias + t);
-        add[0] = w.x, add[1] = w.y, add[2] = w.z, add[3] = w.w;
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      const int t = 4 * (k0 + u * stride) - shift;
+      if (k0 + u * stride >= quads) break;
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        // every operation rounds by itself, in the order of the definition: a plain evaluation gives the same bits
+        float &z = y[u][e];
+        if ((said[u] >> e) & 1u) {
+          z = z > 0.0f ? __fdiv_rn(z, repetition) : __fmul_rn(z, repetition);
+          if (n[u][e] > 0) z = __fsub_rn(z, __fadd_rn(__fmul_rn(frequency, (float)n[u][e]), presence));
+        }
+        if (bias) z = __fadd_rn(z, add[u][e]);
+        if (!((open[u] >> e) & 1u)) z = -CUDART_INF_F;
+        if (z > best.value && t + e >= 0 && t + e < V) best = {z, t + e};  // (NaN is never chosen)
+      }
+      if (t >= 0 && t + 3 < V) {
+        *reinterpret_cast<float4 *>(out + t) = make_float4(y[u][0], y[u][1], y[u][2], y[u][3]);
       } else {
 #pragma unroll
-        for (int e = 0; e < 4; e++) add[e] = bias[min(max(t + e, 0), V - 1)];
+        for (int e = 0; e < 4; e++)
+          if (t + e >= 0 && t + e < V) out[t + e] = y[u][e];
       }
     }
-#pragma unroll
-    for (int e = 0; e < 4; e++) {
-      // every operation rounds by itself, in the order of the definition: a plain evaluation gives the same bits
-      if (((said >> e) & 1u) && t + e >= 0 && t + e < V) {
-        y[e] = y[e] > 0.0f ? __fdiv_rn(y[e], repetition) : __fmul_rn(y[e], repetition);
-        const int n = counts[t + e];
-        if (n > 0) y[e] = __fsub_rn(y[e], __fadd_rn(__fmul_rn(frequency, (float)n), presence));
-      }
-      if (bias) y[e] = __fadd_rn(y[e], add[e]);
-      if (!((open >> e) & 1u)) y[e] = -CUDART_INF_F;
-    }
-    if (inside) {
-      *reinterpret_cast<float4 *>(out + t) = make_float4(y[0], y[1], y[2], y[3]);
-    } else {
-#pragma unroll
-      for (int e = 0; e < 4; e++)
-        if (t + e >= 0 && t + e < V) out[t + e] = y[e];
-    }
-#pragma unroll
-    for (int e = 0; e < 4; e++)
-      if (y[e] > best.value && t + e >= 0 && t + e < V) best = {y[e], t + e};  // (NaN is never chosen)
   }
 #pragma unroll
   for (int d = 16; d; d >>= 1) best = better(best, Best{__shfl_xor_sync(BN_FULL, best.value, d), __shfl_xor_sync(BN_FULL, best.at, d)});
@@ -152,19 +175,21 @@ extern "C" int bn_logits(const void *x, int fp32, int64_t x_row, int64_t batch, 
   if (batch < 0 || batch > 65535 || V < 1 || V > 0x3FFFFFFF) return bn::fail(BN_ERR_ARG, "bn_logits: bad size");
   if (!rules || (batch && (!x || !out || !token)) || (rules && rules->seen && !rules->counts)) return bn::fail(BN_ERR_ARG, "bn_logits: null pointer");
   if (batch == 0) return BN_OK;
-  constexpr int threads = 512;
+  constexpr int threads = 512, quads = 2;
   bn::LogitsArgs a{x, out, token, x_row, out_row, (int)V, *rules};
-  // blocks of a row: one per 512 quads, up to 8 (the portable cluster size)
-  const int64_t need = (V + 4 * threads - 1) / (4 * threads);
+  // blocks of a row: up to 8 (the portable cluster size), 16 where the rows are few
+  const int64_t need = (V + 4 * threads * quads - 1) / (4 * threads * quads);
+  const unsigned most = batch <= 8 ? 16 : 8;
   unsigned blocks = 1;
-  while (blocks < 8 && blocks < need) blocks *= 2;
+  while (blocks < most && blocks < need) blocks *= 2;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(blocks, (unsigned)batch), cfg.blockDim = dim3(threads), cfg.stream = (cudaStream_t)stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = blocks, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr, cfg.numAttrs = 1;
-  if (fp32) BN_CUDA(cudaLaunchKernelEx(&cfg, bn::logits_kernel<float, threads>, a));
-  else BN_CUDA(cudaLaunchKernelEx(&cfg, bn::logits_kernel<uint16_t, threads>, a));
+  auto kern = fp32 ? bn::logits_kernel<float, threads, quads> : bn::logits_kernel<uint16_t, threads, quads>;
+  if (blocks > 8) BN_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+  BN_CUDA(cudaLaunchKernelEx(&cfg, kern, a));
   return bn::launched("logits_kernel");
 }

@@ -25,19 +25,18 @@ KINDS = {"int8": 0, "e4m3": 1}  # BN_KV8_INT8, BN_KV8_E4M3
 
 
 def _rows(t: torch.Tensor, name: str, dims: int, device) -> torch.Tensor:
-    """Checks a BF16 tensor of rows (its last dimension a head's) and gives it with rows that the kernels
-    can read: neighbouring elements, every row on 16 bytes."""
-    if not isinstance(t, torch.Tensor) or t.dtype != torch.bfloat16 or t.dim() != dims:
+    """Checks a BF16 tensor of rows (its last dimension a head's) on CUDA device number `device` and gives it with
+    rows that the kernels can read: neighbouring elements, every row on 16 bytes."""
+    if not isinstance(t, torch.Tensor) or t.dtype is not torch.bfloat16 or t.dim() != dims:
         raise ValueError(f"{name} has to be a bfloat16 tensor of {dims} dimensions")
-    if t.device != device:
-        raise ValueError(f"{name} is on {t.device}, the call on {device}")
+    if t.get_device() != device:
+        raise ValueError(f"{name} is on {t.device}, the call on cuda:{device}")
     if t.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{name} asks for a gradient: attention here has none (use torch.no_grad)")
-    if t.stride(-1) != 1 or t.data_ptr() % 16 or any(s % 8 for s, n in zip(t.stride()[:-1], t.shape[:-1]) if n > 1):
-        t = t.contiguous()
-        if t.data_ptr() % 16:
-            t = t.clone()
-    return t
+    if t.data_ptr() % 16 == 0 and (t.is_contiguous() or (t.stride(-1) == 1 and not any(s % 8 for s, n in zip(t.stride()[:-1], t.shape[:-1]) if n > 1))):
+        return t  # (a contiguous tensor's rows lie on 16 bytes: a head has 64 dimensions at least)
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
 def _steps(t: torch.Tensor):
@@ -48,8 +47,8 @@ def _steps(t: torch.Tensor):
 def _numbers(t, name: str, n: int, device, dtype=torch.int32) -> torch.Tensor | None:
     if t is None:
         return None
-    if not isinstance(t, torch.Tensor) or t.device != device or t.dim() != 1 or t.numel() != n or (dtype == torch.int32 and t.is_floating_point()):
-        raise ValueError(f"{name} has to be a tensor of {n} {'whole ' if dtype == torch.int32 else ''}numbers on {device}")
+    if not isinstance(t, torch.Tensor) or t.get_device() != device or t.dim() != 1 or t.numel() != n or (dtype == torch.int32 and t.is_floating_point()):
+        raise ValueError(f"{name} has to be a tensor of {n} {'whole ' if dtype == torch.int32 else ''}numbers on cuda:{device}")
     return t.to(dtype).contiguous()
 
 
@@ -66,8 +65,8 @@ def overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
 
 def _out(out, like: torch.Tensor, device, *inputs) -> torch.Tensor:
     if out is None:
-        return torch.empty(like.shape, dtype=torch.bfloat16, device=device)
-    if not isinstance(out, torch.Tensor) or out.dtype != torch.bfloat16 or out.shape != like.shape or out.device != device or out.requires_grad:
+        return torch.empty(like.shape, dtype=torch.bfloat16, device=like.device)
+    if not isinstance(out, torch.Tensor) or out.dtype != torch.bfloat16 or out.shape != like.shape or out.get_device() != device or out.requires_grad:
         raise ValueError("out has to be a bfloat16 tensor of q's shape on its device")
     if out.stride(-1) != 1 or out.data_ptr() % 16 or any(s % 8 or s == 0 for s, n in zip(out.stride()[:-1], out.shape[:-1]) if n > 1):
         raise ValueError("out's rows have to lie apart, each of neighbouring elements from a 16-byte boundary on")
@@ -76,8 +75,14 @@ def _out(out, like: torch.Tensor, device, *inputs) -> torch.Tensor:
     return out
 
 
+_score_structs: dict = {}  # bn_scores of calls without slopes, by their options
+
+
 def _scores(dim: int, heads: int, device, scale, softcap, window, slopes, causal):
     """The bn_scores of a call, and the slopes that it points at."""
+    options = (dim, scale, softcap, window, causal)
+    if slopes is None and options in _score_structs:
+        return _score_structs[options], None
     if softcap is not None and not (softcap > 0 and math.isfinite(softcap)):
         raise ValueError("softcap has to be a positive number")
     if window is not None and not 1 <= window < 1 << 30:
@@ -85,14 +90,18 @@ def _scores(dim: int, heads: int, device, scale, softcap, window, slopes, causal
     if scale is not None and not math.isfinite(scale):
         raise ValueError("scale has to be a finite number")
     slopes = _numbers(slopes, "slopes", heads, device, torch.float32)
-    return _native.Scores(1.0 / math.sqrt(dim) if scale is None else scale, softcap or 0.0, window or 0, ck._p(slopes), int(bool(causal))), slopes
+    made = _native.Scores(1.0 / math.sqrt(dim) if scale is None else scale, softcap or 0.0, window or 0, ck._p(slopes), int(bool(causal)))
+    if slopes is None:
+        if len(_score_structs) >= 64:
+            _score_structs.clear()
+        _score_structs[options] = made
+    return made, slopes
 
 
-def _device(t) -> torch.device:
-    dev = ck.require_cuda()
-    if not isinstance(t, torch.Tensor) or t.device != dev:
-        raise ValueError(f"q has to be a tensor on the current device, {dev}")
-    return dev
+def _device(t) -> int:
+    if not isinstance(t, torch.Tensor) or not t.is_cuda or t.get_device() != torch._C._cuda_getDevice():
+        raise ValueError(f"q has to be a tensor on the current device, {ck.require_cuda()}")
+    return t.get_device()
 
 
 def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets: torch.Tensor | None = None, *, causal: bool = True, scale: float | None = None, softcap: float | None = None, window: int | None = None, slopes: torch.Tensor | None = None, prefix: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
@@ -144,6 +153,7 @@ class KV8Cache:
         if dev.type != "cuda":
             raise ValueError(f"the cache lives on a CUDA device, not {dev}")
         self.device = dev if dev.index is not None else ck.require_cuda()
+        self._index, self._work = self.device.index, {}  # device number; workspace bytes by (tokens, heads)
         self.layers, self.batch, self.kv_heads, self.head_dim, self.max_seq, self.kind, self.block = layers, batch, kv_heads, head_dim, max_seq, kind, block
         rows = -(-max_seq // 64) * 64
         new = lambda *shape, dtype: torch.zeros((layers, batch, kv_heads, *shape), dtype=dtype, device=self.device)  # noqa: E731
@@ -160,12 +170,12 @@ class KV8Cache:
     def _layer(self, layer: int):
         if not 0 <= layer < self.layers:
             raise ValueError(f"layer {layer} of {self.layers}")
-        if torch.cuda.current_device() != self.device.index:
+        if torch._C._cuda_getDevice() != self._index:
             raise ValueError(f"the cache is on {self.device}, the current device is another one")
         return ctypes.byref(self._structs[layer])
 
     def _new(self, t, name: str, heads: int | None = None) -> torch.Tensor:
-        t = _rows(t, name, 4, self.device)
+        t = _rows(t, name, 4, self._index)
         if t.shape[0] != self.batch or t.shape[3] != self.head_dim or (heads is not None and t.shape[2] != heads):
             raise ValueError(f"{name} {tuple(t.shape)}: [batch {self.batch}, tokens, {'heads' if heads is None else heads}, {self.head_dim}] expected")
         return t
@@ -179,7 +189,7 @@ class KV8Cache:
         k, v = self._new(k, "k", self.kv_heads), self._new(v, "v", self.kv_heads)
         if k.shape != v.shape:
             raise ValueError(f"k {tuple(k.shape)} and v {tuple(v.shape)} differ")
-        counts = _numbers(counts, "counts", self.batch, self.device)
+        counts = _numbers(counts, "counts", self.batch, self._index)
         if k.shape[1]:
             ck._call("bn_kv8_append", at, ck._p(k), *_steps(k), ck._p(v), *_steps(v), k.shape[1], ck._p(counts))
 
@@ -196,18 +206,23 @@ class KV8Cache:
             raise ValueError(f"{heads} query heads over {self.kv_heads} key heads")
         if (k is None) != (v is None):
             raise ValueError("k and v come together")
-        counts = _numbers(counts, "counts", self.batch, self.device)
-        prefix = _numbers(prefix, "prefix", self.batch, self.device)
-        scores, slopes = _scores(self.head_dim, heads, self.device, scale, softcap, window, slopes, causal)
-        y = _out(out, q, self.device, q, k, v)
-        if k is not None:
-            if k.dim() != 4 or k.shape[1] != tokens:
-                raise ValueError(f"k {tuple(k.shape)} for {tokens} tokens")
-            self.append(layer, k, v, counts)
+        counts = _numbers(counts, "counts", self.batch, self._index)
+        prefix = _numbers(prefix, "prefix", self.batch, self._index)
+        scores, slopes = _scores(self.head_dim, heads, self._index, scale, softcap, window, slopes, causal)
+        y = _out(out, q, self._index, q, k, v)
+        if k is None:
+            new = (None, 0, 0, 0, None, 0, 0, 0)
+        else:
+            k, v = self._new(k, "k", self.kv_heads), self._new(v, "v", self.kv_heads)
+            if k.shape[1] != tokens or v.shape[1] != tokens:
+                raise ValueError(f"k {tuple(k.shape)} and v {tuple(v.shape)} for {tokens} tokens")
+            new = (k.data_ptr(), *_steps(k), v.data_ptr(), *_steps(v))
         if tokens:
-            need = _native.load("cuda").bn_kv8_workspace(at, tokens, heads)
-            work = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
-            ck._call("bn_kv8_attend", at, ck._p(q), *_steps(q), tokens, heads, ck._p(counts), ck._p(prefix), ctypes.byref(scores), ck._p(y), *_steps(y), int(out is None), ck._p(work), need)
+            need = self._work.get((tokens, heads))
+            if need is None:
+                need = self._work[tokens, heads] = _native.load("cuda").bn_kv8_workspace(at, tokens, heads)
+            work = torch.empty(need, dtype=torch.uint8, device=self.device)
+            ck._call("bn_kv8_attend", at, q.data_ptr(), *_steps(q), *new, tokens, heads, ck._p(counts), ck._p(prefix), ctypes.byref(scores), y.data_ptr(), *_steps(y), int(out is None), work.data_ptr(), need)
         return y
 
     def advance(self, n) -> None:
@@ -216,7 +231,7 @@ class KV8Cache:
         long as the new length lies in the block that was open before, in the one that is open behind all
         the tokens, or on a border of blocks."""
         at = self._layer(0)
-        counts = _numbers(n, "n", self.batch, self.device) if isinstance(n, torch.Tensor) else None
+        counts = _numbers(n, "n", self.batch, self._index) if isinstance(n, torch.Tensor) else None
         ck._call("bn_kv8_advance", at, 0 if counts is not None else n, ck._p(counts))
 
     def dense(self, layer: int):

@@ -40,7 +40,7 @@ class TokenCounts:
             tokens = tokens[:, None]
         if tokens.dim() != 2 or tokens.shape[0] != self.batch:
             raise ValueError(f"tokens {tuple(tokens.shape)} for a batch of {self.batch}")
-        if torch.cuda.current_device() != self.device.index:
+        if torch._C._cuda_getDevice() != self.device.index:
             raise ValueError(f"the counts are on {self.device}, the current device is another one")
         if tokens.shape[1] > 1 and tokens.stride(1) != 1:
             tokens = tokens.contiguous()
@@ -73,9 +73,9 @@ def process_logits(logits: torch.Tensor, said: TokenCounts | None = None, *, rep
     [ceil(vocab / 32)] or [batch, ceil(vocab / 32)], set = allowed) is clear the logit becomes -inf.
     Penalties are numbers or float tensors [batch]. tokens: each row's lowest index of its largest logit, -1 if
     nothing is left above -inf (NaN is never chosen). `out`: where to write the logits (may be `logits` itself if float32)."""
-    dev = ck.require_cuda()
-    if not isinstance(logits, torch.Tensor) or logits.dtype not in (torch.bfloat16, torch.float32) or logits.dim() != 2 or logits.device != dev:
-        raise ValueError(f"logits have to be bfloat16 or float32 [batch, vocab] on the current device, {dev}")
+    if not isinstance(logits, torch.Tensor) or logits.dtype not in (torch.bfloat16, torch.float32) or logits.dim() != 2 or not logits.is_cuda or logits.get_device() != torch._C._cuda_getDevice():
+        raise ValueError(f"logits have to be bfloat16 or float32 [batch, vocab] on the current device, {ck.require_cuda()}")
+    dev = logits.device
     if logits.requires_grad and torch.is_grad_enabled():
         raise ValueError("logits ask for a gradient: there is none here (use torch.no_grad)")
     batch, vocab = logits.shape

@@ -336,13 +336,14 @@ int bn_kv8_append(const bn_kv8 *c, const uint16_t *k, int64_t k_seq, int64_t k_t
                   const uint16_t *v, int64_t v_seq, int64_t v_token, int64_t v_head, int64_t tokens,
                   const int32_t *counts, void *stream);
 
-/* Attention of those tokens over everything up to themselves, after they were appended and before `length`
- * moves on: query t of sequence b has position length[b] + t, its keys are the length[b] + counts[b] first.
+/* Attention of those tokens over everything up to themselves, before `length` moves on. With k and v (NULL or not
+ * together) they are appended first; otherwise bn_kv8_append did it. Query t of sequence b has position length[b] + t, its keys are the length[b] + counts[b] first.
  * prefix [batch] or NULL. Rows of tokens that are not real are zeroed if zero_rest, else left as they are.
  * workspace: bn_kv8_workspace bytes on 16 bytes, for this call alone. */
 uint64_t bn_kv8_workspace(const bn_kv8 *c, int64_t tokens, int64_t heads);
 int bn_kv8_attend(const bn_kv8 *c, const uint16_t *q, int64_t q_seq, int64_t q_token, int64_t q_head,
-                  int64_t tokens, int64_t heads, const int32_t *counts, const int32_t *prefix,
+                  const uint16_t *k, int64_t k_seq, int64_t k_token, int64_t k_head, const uint16_t *v,
+                  int64_t v_seq, int64_t v_token, int64_t v_head, int64_t tokens, int64_t heads, const int32_t *counts, const int32_t *prefix,
                   const bn_scores *scores, uint16_t *out, int64_t o_seq, int64_t o_token, int64_t o_head,
                   int zero_rest, void *workspace, uint64_t workspace_bytes, void *stream);
 

@@ -49,7 +49,7 @@ def test_caches_refused(change):
     s = scores()
     for call in (
         lambda: _native.call("cuda", "bn_kv8_append", c, BUF, 256, 256, 128, BUF, 256, 256, 128, 1, None, None),
-        lambda: _native.call("cuda", "bn_kv8_attend", c, BUF, 512, 512, 128, 1, 4, None, None, C.byref(s), BUF, 512, 512, 128, 0, None, 0, None),
+        lambda: _native.call("cuda", "bn_kv8_attend", c, BUF, 512, 512, 128, None, 0, 0, 0, None, 0, 0, 0, 1, 4, None, None, C.byref(s), BUF, 512, 512, 128, 0, None, 0, None),
         lambda: _native.call("cuda", "bn_kv8_advance", c, 1, None, None),
         lambda: _native.call("cuda", "bn_kv8_dense", c, BUF, BUF, None),
     ):
@@ -57,12 +57,12 @@ def test_caches_refused(change):
             call()
 
 
-def attend(c=None, q=BUF, qs=(512, 512, 128), tokens=1, heads=4, s=None, out=BUF, os=(512, 512, 128), work=BUF, bytes=1 << 40):
+def attend(c=None, q=BUF, qs=(512, 512, 128), k=None, tokens=1, heads=4, s=None, out=BUF, os=(512, 512, 128), work=BUF, bytes=1 << 40):
     c, s = cache() if c is None else c, scores() if s is None else s
-    return _native.call("cuda", "bn_kv8_attend", C.byref(c), q, *qs, tokens, heads, None, None, C.byref(s), out, *os, 0, work, bytes, None)
+    return _native.call("cuda", "bn_kv8_attend", C.byref(c), q, *qs, k, 256, 256, 128, None, 256, 256, 128, tokens, heads, None, None, C.byref(s), out, *os, 0, work, bytes, None)
 
 
-@pytest.mark.parametrize("change", [dict(q=None), dict(out=None), dict(q=BUF + 2), dict(qs=(512, 512, 4)), dict(os=(4, 512, 128)), dict(tokens=-1), dict(tokens=1 << 40), dict(heads=0), dict(heads=3), dict(heads=1 << 20), dict(s=scores(window=-1)), dict(s=scores(softcap=-1.0))])
+@pytest.mark.parametrize("change", [dict(q=None), dict(k=BUF), dict(out=None), dict(q=BUF + 2), dict(qs=(512, 512, 4)), dict(os=(4, 512, 128)), dict(tokens=-1), dict(tokens=1 << 40), dict(heads=0), dict(heads=3), dict(heads=1 << 20), dict(s=scores(window=-1)), dict(s=scores(softcap=-1.0))])
 def test_attend_refuses(change):
     with pytest.raises(_native.NativeError, match="bad argument: bn_kv8_attend"):
         attend(**change)

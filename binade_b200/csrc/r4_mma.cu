@@ -23,13 +23,13 @@
 //
 // Every wait is bounded: when one gives up, a status flag is set, every thread still reaches the
 // end of the kernel, and the tensor memory is released.
-#include <cuda.h>
 #include <stdio.h>
 #include <stdlib.h>
 
 #include "common.cuh"
 #include "decode.cuh"
 #include "oct.cuh"
+#include "tcgen05.cuh"
 
 namespace bn {
 
@@ -46,18 +46,6 @@ constexpr uint32_t MMA_SMEM_MAX = 226 * 1024;  // dynamic part; the pair-table b
 
 __device__ int g_mma_error;  // 1: a bounded wait gave up
 
-__device__ __forceinline__ void mm_bar_init(uint32_t bar, uint32_t count) {
-  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
-}
-__device__ __forceinline__ void mm_bar_arrive(uint32_t bar) {
-  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
-}
-__device__ __forceinline__ void mm_bar_expect_tx(uint32_t bar, uint32_t bytes) {
-  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap *map, int x, int y, uint32_t bar) {
-  asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(bar) : "memory");
-}
 __device__ __forceinline__ bool mm_bar_wait(uint32_t bar, uint32_t parity) {
   // (a try with a suspend-time hint compiles to a sleep-and-poll loop of its own: more
   // instructions for the same wait, measured, so the plain form is kept)
@@ -78,60 +66,6 @@ __device__ __forceinline__ bool mm_bar_wait(uint32_t bar, uint32_t parity) {
 // The wait of a whole warp: every lane learns when some lane's gave up, so that the warp stays
 // together for what has to be executed by all of it (elect.sync, tcgen05.ld).
 __device__ __forceinline__ bool mm_bar_wait_warp(uint32_t bar, uint32_t parity) { return __all_sync(BN_FULL, mm_bar_wait(bar, parity)); }
-// Whether the phase is over already; does not wait.
-__device__ __forceinline__ bool mm_bar_test(uint32_t bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(ok)
-      : "r"(bar), "r"(parity)
-      : "memory");
-  return ok != 0;
-}
-// True in one lane of the warp, all of which has to get here: ahead of any wait. Instructions that
-// a single thread issues (MMAs, commits, bulk copies) take their operands from uniform registers;
-// behind `lane == 0` the compiler has to assume divergent values and wraps each of them in code that
-// makes them uniform.
-__device__ __forceinline__ bool elect_one() {
-  uint32_t one;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "elect.sync _|p, 0xffffffff;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(one));
-  return one != 0;
-}
-__device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
-__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-
-// Shared-memory matrix descriptor of a K-major, 128-byte-swizzled operand tile that starts at
-// shared address `addr` (1024-byte aligned atom; `addr` may point 32 * j bytes into the first
-// row to select the j-th group of 16 k): start address >> 4 in bits 0..13, leading byte offset
-// (unused for swizzled K-major, set to 1) in 16..29, stride between 8-row groups (1024 B) >> 4
-// in 32..45, descriptor version 1 in 46..47, layout 2 = 128-byte swizzle in 61..63.
-__device__ __forceinline__ uint64_t smem_desc(uint32_t addr) {
-  return (uint64_t)((addr >> 4) & 0x3FFFu) | (1ull << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
-}
-// Instruction descriptor: fp32 accumulate (bits 4..5 = 1), A and B BF16 (bits 7..9, 10..12 = 1),
-// both K-major (bits 15, 16 = 0), N >> 3 in bits 17..22, M >> 4 in bits 24..28.
-__host__ __device__ constexpr uint32_t mma_idesc(int m, int n) {
-  return (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
-}
-__device__ __forceinline__ void mma_bf16(uint32_t tmem_d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
-      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
-      : "memory");
-}
-__device__ __forceinline__ void mma_commit(uint32_t bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
-}
-
 struct MmaArgs {
   bn_r4 w;
   uint16_t *y;
@@ -144,9 +78,6 @@ struct MmaArgs {
   // slices' fp32 sums added in slice order, then one rounding to BF16
   int split, slice_tiles;
 };
-
-// Byte offset of (row r, 16-byte chunk c of the row's 128 bytes) inside a swizzled atom.
-__device__ __forceinline__ uint32_t swz(uint32_t r, uint32_t c) { return r * 128u + ((c ^ (r & 7u)) << 4); }
 
 // Shared addresses of a block's stage ring and barriers.
 struct MmaWindow {
@@ -632,18 +563,6 @@ __global__ void __launch_bounds__((MAXW + 2) * 32, 1) r4_mma_oct_kernel(const __
   tc_fence_before();
   __syncthreads();
   if (mma_warp) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(a.tmem_cols) : "memory");
-}
-
-typedef CUresult (*TensorMapEncodeFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-static TensorMapEncodeFn tensor_map_encoder() {
-  static TensorMapEncodeFn fn = nullptr;
-  if (!fn) {
-    void *p = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess && q == cudaDriverEntryPointSuccess) fn = (TensorMapEncodeFn)p;
-  }
-  return fn;
 }
 
 static int mma_sms() {

@@ -36,22 +36,4 @@ __device__ __forceinline__ float capped(float z, float cap_log2e) { return fmaf(
 __device__ __forceinline__ float bf16_to_f32(uint32_t bits) { return __uint_as_float(bits << 16); }
 #endif
 
-// The document of a packed batch that token t is in: true with its bounds [from, to), false when no
-// document holds the token. Offsets that do not rise, or leave [0, T], name no token.
-__device__ __forceinline__ bool document_of(const int32_t *__restrict__ offsets, int n, int T, int t, int &doc, int &from, int &to) {
-  if (!offsets) {
-    doc = 0, from = 0, to = T;
-    return t < T;
-  }
-  int a = 0, b = n;  // the last i with offsets[i] <= t lies in [a, b], if there is one
-  while (a < b) {
-    const int m = (a + b + 1) >> 1;
-    if (offsets[m] <= t) a = m;
-    else b = m - 1;
-  }
-  if (a >= n) return false;
-  doc = a, from = offsets[a], to = offsets[a + 1];
-  return from >= 0 && from <= t && t < to && to <= T;
-}
-
 }  // namespace bn

@@ -117,6 +117,7 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets: torch.
     q = _rows(q, "q", 3, dev)
     T, heads, D = q.shape
     k, v = _rows(k, "k", 3, dev), _rows(v, "v", 3, dev)
+    q, k, v = (t.contiguous() if 0 in t.stride() else t for t in (q, k, v))  # (expanded rows)
     kv = k.shape[1]
     if D not in HEAD_DIMS or k.shape != (T, kv, D) or v.shape != k.shape or kv < 1 or heads < 1 or heads % kv:
         raise ValueError(f"q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}: heads of 64, 128 or 256, query heads a multiple of key heads, the same tokens")

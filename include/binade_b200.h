@@ -331,7 +331,7 @@ typedef struct bn_kv8 {
 
 /* Up to `tokens` new tokens of every sequence, of which counts[b] are real (NULL: all), written behind the
  * length[b] that it holds; rows k, v (sequence, token, head) in BF16. Tokens that do not fit in max_seq are dropped, and
- * the device status says so (bits 24..30). */
+ * the device status says so (bits 24..27). */
 int bn_kv8_append(const bn_kv8 *c, const uint16_t *k, int64_t k_seq, int64_t k_token, int64_t k_head,
                   const uint16_t *v, int64_t v_seq, int64_t v_token, int64_t v_head, int64_t tokens,
                   const int32_t *counts, void *stream);
@@ -413,7 +413,7 @@ int bn_push_gather_beside(const void *const *locals, const uint64_t *bytes, int 
 
 /* Device-side status of the calling thread's current device: 0, or non-zero once a kernel of
  * this library gave up a bounded wait or refused a launch whose shared-memory window did not
- * match (its output is then incomplete): bits 0..7 the batch-1 matvec kernels, bits 8..15 the tensor-core GEMM, bits 16..23 the peer exchange, bits 24..30 tokens that a key/value cache had no room for. Every wait inside the
+ * match (its output is then incomplete): bits 0..7 the batch-1 matvec kernels, bits 8..15 the tensor-core GEMM, bits 16..23 the peer exchange, bits 24..27 tokens that a key/value cache had no room for, bits 28..30 the attention of prompts. Every wait inside the
  * kernels is bounded, so a lost copy or an absent peer ends in this status instead of a hang.
  * Synchronises with the device. No counterpart in the reference. */
 int bn_device_status(int *status);

@@ -158,13 +158,6 @@ __device__ __forceinline__ bool piece_of(const PromptArgs &a, int group, int64_t
   return true;
 }
 
-// One score (the raw sum of products) to powers of two, with cap and bias.
-__device__ __forceinline__ float full_score(const PromptArgs &a, float dot, float slope, int gap) {
-  float s = dot * a.scale;
-  s = a.cap > 0.0f ? capped(s * (2.0f * LOG2E / a.cap), a.cap * LOG2E) : s * LOG2E;
-  return fmaf(-slope, (float)gap, s);
-}
-
 __device__ __forceinline__ uint64_t pair_f32(float lo, float hi) {
   uint64_t r;
   asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
@@ -181,14 +174,19 @@ __device__ __forceinline__ uint64_t add_f32x2(uint64_t a, uint64_t b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
+__device__ __forceinline__ uint64_t mul_f32x2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
 __device__ __forceinline__ uint32_t bf16_pair(float lo, float hi) {
   uint32_t r;
   asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
 }
 
-// PLAIN: no cap, no bias, a positive scale.
-template <int D, bool PLAIN>
+// PLAIN: no cap, no bias, a positive scale. Else CAP: a cap.
+template <int D, bool PLAIN, bool CAP>
 __global__ void __launch_bounds__(PROMPT_THREADS, 1) prompt_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, const __grid_constant__ PromptArgs a, int group_log2, int head_groups) {
   using G = Tiles<D>;
   constexpr int NQ = G::NQ, BN = G::BN, ST = G::STAGES;
@@ -201,7 +199,7 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) prompt_kernel(const __grid_
 
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (threadIdx.x == 0) {
-    for (int i = 0; i < 2; i++) mm_bar_init(q_full + 8 * i, 1), mm_bar_init(s_full + 8 * i, 1), mm_bar_init(p_full + 8 * i, 128), mm_bar_init(o_done + 8 * i, 1);
+    for (int i = 0; i < 2; i++) mm_bar_init(q_full + 8 * i, 1), mm_bar_init(s_full + 8 * i, 1), mm_bar_init(p_full + 8 * i, NQ == 2 ? 128 : 256), mm_bar_init(o_done + 8 * i, 1);
     for (int i = 0; i < ST; i++) mm_bar_init(ring_full + 8 * i, 1), mm_bar_init(ring_empty + 8 * i, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -324,9 +322,15 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) prompt_kernel(const __grid_
       __syncwarp();
     }
     for (int t = max(0, at - ST); t < at && ok; t++) ok = prompt_wait_warp(ring_empty + 8 * (t % ST), (t / ST) & 1);  // nor does a product
-  } else if (NQ == 2 || warp < 4) {
+  } else if (warp < SOFTMAX_WARPS) {
     // ---------------------------------------------------------------- softmax
-    const int i = (int)warp >> 2, row = (int)((warp & 3) * 32 + lane);
+    // Two query tiles: four warps each. One: two warps share 32 rows, each with half the columns; they tell one another
+    // their maxima, and in the end their weights, through shared memory.
+    constexpr int CN = NQ == 2 ? BN : BN / 2, OD = NQ == 2 ? D : D / 2;
+    const int i = NQ == 2 ? (int)warp >> 2 : 0, part = NQ == 2 ? 0 : (int)warp >> 2, row = (int)((warp & 3) * 32 + lane);
+    const int col0 = part * CN;
+    __shared__ float told[NQ == 2 ? 1 : 2][2][NQ == 2 ? 1 : 128];
+    auto both_halves = [&]() { asm volatile("bar.sync 1, 256;" ::: "memory"); };
     const uint32_t lanes = ((warp & 3) * 32u) << 16;
     const int at_row = p.row0 + 128 * i + row, tok = at_row >> group_log2, head = head0 + (at_row & (group - 1));
     const bool real = j1[i] > j0[i] && tok < p.L;
@@ -335,36 +339,68 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) prompt_kernel(const __grid_
     visible_keys(min((p.row0 + 128 * i + 127) >> group_log2, p.L - 1), p.L, p.prefix, a.window, a.causal, lo_most, other);
     visible_keys((p.row0 + 128 * i) >> group_log2, p.L, p.prefix, a.window, a.causal, other, hi_least);
     const float slope = !PLAIN && a.slopes && real ? a.slopes[head] * LOG2E : 0.0f;
+    const int first_tok = (p.row0 + 128 * i) >> group_log2;
     const float c = a.scale * LOG2E;
-    const uint32_t o_at = tmem + G::O_AT + i * D + lanes;
+    const uint32_t o_at = tmem + G::O_AT + i * D + part * OD + lanes;
     float m = NOTHING, l = 0.0f;
     bool ok = true;
     for (int j = j0[i]; j < j1[i]; j++) {
       const int n = j - j0[i], buf = NQ == 2 ? i : n & 1;
-      const uint32_t s_at = tmem + G::S_AT + buf * BN + lanes;
+      const uint32_t s_at = tmem + G::S_AT + buf * BN + lanes;  // (P: half the columns)
       if (ok) ok = prompt_wait_warp(s_full + 8 * buf, NQ == 2 ? n & 1 : (n >> 1) & 1);
-      if (!ok) break;
-      tc_fence_after();
-      uint32_t s[BN];
-#pragma unroll
-      for (int x = 0; x < BN; x += 32) tmem_load32(s_at + x, s + x);
-      tmem_wait_loads();
-      const int key0 = j * BN;
-      if constexpr (!PLAIN) {
-#pragma unroll
-        for (int x = 0; x < BN; x++) s[x] = __float_as_uint(full_score(a, __uint_as_float(s[x]), slope, abs(tok - (key0 + x))));
+      if (!ok) {  // (no half waits for one that gave up)
+        if constexpr (NQ == 1) both_halves();
+        continue;
       }
-      if (key0 < lo_most || key0 + BN > hi_least) {
+      tc_fence_after();
+      uint32_t s[CN];
+#pragma unroll
+      for (int x = 0; x < CN; x += 32) tmem_load32(s_at + col0 + x, s + x);
+      tmem_wait_loads();
+      const int key0 = j * BN + col0;
+      if constexpr (CAP) {
+        const uint64_t f = pair_f32(a.scale * (2.0f * LOG2E / a.cap), a.scale * (2.0f * LOG2E / a.cap));
+#pragma unroll
+        for (int x = 0; x < CN; x += 2) {
+          float z0, z1;
+          split_f32(mul_f32x2(pair_f32(__uint_as_float(s[x]), __uint_as_float(s[x + 1])), f), z0, z1);
+          s[x] = __float_as_uint(capped(z0, a.cap * LOG2E)), s[x + 1] = __float_as_uint(capped(z1, a.cap * LOG2E));
+        }
+      }
+      if constexpr (!PLAIN) {  // s c - slope |i - j|; the bias is a line where all keys lie before the queries
+        const uint64_t f = pair_f32(CAP ? 1.0f : c, CAP ? 1.0f : c);
+        const float gap = (float)(tok - key0);
+        if (key0 + CN <= first_tok) {
+          const uint64_t up = pair_f32(slope, slope), from = pair_f32(-slope * gap, -slope * gap);
+#pragma unroll
+          for (int x = 0; x < CN; x += 2) {
+            float v0, v1;
+            split_f32(fma_f32x2(pair_f32(__uint_as_float(s[x]), __uint_as_float(s[x + 1])), f, fma_f32x2(up, pair_f32((float)x, (float)(x + 1)), from)), v0, v1);
+            s[x] = __float_as_uint(v0), s[x + 1] = __float_as_uint(v1);
+          }
+        } else {
+#pragma unroll
+          for (int x = 0; x < CN; x++) s[x] = __float_as_uint(fmaf(-slope, fabsf(gap - (float)x), __uint_as_float(s[x]) * (CAP ? 1.0f : c)));
+        }
+      }
+      if (key0 < lo_most || key0 + CN > hi_least) {
         const uint32_t from = (uint32_t)(lo - key0), count = (uint32_t)(hi - lo);
 #pragma unroll
-        for (int x = 0; x < BN; x++)
+        for (int x = 0; x < CN; x++)
           if ((uint32_t)x - from >= count) s[x] = 0xFF800000u;  // -inf
       }
       float top = __uint_as_float(s[0]), top2 = __uint_as_float(s[1]);
 #pragma unroll
-      for (int x = 2; x < BN; x += 2) top = fmaxf(top, __uint_as_float(s[x])), top2 = fmaxf(top2, __uint_as_float(s[x + 1]));
+      for (int x = 2; x < CN; x += 2) top = fmaxf(top, __uint_as_float(s[x])), top2 = fmaxf(top2, __uint_as_float(s[x + 1]));
       top = fmaxf(top, top2);
       if constexpr (PLAIN) top *= c;
+      if constexpr (NQ == 1) {
+        told[n & 1][part][row] = top;
+        tc_fence_before();  // the other half's scores have been read when its weights are written over them
+        both_halves();
+        tc_fence_after();
+        top = fmaxf(top, told[n & 1][part ^ 1][row]);
+      }
       if (__any_sync(BN_FULL, top > m + RISE)) {
         const bool rise = top > m + RISE;
         const float keep = rise ? ex2(m - top) : 1.0f;
@@ -374,7 +410,7 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) prompt_kernel(const __grid_
           if (ok) ok = prompt_wait_warp(o_done + 8 * i, (n - 1) & 1);
           tc_fence_after();
 #pragma unroll 1
-          for (int x = 0; x < D; x += 32) {
+          for (int x = 0; x < OD; x += 32) {
             uint32_t o[32];
             tmem_load32(o_at + x, o);
             tmem_wait_loads();
@@ -387,7 +423,7 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) prompt_kernel(const __grid_
       const uint64_t cc = pair_f32(PLAIN ? c : 1.0f, PLAIN ? c : 1.0f), mm = pair_f32(-m, -m);
       uint64_t sum = 0, sum2 = 0;
 #pragma unroll
-      for (int x = 0; x < BN; x += 4) {
+      for (int x = 0; x < CN; x += 4) {
         float e0, e1, e2, e3;
         split_f32(fma_f32x2(pair_f32(__uint_as_float(s[x]), __uint_as_float(s[x + 1])), cc, mm), e0, e1);
         split_f32(fma_f32x2(pair_f32(__uint_as_float(s[x + 2]), __uint_as_float(s[x + 3])), cc, mm), e2, e3);
@@ -395,8 +431,12 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) prompt_kernel(const __grid_
         sum = add_f32x2(sum, pair_f32(e0, e1)), sum2 = add_f32x2(sum2, pair_f32(e2, e3));
         s[x / 2] = bf16_pair(e0, e1), s[x / 2 + 1] = bf16_pair(e2, e3);
       }
+      if constexpr (NQ == 2) {
 #pragma unroll
-      for (int x = 0; x < BN / 2; x += 32) tmem_store32(s_at + x, s + x);
+        for (int x = 0; x < CN / 2; x += 32) tmem_store32(s_at + x, s + x);
+      } else {
+        tmem_store16(s_at + col0 / 2, s);
+      }
       float s0, s1;
       split_f32(add_f32x2(sum, sum2), s0, s1);
       l += s0 + s1;
@@ -408,12 +448,17 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1) prompt_kernel(const __grid_
     if (j1[i] > j0[i]) {
       if (ok) ok = prompt_wait_warp(o_done + 8 * i, (j1[i] - j0[i] - 1) & 1);
       tc_fence_after();
+      if constexpr (NQ == 1) {
+        told[0][part][row] = l;  // (a tile's maxima lie in [1] or have been read by both halves: their last product is done)
+        both_halves();
+        l += told[0][part ^ 1][row];
+      }
       bool odd = !(l > 0.0f && l <= 3.0e38f);
       const float inv = 1.0f / l;
-      uint16_t *const out = a.out + (int64_t)(p.from + tok) * a.o_token + head * a.o_head;
+      uint16_t *const out = a.out + (int64_t)(p.from + tok) * a.o_token + head * a.o_head + part * OD;
       if (ok) {
 #pragma unroll 1
-        for (int x = 0; x < D; x += 32) {
+        for (int x = 0; x < OD; x += 32) {
           uint32_t o[32];
           tmem_load32(o_at + x, o);
           tmem_wait_loads();
@@ -471,7 +516,7 @@ int prompt_launch(const PromptArgs &a, cudaStream_t stream) {
     return fail(BN_ERR_ARG, "bn_attention: no tensor map for these strides");
   const int64_t blocks = ((int64_t)a.T * group / G::ROWS + a.docs + 1) * head_groups;
   if (blocks > 0x7FFFFFFF) return fail(BN_ERR_ARG, "bn_attention: too many rows");
-  auto kern = a.cap == 0.0f && !a.slopes && a.scale > 0.0f ? prompt_kernel<D, true> : prompt_kernel<D, false>;
+  auto kern = a.cap > 0.0f ? prompt_kernel<D, false, true> : !a.slopes && a.scale > 0.0f ? prompt_kernel<D, true, false> : prompt_kernel<D, false, false>;
   BN_CUDA(allow_smem(kern, G::SMEM));
   cudaLaunchConfig_t cfg{};
   cudaLaunchAttribute attr[1];

@@ -64,6 +64,10 @@ int kv8_status(int *status);  // kv8.cu
 int kv8_status_reset();
 int attention_status(int *status);  // attention.cu
 int attention_status_reset();
+// Attention of chunks over a cache (kv8_chunk.cu)
+int kv8_chunk(const bn_kv8 *c, const uint16_t *q, int64_t q_seq, int64_t q_token, int64_t q_head, int64_t tokens, int64_t heads, const int32_t *counts, const int32_t *prefix, const bn_scores *scores, uint16_t *out, int64_t o_seq, int64_t o_token, int64_t o_head, int zero_rest, cudaStream_t stream);
+int kv8_chunk_status(int *status);
+int kv8_chunk_status_reset();
 int mma_status_reset();
 int stream_status_reset();
 int oct_status_reset();

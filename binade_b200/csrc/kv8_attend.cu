@@ -724,6 +724,14 @@ int attend_kind(const AttendArgs &a, int mt, cudaStream_t s) {
   return attend_launch<256, KIND, 1, PLAIN>(a, s);
 }
 
+// Whether many rows go to the other kernel (kv8_chunk.cu), which reads a sequence's keys once for 256 rows (128 with heads
+// of 256), but by one block from end to end.
+bool chunk_wins(const bn_kv8 *c, int64_t tokens, int64_t heads) {
+  const int64_t rows = heads / c->kv_heads * tokens, units = c->batch * c->kv_heads, per_block = c->D == 256 ? 128 : 256;
+  const int64_t groups = (rows + 31) / 32, waves = (units * ((rows + per_block - 1) / per_block) + sm_count() - 1) / sm_count();
+  return rows > 32 && units * groups > 100 * waves;
+}
+
 bool attend_sizes(const bn_kv8 *c, int64_t tokens, int64_t heads) { return tokens >= 0 && tokens <= 0x3FFFFFFF && heads >= 1 && heads <= 4096 && heads % c->kv_heads == 0; }
 
 }  // namespace
@@ -731,7 +739,7 @@ bool attend_sizes(const bn_kv8 *c, int64_t tokens, int64_t heads) { return token
 
 extern "C" uint64_t bn_kv8_workspace(const bn_kv8 *c, int64_t tokens, int64_t heads) {
   if (bn::kv8_refusal(c) || !bn::attend_sizes(c, tokens, heads) || tokens == 0) return 0;
-  return bn::plan_of(c, tokens, heads).bytes;
+  return bn::chunk_wins(c, tokens, heads) ? 0 : bn::plan_of(c, tokens, heads).bytes;
 }
 
 extern "C" int bn_kv8_attend(const bn_kv8 *c, const uint16_t *q, int64_t q_seq, int64_t q_token, int64_t q_head, const uint16_t *k, int64_t k_seq, int64_t k_token, int64_t k_head, const uint16_t *v, int64_t v_seq, int64_t v_token, int64_t v_head, int64_t tokens, int64_t heads, const int32_t *counts, const int32_t *prefix, const bn_scores *scores, uint16_t *out, int64_t o_seq, int64_t o_token, int64_t o_head, int zero_rest, void *workspace, uint64_t workspace_bytes, void *stream) {
@@ -741,7 +749,14 @@ extern "C" int bn_kv8_attend(const bn_kv8 *c, const uint16_t *q, int64_t q_seq, 
   if (((uintptr_t)q | (uintptr_t)out) & 15 || (q_seq | q_token | q_head | o_seq | o_token | o_head) & 7) return bn::fail(BN_ERR_ARG, "bn_kv8_attend: rows have to start on 16 bytes");
   if (scores->window < 0 || scores->window > 0x3FFFFFFF || !(scores->softcap >= 0.0f)) return bn::fail(BN_ERR_ARG, "bn_kv8_attend: negative window or cap");
   if (tokens == 0) return BN_OK;
+  const bool chunk = bn::chunk_wins(c, tokens, heads);
   const bn::Plan p = bn::plan_of(c, tokens, heads);
+  if (chunk && ((tokens > 1 && !q_token) || (heads > 1 && !q_head) || (c->batch > 1 && !q_seq) || (q_seq | q_token | q_head) < 0)) return bn::fail(BN_ERR_ARG, "bn_kv8_attend: query rows have to lie apart");
+  if (chunk) {
+    if (k)
+      if (const int e = bn_kv8_append(c, k, k_seq, k_token, k_head, v, v_seq, v_token, v_head, tokens, counts, stream)) return e;
+    return bn::kv8_chunk(c, q, q_seq, q_token, q_head, tokens, heads, counts, prefix, scores, out, o_seq, o_token, o_head, zero_rest, (cudaStream_t)stream);
+  }
   if (!workspace || (uintptr_t)workspace & 15 || workspace_bytes < p.bytes) return bn::fail(BN_ERR_CAPACITY, "bn_kv8_attend: the workspace is smaller than bn_kv8_workspace says, or not on 16 bytes");
   if (c->batch * heads * tokens > 0x7FFFFFFF) return bn::fail(BN_ERR_ARG, "bn_kv8_attend: too many rows for one call");
   if (k)

@@ -640,12 +640,13 @@ extern "C" int bn_device_status_reset(void) {
   if (int e = bn::mma_status_reset()) return e;
   if (int e = bn::kv8_status_reset()) return e;
   if (int e = bn::attention_status_reset()) return e;
+  if (int e = bn::kv8_chunk_status_reset()) return e;
   return bn::exchange_status_reset();
 }
 
 extern "C" int bn_device_status(int *status) {
   if (!status) return bn::fail(BN_ERR_ARG, "bn_device_status: null pointer");
-  int stream = 0, mma = 0, xch = 0, oct = 0, kv8 = 0, attention = 0;
+  int stream = 0, mma = 0, xch = 0, oct = 0, kv8 = 0, attention = 0, chunk = 0;
   BN_CUDA(cudaMemcpyFromSymbol(&stream, bn::g_stream_error, sizeof(int)));
   if (int e = bn::oct_status(&oct)) return e;
   if (oct) stream |= 4;
@@ -655,6 +656,7 @@ extern "C" int bn_device_status(int *status) {
   if (int e = bn::exchange_status(&xch)) return e;
   if (int e = bn::kv8_status(&kv8)) return e;
   if (int e = bn::attention_status(&attention)) return e;
-  *status = stream | (mma << 8) | (xch << 16) | (kv8 << 24) | (attention << 28);
+  if (int e = bn::kv8_chunk_status(&chunk)) return e;
+  *status = stream | (mma << 8) | (xch << 16) | (kv8 << 24) | ((attention | chunk) << 28);
   return BN_OK;
 }

@@ -202,6 +202,8 @@ class KV8Cache:
         counts come back as zeros, or, with `out` given, stay as they are."""
         at = self._layer(layer)
         q = self._new(q, "q")
+        if 0 in q.stride():  # (expanded rows)
+            q = q.contiguous()
         tokens, heads = q.shape[1], q.shape[2]
         if heads < 1 or heads % self.kv_heads:
             raise ValueError(f"{heads} query heads over {self.kv_heads} key heads")

@@ -30,7 +30,7 @@ namespace bn {
 
 namespace {
 
-__device__ int g_prompt_error;  // 1: a bounded wait gave up
+__device__ int g_prompt_error;  // 1: a bounded wait gave up; 2: the shared window did not fit
 
 struct PromptArgs {
   const uint16_t *q, *k, *v;
@@ -162,7 +162,14 @@ struct Tiles {
   static constexpr int BN = D == 256 ? 64 : 128;     // keys of a step
   static constexpr int STAGES = D == 64 ? 8 : 4;     // ring slots of a K or V tile
   static constexpr uint32_t TILE_BYTES = BN * D * 2, Q_BYTES = 128 * D * 2;
-  static constexpr uint32_t SMEM = 1024 + NQ * Q_BYTES + STAGES * TILE_BYTES + 320 + SCALES_AHEAD * 2 * (BN / 16) * 4;
+  static constexpr uint32_t RAW_BYTES = BN * D;      // a tile of codes as they lie: two of them wait for the warps that turn them into BF16
+  static constexpr uint32_t BARS = 384, SCALES = SCALES_AHEAD * 2 * (BN / 16) * 4;
+  static constexpr uint32_t TOLD = NQ == 1 ? 2048 : 0;  // two halves' maxima, for two tiles
+  static constexpr uint32_t WINDOW = NQ * Q_BYTES + STAGES * TILE_BYTES + BARS + SCALES + TOLD, WINDOW_CODES = WINDOW + 2 * RAW_BYTES;
+  // with room to start on 1024 bytes; not where all of a block's shared memory is taken (the window starts on 1024
+  // bytes when there is no static shared memory; a block whose window does not is refused)
+  static constexpr uint32_t SMEM = WINDOW + 1024, SMEM_CODES = D == 256 ? WINDOW_CODES : WINDOW_CODES + 1024;
+  static_assert(SMEM_CODES <= 227 * 1024, "a block's shared memory");
   static constexpr uint32_t S_AT = 0, O_AT = 2 * BN;  // tensor memory columns: two S buffers, then the sums
 };
 
@@ -238,9 +245,15 @@ __device__ __forceinline__ uint2 codes_bf16(uint32_t w) {
 }
 __device__ __forceinline__ void sts8(uint32_t at, uint2 v) { asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(at), "r"(v.x), "r"(v.y) : "memory"); }
 __device__ __forceinline__ void sts16(uint32_t at, uint4 v) { asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory"); }
+__device__ __forceinline__ uint4 lds16(uint32_t at) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+  return v;
+}
+__device__ __forceinline__ void sts_f32(uint32_t at, float v) { asm volatile("st.shared.f32 [%0], %1;" ::"r"(at), "f"(v) : "memory"); }
 __device__ __forceinline__ float lds_f32(uint32_t at) {
   float v;
-  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(at));
+  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
   return v;
 }
 
@@ -282,13 +295,18 @@ __global__ void __launch_bounds__(Roles<SRC>::WARPS * 32, 1) prompt_kernel(const
   const int group = 1 << group_log2;
   const uint32_t base = (smem_addr(prompt_smem) + 1023u) & ~1023u;
   const uint32_t q_at = base, ring_at = q_at + NQ * G::Q_BYTES, bars = ring_at + ST * G::TILE_BYTES;
-  const uint32_t q_full = bars, s_full = bars + 16, p_full = bars + 32, o_done = bars + 48, ring_full = bars + 64, ring_empty = ring_full + 8 * ST, scale_full = ring_empty + 8 * ST, tmem_slot = scale_full + 8 * SCALES_AHEAD, scales_at = bars + 320;
+  const uint32_t q_full = bars, s_full = bars + 16, p_full = bars + 32, o_done = bars + 48, ring_full = bars + 64, ring_empty = ring_full + 8 * ST, scale_full = ring_empty + 8 * ST, raw_full = scale_full + 8 * SCALES_AHEAD, raw_empty = raw_full + 16, tmem_slot = raw_empty + 16, scales_at = bars + G::BARS, told_at = scales_at + G::SCALES, raw_at = told_at + G::TOLD;
+  if (base + (CODES ? G::WINDOW_CODES : G::WINDOW) > smem_addr(prompt_smem) + (CODES ? G::SMEM_CODES : G::SMEM)) {
+    if (threadIdx.x == 0) atomicExch(&g_prompt_error, 2);
+    return;
+  }
 
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; i++) mm_bar_init(q_full + 8 * i, 1), mm_bar_init(s_full + 8 * i, 1), mm_bar_init(p_full + 8 * i, NQ == 2 ? 128 : 256), mm_bar_init(o_done + 8 * i, 1);
     for (int i = 0; i < ST; i++) mm_bar_init(ring_full + 8 * i, CODES ? 4 : 1), mm_bar_init(ring_empty + 8 * i, 1);
     for (int i = 0; i < SCALES_AHEAD; i++) mm_bar_init(scale_full + 8 * i, 4);
+    for (int i = 0; i < 2; i++) mm_bar_init(raw_full + 8 * i, 1), mm_bar_init(raw_empty + 8 * i, 4);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == MMA_WARP) {
@@ -354,6 +372,25 @@ __global__ void __launch_bounds__(Roles<SRC>::WARPS * 32, 1) prompt_kernel(const
           if (j > J0) fetch(&v_map, j - 1);
         }
         for (int t = max(0, at - ST); t < at; t++) prompt_wait(ring_full + 8 * (t % ST), (t / ST) & 1);  // no copy outlives the block
+      } else {
+        const int full = p.L / a.c.block * a.c.block;
+        const int64_t unit = p.b * a.kv_heads + kv;
+        int at = 0;
+        bool ok = true;
+        auto fetch = [&](const uint8_t *codes, int j) {  // the tile's codes: one run of bytes, as far as its blocks are full
+          const int s = at % 2, key0 = j * BN;
+          if (at >= 2 && ok) ok = prompt_wait(raw_empty + 8 * s, ((at / 2) & 1) ^ 1);
+          if (!ok) return;
+          const uint32_t bytes = (uint32_t)(min(max(full - key0, 0), BN) * D);
+          mm_bar_expect_tx(raw_full + 8 * s, bytes);
+          if (bytes) asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(raw_at + s * G::RAW_BYTES), "l"(codes + (unit * a.c.rows + key0) * D), "r"(bytes), "r"(raw_full + 8 * s) : "memory");
+          at++;
+        };
+        for (int j = J0; j <= J1 && ok; j++) {
+          if (j < J1) fetch(a.c.k, j);
+          if (j > J0) fetch(a.c.v, j - 1);
+        }
+        for (int t = max(0, at - 2); t < at; t++) prompt_wait(raw_full + 8 * (t % 2), (t / 2) & 1);
       }
 #pragma unroll
       for (int i = 0; i < NQ; i++)
@@ -424,22 +461,21 @@ __global__ void __launch_bounds__(Roles<SRC>::WARPS * 32, 1) prompt_kernel(const
     fewer_registers<Roles<SRC>::OTHER_REGS>();
     // ---------------------------------------------------------------- codes to BF16
     if constexpr (CODES) {
-        constexpr int PIECES = BN * D / 2048;  // 16-byte pieces of a tile that a thread has
+        constexpr int PIECES = BN * D / 2048;  // 16-byte pieces of a tile's codes that a thread has
       const int tid = (int)threadIdx.x - CODE_WARP * 32, full = p.L / a.c.block * a.c.block;
       const int64_t unit = p.b * a.kv_heads + kv;
       const uint16_t *const k_tail = a.c.k_tail + (unit * 2 + (work ? kv8_slot(a.c, p.b, p.held, p.L / a.c.block) : 0)) * a.c.block * D, *const v_tail = a.c.v_tail + (k_tail - a.c.k_tail);
       int at = 0;
       bool ok = true;
+      auto scale_of = [&](int j) {  // of both sides, for 16 keys a thread; 1 in the open block
+        const int side = tid / (BN / 16), key = j * BN + tid % (BN / 16) * 16;
+        return tid < 2 * (BN / 16) && key < full ? (side ? a.c.v_scale : a.c.k_scale)[unit * (a.c.rows / a.c.block) + key / a.c.block] : 1.0f;
+      };
+      float scale = J0 < J1 ? scale_of(J0) : 1.0f;
       auto fetch = [&](bool values, int j) {
         const int s = at % ST, key0 = j * BN;
-        const uint32_t to = ring_at + s * G::TILE_BYTES;
-        const uint8_t *const from = (values ? a.c.v : a.c.k) + (unit * a.c.rows + key0) * D;
-        uint4 w[PIECES];
-#pragma unroll
-        for (int i = 0; i < PIECES; i++) {
-          const int q = tid + 128 * i, key = key0 + (values ? q / (D / 4) * 4 : q / (D / 16));
-          if (key < full) w[i] = *reinterpret_cast<const uint4 *>(from + (int64_t)q * 16);
-        }
+        const uint32_t to = ring_at + s * G::TILE_BYTES, raw = raw_at + (at % 2) * G::RAW_BYTES + tid * 16;
+        if (ok) ok = prompt_wait_warp(raw_full + 8 * (at % 2), (at / 2) & 1);
         if (at >= ST && ok) ok = prompt_wait_warp(ring_empty + 8 * s, ((at / ST) & 1) ^ 1);
         if (!ok) return;
 #pragma unroll
@@ -449,7 +485,8 @@ __global__ void __launch_bounds__(Roles<SRC>::WARPS * 32, 1) prompt_kernel(const
             const int key = q / (D / 4) * 4, d = q % (D / 4) * 4;
             const uint32_t dst = to + (d / 64) * (BN * 128) + (d % 8) * 2;
             if (key0 + key < full) {
-              const uint32_t a01 = __byte_perm(w[i].x, w[i].y, 0x5140), b01 = __byte_perm(w[i].x, w[i].y, 0x7362), a23 = __byte_perm(w[i].z, w[i].w, 0x5140), b23 = __byte_perm(w[i].z, w[i].w, 0x7362);
+              const uint4 w = lds16(raw + 2048 * i);
+              const uint32_t a01 = __byte_perm(w.x, w.y, 0x5140), b01 = __byte_perm(w.x, w.y, 0x7362), a23 = __byte_perm(w.z, w.w, 0x5140), b23 = __byte_perm(w.z, w.w, 0x7362);
               sts8(dst + swz(key, d % 64 / 8), codes_bf16<SRC>(__byte_perm(a01, a23, 0x5410)));
               sts8(dst + swz(key + 1, d % 64 / 8), codes_bf16<SRC>(__byte_perm(a01, a23, 0x7632)));
               sts8(dst + swz(key + 2, d % 64 / 8), codes_bf16<SRC>(__byte_perm(b01, b23, 0x5410)));
@@ -463,7 +500,8 @@ __global__ void __launch_bounds__(Roles<SRC>::WARPS * 32, 1) prompt_kernel(const
             const uint32_t dst = to + (d / 64) * (BN * 128);
             uint4 lo = make_uint4(0, 0, 0, 0), hi = lo;
             if (key0 + key < full) {
-              const uint2 c0 = codes_bf16<SRC>(w[i].x), c1 = codes_bf16<SRC>(w[i].y), c2 = codes_bf16<SRC>(w[i].z), c3 = codes_bf16<SRC>(w[i].w);
+              const uint4 w = lds16(raw + 2048 * i);
+              const uint2 c0 = codes_bf16<SRC>(w.x), c1 = codes_bf16<SRC>(w.y), c2 = codes_bf16<SRC>(w.z), c3 = codes_bf16<SRC>(w.w);
               lo = make_uint4(c0.x, c0.y, c1.x, c1.y), hi = make_uint4(c2.x, c2.y, c3.x, c3.y);
             } else if (key0 + key < p.L) {
               const uint4 *const row = reinterpret_cast<const uint4 *>(k_tail + (int64_t)(key0 + key - full) * D + d);
@@ -472,19 +510,16 @@ __global__ void __launch_bounds__(Roles<SRC>::WARPS * 32, 1) prompt_kernel(const
             sts16(dst + swz(key, d % 64 / 8), lo), sts16(dst + swz(key, d % 64 / 8 + 1), hi);
           }
         }
-        if (!values) {  // both scales of the tile's keys, 16 at a time; 1 in the open block
-          const int idx = j - J0;
-          if (tid < 2 * (BN / 16)) {
-            const int side = tid / (BN / 16), key = key0 + tid % (BN / 16) * 16;
-            const float scale = key < full ? (side ? a.c.v_scale : a.c.k_scale)[unit * (a.c.rows / a.c.block) + key / a.c.block] : 1.0f;
-            asm volatile("st.shared.f32 [%0], %1;" ::"r"(scales_at + (uint32_t)((idx % SCALES_AHEAD) * 2 * (BN / 16) + tid) * 4u), "f"(scale) : "memory");
-          }
+        if (!values) {  // both scales of the tile's keys, 16 at a time
+          const int idx = (j - J0) % SCALES_AHEAD;
+          if (tid < 2 * (BN / 16)) sts_f32(scales_at + (uint32_t)(idx * 2 * (BN / 16) + tid) * 4u, scale);
           __syncwarp();
-          if (lane == 0) mm_bar_arrive(scale_full + 8 * (idx % SCALES_AHEAD));
+          if (lane == 0) mm_bar_arrive(scale_full + 8 * idx);
+          scale = scale_of(j + 1);  // (past the last full block: 1)
         }
         fence_async_smem();  // the tensor core reads shared memory through the async proxy
         __syncwarp();
-        if (lane == 0) mm_bar_arrive(ring_full + 8 * s);
+        if (lane == 0) mm_bar_arrive(ring_full + 8 * s), mm_bar_arrive(raw_empty + 8 * (at % 2));
         at++;
       };
       for (int j = J0; j <= J1 && ok; j++) {
@@ -500,7 +535,7 @@ __global__ void __launch_bounds__(Roles<SRC>::WARPS * 32, 1) prompt_kernel(const
     constexpr int CN = NQ == 2 ? BN : BN / 2, OD = NQ == 2 ? D : D / 2;
     const int i = NQ == 2 ? (int)warp >> 2 : 0, part = NQ == 2 ? 0 : (int)warp >> 2, row = (int)((warp & 3) * 32 + lane);
     const int col0 = part * CN;
-    __shared__ float told[NQ == 2 ? 1 : 2][2][NQ == 2 ? 1 : 128];
+    auto told = [&](int n, int half) { return told_at + (uint32_t)(((n & 1) * 2 + half) * 128 + row) * 4u; };
     auto both_halves = [&]() { asm volatile("bar.sync 1, 256;" ::: "memory"); };
     const uint32_t lanes = ((warp & 3) * 32u) << 16;
     const int at_row = p.row0 + 128 * i + row, tok = at_row >> group_log2, head = head0 + (at_row & (group - 1));
@@ -581,11 +616,11 @@ __global__ void __launch_bounds__(Roles<SRC>::WARPS * 32, 1) prompt_kernel(const
       top = fmaxf(top, top2);
       if constexpr (PLAIN) top *= c;
       if constexpr (NQ == 1) {
-        told[n & 1][part][row] = top;
+        sts_f32(told(n, part), top);
         tc_fence_before();  // the other half's scores have been read when its weights are written over them
         both_halves();
         tc_fence_after();
-        top = fmaxf(top, told[n & 1][part ^ 1][row]);
+        top = fmaxf(top, lds_f32(told(n, part ^ 1)));
       }
       if (__any_sync(BN_FULL, top > m + RISE)) {
         const bool rise = top > m + RISE;
@@ -640,9 +675,9 @@ __global__ void __launch_bounds__(Roles<SRC>::WARPS * 32, 1) prompt_kernel(const
       if (ok) ok = prompt_wait_warp(o_done + 8 * (NQ == 2 ? i : n & 1), NQ == 2 ? n & 1 : (n >> 1) & 1);
       tc_fence_after();
       if constexpr (NQ == 1) {
-        told[0][part][row] = l;  // (a tile's maxima lie in [1] or have been read by both halves: their last product is done)
+        sts_f32(told(0, part), l);  // (the last tile's maxima have been read by both halves: its product is done)
         both_halves();
-        l += told[0][part ^ 1][row];
+        l += lds_f32(told(0, part ^ 1));
       }
       bool odd = !(l > 0.0f && l <= 3.0e38f);
       const float inv = 1.0f / l;
@@ -712,12 +747,13 @@ inline int block_group_log2(int64_t heads, int64_t kv_heads) {
 template <int D, int SRC>
 int prompt_launch(const PromptArgs &a, const CUtensorMap &q_map, const CUtensorMap &k_map, const CUtensorMap &v_map, int64_t blocks, int log2, cudaStream_t stream) {
   auto kern = a.cap > 0.0f ? prompt_kernel<D, false, true, SRC> : !a.slopes && a.scale > 0.0f ? prompt_kernel<D, true, false, SRC> : prompt_kernel<D, false, false, SRC>;
-  BN_CUDA(allow_smem(kern, Tiles<D>::SMEM));
+  const uint32_t smem = SRC == FROM_BF16 ? Tiles<D>::SMEM : Tiles<D>::SMEM_CODES;
+  BN_CUDA(allow_smem(kern, smem));
   cudaLaunchConfig_t cfg{};
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.gridDim = dim3((unsigned)blocks), cfg.blockDim = dim3(Roles<SRC>::WARPS * 32), cfg.dynamicSmemBytes = Tiles<D>::SMEM, cfg.stream = stream, cfg.attrs = attr, cfg.numAttrs = 1;
+  cfg.gridDim = dim3((unsigned)blocks), cfg.blockDim = dim3(Roles<SRC>::WARPS * 32), cfg.dynamicSmemBytes = smem, cfg.stream = stream, cfg.attrs = attr, cfg.numAttrs = 1;
   BN_CUDA(cudaLaunchKernelEx(&cfg, kern, q_map, k_map, v_map, a, log2, a.heads >> log2));
   return launched("prompt_kernel");
 }

@@ -133,15 +133,15 @@ __device__ __noinline__ void attend_row(const PromptArgs &a, const Piece &p, int
   for (int e = 0; e < E; e++) out[e] = f32_to_bf16_bits(o[e]);
 }
 
-// Warps 0 .. 7 do the softmax; the next four turn codes into BF16 where there are codes; then the warp that copies and the
-// one that issues products, of a group of four. Registers move from the others to the softmax: the groups' shares add up
-// to what the block was launched with (3 x 168 or 4 x 128).
+// Warps 0 .. 7 do the softmax; the next eight turn codes into BF16 where there are codes; then the warp that copies and
+// the one that issues products, of a group of four. Registers move from the others to the softmax: the groups' shares add
+// up to what the block was launched with (3 x 168 or 5 x 96).
 template <int SRC>
 struct Roles {
-  static constexpr int WARPS = SRC == FROM_BF16 ? 12 : 16, TMA_WARP = WARPS - 4, MMA_WARP = WARPS - 3;
-  static constexpr int SOFTMAX_REGS = SRC == FROM_BF16 ? 208 : 184, OTHER_REGS = SRC == FROM_BF16 ? 88 : 72;
+  static constexpr int WARPS = SRC == FROM_BF16 ? 12 : 20, TMA_WARP = WARPS - 4, MMA_WARP = WARPS - 3;
+  static constexpr int SOFTMAX_REGS = SRC == FROM_BF16 ? 208 : 168, OTHER_REGS = SRC == FROM_BF16 ? 88 : 48;
 };
-constexpr int SOFTMAX_WARPS = 8, CODE_WARP = 8;
+constexpr int SOFTMAX_WARPS = 8, CODE_WARP = 8, CODE_WARPS = 8;
 constexpr int SCALES_AHEAD = 8;  // key tiles whose scales the block holds: more than the ring can be ahead of the softmax
 template <int N>
 __device__ __forceinline__ void more_registers() {
@@ -227,21 +227,18 @@ __device__ __forceinline__ bool chunk_of(const PromptArgs &a, int group, int64_t
   return p.row0 < (int64_t)p.n * group;
 }
 
-// Four codes of a word as BF16 (two words), exactly.
-template <int KIND>
-__device__ __forceinline__ uint2 codes_bf16(uint32_t w) {
-  uint32_t r[2];
-#pragma unroll
-  for (int i = 0; i < 2; i++) {
-    if constexpr (KIND == KV8_INT8) {  // byte u = code + 128: (128 + the low seven bits) less 128, or 256 where the code is below 0
-      const uint32_t t = __byte_perm(w, 0x43434343u, i ? 0x4342 : 0x4140);
-      asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(r[i]) : "r"(t & 0xFF7FFF7Fu), "r"((t & 0x00800080u) ^ 0x43804380u));
-    } else {  // sign, exponent and mantissa in BF16's places are the value times 2^-120
-      const uint32_t t = __byte_perm(w, 0u, i ? 0x3424 : 0x1404);
-      asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r[i]) : "r"((t & 0x80008000u) | ((t >> 4) & 0x07F007F0u)), "r"(0x7B807B80u));
-    }
+// Two codes, of the low or the HIGH half of a word, as BF16, exactly.
+template <int KIND, bool HIGH>
+__device__ __forceinline__ uint32_t codes_bf16(uint32_t w) {
+  uint32_t r;
+  if constexpr (KIND == KV8_INT8) {  // byte u = code + 128: (128 + the low seven bits) less 128, or 256 where the code is below 0
+    const uint32_t t = __byte_perm(w, 0x43434343u, HIGH ? 0x4342 : 0x4140);
+    asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(t & 0xFF7FFF7Fu), "r"((t & 0x00800080u) ^ 0x43804380u));
+  } else {  // sign, exponent and mantissa in BF16's places are the value times 2^-120
+    const uint32_t t = __byte_perm(w, 0u, HIGH ? 0x3424 : 0x1404);
+    asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"((t & 0x80008000u) | ((t >> 4) & 0x07F007F0u)), "r"(0x7B807B80u));
   }
-  return make_uint2(r[0], r[1]);
+  return r;
 }
 __device__ __forceinline__ void sts8(uint32_t at, uint2 v) { asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(at), "r"(v.x), "r"(v.y) : "memory"); }
 __device__ __forceinline__ void sts16(uint32_t at, uint4 v) { asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory"); }
@@ -304,9 +301,9 @@ __global__ void __launch_bounds__(Roles<SRC>::WARPS * 32, 1) prompt_kernel(const
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; i++) mm_bar_init(q_full + 8 * i, 1), mm_bar_init(s_full + 8 * i, 1), mm_bar_init(p_full + 8 * i, NQ == 2 ? 128 : 256), mm_bar_init(o_done + 8 * i, 1);
-    for (int i = 0; i < ST; i++) mm_bar_init(ring_full + 8 * i, CODES ? 4 : 1), mm_bar_init(ring_empty + 8 * i, 1);
-    for (int i = 0; i < SCALES_AHEAD; i++) mm_bar_init(scale_full + 8 * i, 4);
-    for (int i = 0; i < 2; i++) mm_bar_init(raw_full + 8 * i, 1), mm_bar_init(raw_empty + 8 * i, 4);
+    for (int i = 0; i < ST; i++) mm_bar_init(ring_full + 8 * i, CODES ? CODE_WARPS : 1), mm_bar_init(ring_empty + 8 * i, 1);
+    for (int i = 0; i < SCALES_AHEAD; i++) mm_bar_init(scale_full + 8 * i, CODE_WARPS);
+    for (int i = 0; i < 2; i++) mm_bar_init(raw_full + 8 * i, 1), mm_bar_init(raw_empty + 8 * i, CODE_WARPS);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == MMA_WARP) {
@@ -461,10 +458,20 @@ __global__ void __launch_bounds__(Roles<SRC>::WARPS * 32, 1) prompt_kernel(const
     fewer_registers<Roles<SRC>::OTHER_REGS>();
     // ---------------------------------------------------------------- codes to BF16
     if constexpr (CODES) {
-        constexpr int PIECES = BN * D / 2048;  // 16-byte pieces of a tile's codes that a thread has
+        constexpr int THREADS = CODE_WARPS * 32, PIECES = BN * D / 16 / THREADS;  // 16-byte pieces of a tile's codes that a thread has
       const int tid = (int)threadIdx.x - CODE_WARP * 32, full = p.L / a.c.block * a.c.block;
       const int64_t unit = p.b * a.kv_heads + kv;
       const uint16_t *const k_tail = a.c.k_tail + (unit * 2 + (work ? kv8_slot(a.c, p.b, p.held, p.L / a.c.block) : 0)) * a.c.block * D, *const v_tail = a.c.v_tail + (k_tail - a.c.k_tail);
+      // Where a thread's first piece lies: K sixteen dimensions of a key, V four dimensions of four keys. The next pieces lie
+      // K_STEP or V_STEP keys on, a multiple of eight: the swizzle is the same.
+      constexpr int K_STEP = THREADS * 16 / D, V_STEP = THREADS * 16 / D;
+      static_assert(K_STEP % 8 == 0, "");
+      const int k_key = tid / (D / 16), k_dim = tid % (D / 16) * 16, v_key = tid / (D / 4) * 4, v_dim = tid % (D / 4) * 4;
+      const uint32_t k_to = (k_dim / 64) * (BN * 128), k_lo = k_to + swz(k_key, k_dim % 64 / 8), k_hi = k_to + swz(k_key, k_dim % 64 / 8 + 1);
+      const bool k_swap = D > 64 && (tid & 4);  // lanes of the next 64 dimensions store their second half first: other banks
+      uint32_t v_to[4];
+#pragma unroll
+      for (int r = 0; r < 4; r++) v_to[r] = (v_dim / 64) * (BN * 128) + (v_dim % 8) * 2 + swz(v_key + r, v_dim % 64 / 8);
       int at = 0;
       bool ok = true;
       auto scale_of = [&](int j) {  // of both sides, for 16 keys a thread; 1 in the open block
@@ -475,39 +482,37 @@ __global__ void __launch_bounds__(Roles<SRC>::WARPS * 32, 1) prompt_kernel(const
       auto fetch = [&](bool values, int j) {
         const int s = at % ST, key0 = j * BN;
         const uint32_t to = ring_at + s * G::TILE_BYTES, raw = raw_at + (at % 2) * G::RAW_BYTES + tid * 16;
+        const bool whole = key0 + BN <= full;
         if (ok) ok = prompt_wait_warp(raw_full + 8 * (at % 2), (at / 2) & 1);
         if (at >= ST && ok) ok = prompt_wait_warp(ring_empty + 8 * s, ((at / ST) & 1) ^ 1);
         if (!ok) return;
 #pragma unroll
         for (int i = 0; i < PIECES; i++) {
-          const int q = tid + 128 * i;
-          if (values) {  // four keys of four dimensions
-            const int key = q / (D / 4) * 4, d = q % (D / 4) * 4;
-            const uint32_t dst = to + (d / 64) * (BN * 128) + (d % 8) * 2;
-            if (key0 + key < full) {
-              const uint4 w = lds16(raw + 2048 * i);
+          const uint32_t dst = to + i * (K_STEP * 128);
+          const uint4 w = lds16(raw + i * (THREADS * 16));
+          if (values) {
+            const int key = key0 + v_key + i * V_STEP;
+            if (whole || key < full) {  // (blocks have whole rows of four)
               const uint32_t a01 = __byte_perm(w.x, w.y, 0x5140), b01 = __byte_perm(w.x, w.y, 0x7362), a23 = __byte_perm(w.z, w.w, 0x5140), b23 = __byte_perm(w.z, w.w, 0x7362);
-              sts8(dst + swz(key, d % 64 / 8), codes_bf16<SRC>(__byte_perm(a01, a23, 0x5410)));
-              sts8(dst + swz(key + 1, d % 64 / 8), codes_bf16<SRC>(__byte_perm(a01, a23, 0x7632)));
-              sts8(dst + swz(key + 2, d % 64 / 8), codes_bf16<SRC>(__byte_perm(b01, b23, 0x5410)));
-              sts8(dst + swz(key + 3, d % 64 / 8), codes_bf16<SRC>(__byte_perm(b01, b23, 0x7632)));
+              sts8(dst + v_to[0], make_uint2(codes_bf16<SRC, false>(a01), codes_bf16<SRC, false>(a23)));
+              sts8(dst + v_to[1], make_uint2(codes_bf16<SRC, true>(a01), codes_bf16<SRC, true>(a23)));
+              sts8(dst + v_to[2], make_uint2(codes_bf16<SRC, false>(b01), codes_bf16<SRC, false>(b23)));
+              sts8(dst + v_to[3], make_uint2(codes_bf16<SRC, true>(b01), codes_bf16<SRC, true>(b23)));
             } else {
-#pragma unroll
-              for (int r = 0; r < 4; r++) sts8(dst + swz(key + r, d % 64 / 8), key0 + key + r < p.L ? *reinterpret_cast<const uint2 *>(v_tail + (int64_t)(key0 + key + r - full) * D + d) : make_uint2(0, 0));
+#pragma unroll 1
+              for (int r = 0; r < 4; r++) sts8(dst + (v_dim / 64) * (BN * 128) + (v_dim % 8) * 2 + swz(v_key + r, v_dim % 64 / 8), key + r < p.L ? *reinterpret_cast<const uint2 *>(v_tail + (int64_t)(key + r - full) * D + v_dim) : make_uint2(0, 0));
             }
-          } else {  // sixteen dimensions of a key
-            const int key = q / (D / 16), d = q % (D / 16) * 16;
-            const uint32_t dst = to + (d / 64) * (BN * 128);
+          } else {
+            const int key = key0 + k_key + i * K_STEP;
             uint4 lo = make_uint4(0, 0, 0, 0), hi = lo;
-            if (key0 + key < full) {
-              const uint4 w = lds16(raw + 2048 * i);
-              const uint2 c0 = codes_bf16<SRC>(w.x), c1 = codes_bf16<SRC>(w.y), c2 = codes_bf16<SRC>(w.z), c3 = codes_bf16<SRC>(w.w);
-              lo = make_uint4(c0.x, c0.y, c1.x, c1.y), hi = make_uint4(c2.x, c2.y, c3.x, c3.y);
-            } else if (key0 + key < p.L) {
-              const uint4 *const row = reinterpret_cast<const uint4 *>(k_tail + (int64_t)(key0 + key - full) * D + d);
+            if (whole || key < full) {
+              lo = make_uint4(codes_bf16<SRC, false>(w.x), codes_bf16<SRC, true>(w.x), codes_bf16<SRC, false>(w.y), codes_bf16<SRC, true>(w.y));
+              hi = make_uint4(codes_bf16<SRC, false>(w.z), codes_bf16<SRC, true>(w.z), codes_bf16<SRC, false>(w.w), codes_bf16<SRC, true>(w.w));
+            } else if (key < p.L) {
+              const uint4 *const row = reinterpret_cast<const uint4 *>(k_tail + (int64_t)(key - full) * D + k_dim);
               lo = row[0], hi = row[1];
             }
-            sts16(dst + swz(key, d % 64 / 8), lo), sts16(dst + swz(key, d % 64 / 8 + 1), hi);
+            sts16(dst + (k_swap ? k_hi : k_lo), k_swap ? hi : lo), sts16(dst + (k_swap ? k_lo : k_hi), k_swap ? lo : hi);
           }
         }
         if (!values) {  // both scales of the tile's keys, 16 at a time
@@ -566,7 +571,7 @@ __global__ void __launch_bounds__(Roles<SRC>::WARPS * 32, 1) prompt_kernel(const
       tmem_wait_loads();
       const int key0 = j * BN + col0;
       const uint32_t scales = scales_at + (uint32_t)(((j - J0) % SCALES_AHEAD) * 2 * (BN / 16) + col0 / 16) * 4u;
-      if constexpr (CODES) {
+      if constexpr (CODES && !PLAIN) {
 #pragma unroll
         for (int x = 0; x < CN; x += 16) {
           const float ks = lds_f32(scales + x / 4);
@@ -610,11 +615,24 @@ __global__ void __launch_bounds__(Roles<SRC>::WARPS * 32, 1) prompt_kernel(const
         for (int x = 0; x < CN; x++)
           if ((uint32_t)x - from >= count) s[x] = 0xFF800000u;  // -inf
       }
-      float top = __uint_as_float(s[0]), top2 = __uint_as_float(s[1]);
+      float top = -CUDART_INF_F, factor[CODES && PLAIN ? CN / 16 : 1];  // PLAIN over a cache: K's scale goes with c
+      if constexpr (CODES && PLAIN) {
 #pragma unroll
-      for (int x = 2; x < CN; x += 2) top = fmaxf(top, __uint_as_float(s[x])), top2 = fmaxf(top2, __uint_as_float(s[x + 1]));
-      top = fmaxf(top, top2);
-      if constexpr (PLAIN) top *= c;
+        for (int x = 0; x < CN; x += 16) {
+          factor[x / 16] = c * lds_f32(scales + x / 4);
+          float most = __uint_as_float(s[x]), most2 = __uint_as_float(s[x + 1]);
+#pragma unroll
+          for (int e = 2; e < 16; e += 2) most = fmaxf(most, __uint_as_float(s[x + e])), most2 = fmaxf(most2, __uint_as_float(s[x + e + 1]));
+          top = fmaxf(top, fmaxf(most, most2) * factor[x / 16]);
+        }
+      } else {
+        float top2 = __uint_as_float(s[1]);
+        top = __uint_as_float(s[0]);
+#pragma unroll
+        for (int x = 2; x < CN; x += 2) top = fmaxf(top, __uint_as_float(s[x])), top2 = fmaxf(top2, __uint_as_float(s[x + 1]));
+        top = fmaxf(top, top2);
+        if constexpr (PLAIN) top *= c;
+      }
       if constexpr (NQ == 1) {
         sts_f32(told(n, part), top);
         tc_fence_before();  // the other half's scores have been read when its weights are written over them
@@ -641,19 +659,23 @@ __global__ void __launch_bounds__(Roles<SRC>::WARPS * 32, 1) prompt_kernel(const
           }
         }
       }
-      const uint64_t cc = pair_f32(PLAIN ? c : 1.0f, PLAIN ? c : 1.0f), mm = pair_f32(-m, -m);
+      uint64_t cc = pair_f32(PLAIN ? c : 1.0f, PLAIN ? c : 1.0f), vv = 0;
+      const uint64_t mm = pair_f32(-m, -m);
       uint64_t sum = 0, sum2 = 0;
 #pragma unroll
       for (int x = 0; x < CN; x += 4) {
+        if (CODES && x % 16 == 0) {
+          if constexpr (PLAIN) cc = pair_f32(factor[CODES ? x / 16 : 0], factor[CODES ? x / 16 : 0]);
+          const float vs = lds_f32(scales + (BN / 16 + x / 16) * 4);
+          vv = pair_f32(vs, vs);
+        }
         float e0, e1, e2, e3;
         split_f32(fma_f32x2(pair_f32(__uint_as_float(s[x]), __uint_as_float(s[x + 1])), cc, mm), e0, e1);
         split_f32(fma_f32x2(pair_f32(__uint_as_float(s[x + 2]), __uint_as_float(s[x + 3])), cc, mm), e2, e3);
-        e0 = ex2(e0), e1 = ex2(e1), e2 = ex2(e2), e3 = ex2(e3);
-        sum = add_f32x2(sum, pair_f32(e0, e1)), sum2 = add_f32x2(sum2, pair_f32(e2, e3));
-        if constexpr (CODES) {
-          const float vs = lds_f32(scales + (BN / 16 + x / 16) * 4);
-          e0 *= vs, e1 *= vs, e2 *= vs, e3 *= vs;
-        }
+        uint64_t p01 = pair_f32(ex2(e0), ex2(e1)), p23 = pair_f32(ex2(e2), ex2(e3));
+        sum = add_f32x2(sum, p01), sum2 = add_f32x2(sum2, p23);
+        if constexpr (CODES) p01 = mul_f32x2(p01, vv), p23 = mul_f32x2(p23, vv);
+        split_f32(p01, e0, e1), split_f32(p23, e2, e3);
         s[x / 2] = bf16_pair(e0, e1), s[x / 2 + 1] = bf16_pair(e2, e3);
       }
       if constexpr (NQ == 2) {

@@ -62,6 +62,8 @@ int exchange_status(int *status);  // exchange.cu
 int exchange_status_reset();
 int kv8_status(int *status);  // kv8.cu
 int kv8_status_reset();
+int kv8_attend_status(int *status);  // kv8_attend.cu
+int kv8_attend_status_reset();
 int attention_status(int *status);  // attention.cu
 int attention_status_reset();
 // Attention of chunks over a cache (kv8_chunk.cu)

@@ -9,33 +9,6 @@ __device__ int g_kv8_error;  // 1: tokens were brought that the cache has no roo
 
 namespace {
 
-// The nearest code to x / scale, ties to the even one, for finite x; 0 for NaN, the largest code for an infinity.
-// As stored, with 128 added. x times the inverse is off by at most 2^-15 in a quotient of up to 127: only next to the
-// middle of two codes the real quotient decides, by the sign of x - middle * scale, which one rounding keeps.
-__device__ __forceinline__ uint32_t int8_code(float x, float scale, float inv) {
-  const float t = x * inv;
-  int q = __float2int_rn(t);  // NaN: 0
-  const float off = t - (float)q;
-  if (fabsf(fabsf(off) - 0.5f) < 0.0005f) {
-    const float middle = (float)q + (off > 0.0f ? 0.5f : -0.5f), side = fmaf(-middle, scale, x);
-    const int below = (int)floorf(middle);
-    q = side > 0.0f ? below + 1 : side < 0.0f ? below : below + (below & 1);
-  }
-  return (uint32_t)(min(max(q, -127), 127) + 128);
-}
-
-// Least power of two, at least 2^-100, times which 448 (the largest e4m3 value) is not below amax.
-__device__ __forceinline__ float e4m3_scale(float amax) {
-  const uint32_t u = __float_as_uint(amax);
-  const int e = (int)(u >> 23) - 127 - 8 + ((u & 0x7FFFFFu) > 0x600000u);
-  return __uint_as_float((uint32_t)(max(e, -100) + 127) << 23);
-}
-
-__device__ __forceinline__ float finite_size(float x) {
-  const float s = fabsf(x);
-  return s <= 3.4028235e38f ? s : 0.0f;
-}
-
 struct AppendArgs {
   bn_kv8 c;
   const uint16_t *k, *v;
@@ -44,15 +17,10 @@ struct AppendArgs {
   int tokens, rel;  // tokens a sequence brings at most; blocks of the cache that those can touch
 };
 
-// One block of tokens of one sequence and head, keys or values, by 128 threads: a full block is scaled, coded
-// and stored; the tokens of the blocks that were open or stay open go to the tail in BF16. CHUNKS: pieces of
-// eight values that a thread has: neighbours of one token, or for values two neighbours of four tokens, whose codes lie
-// together. The read of the new rows and the write of the codes bound it; a block
-// stays in registers between its maximum and its codes.
+// A block per block of tokens, keys or values. The read of the new rows and the write of the codes bound it.
 template <int CHUNKS>
 __global__ void __launch_bounds__(128) append_kernel(const __grid_constant__ AppendArgs a) {
   const bn_kv8 &c = a.c;
-  __shared__ float part_max[4];
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");  // what made the tokens, and what read the cache before
   uint32_t at = blockIdx.x;
@@ -61,78 +29,14 @@ __global__ void __launch_bounds__(128) append_kernel(const __grid_constant__ App
   const int rel = (int)(at % a.rel);
   at /= a.rel;
   const int h = (int)(at % (uint32_t)c.kv_heads);
-  const int64_t b = at / (uint32_t)c.kv_heads, unit = b * c.kv_heads + h;
+  const int64_t b = at / (uint32_t)c.kv_heads;
   int held, brought;
-  kv8_tokens(c, a.counts, a.tokens, b, held, brought);
-  if (rel == 0 && h == 0 && !values && threadIdx.x == 0) {
-    const int asked = a.counts ? min(max(a.counts[b], 0), a.tokens) : a.tokens;
-    if (asked > brought) atomicExch(&g_kv8_error, 1);
-  }
-  if (brought == 0) return;
-  const int block = c.block, first = held / block, end = held + brought, last = (end - 1) / block;
-  const int D = (int)c.D;
-  const uint16_t *const in = values ? a.v + b * a.v_seq + h * a.v_head : a.k + b * a.k_seq + h * a.k_head;
-  const int64_t step = values ? a.v_token : a.k_token;
-  uint16_t *const tails = (values ? c.v_tail : c.k_tail) + unit * 2 * block * D;
-  const int j = first + rel;
-  if (j > last) return;
-  {
-    const bool full = (j + 1) * (int64_t)block <= end, open = j == first || !full;  // the first block goes to its slot, full or not
-    uint16_t *const tail = tails + (open ? kv8_slot(c, b, held, j) : 0) * block * D;
-    uint4 x[CHUNKS];
-    float amax = 0.0f;
-#pragma unroll
-    for (int i = 0; i < CHUNKS; i++) {
-      const int chunk = (int)threadIdx.x + 128 * i;
-      if (values) {
-        const int row = chunk / (D / 2) * 4, col = chunk % (D / 2) * 2;
-        uint32_t w[4] = {};
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-          const int p = j * block + row + e;
-          if (p < end && (full || p >= held)) w[e] = *reinterpret_cast<const uint32_t *>(p < held ? tail + (row + e) * D + col : in + (int64_t)(p - held) * step + col);
-          if (open && p >= held && p < end) *reinterpret_cast<uint32_t *>(tail + (row + e) * D + col) = w[e];
-        }
-        // dimension by dimension: the order in which the codes lie
-        x[i] = make_uint4(__byte_perm(w[0], w[1], 0x5410), __byte_perm(w[2], w[3], 0x5410), __byte_perm(w[0], w[1], 0x7632), __byte_perm(w[2], w[3], 0x7632));
-      } else {
-        const int row = chunk / (D / 8), col = chunk % (D / 8) * 8, p = j * block + row;
-        x[i] = make_uint4(0, 0, 0, 0);
-        if (p < end && (full || p >= held)) x[i] = *reinterpret_cast<const uint4 *>(p < held ? tail + row * D + col : in + (int64_t)(p - held) * step + col);
-        if (open && p >= held && p < end) *reinterpret_cast<uint4 *>(tail + row * D + col) = x[i];
-      }
-      const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
-#pragma unroll
-      for (int e = 0; e < 4; e++) amax = fmaxf(amax, fmaxf(finite_size(__uint_as_float(w[e] << 16)), finite_size(__uint_as_float(w[e] & 0xFFFF0000u))));
-    }
-    if (!full) return;
-#pragma unroll
-    for (int d = 16; d; d >>= 1) amax = fmaxf(amax, __shfl_xor_sync(BN_FULL, amax, d));
-    if (lane_id() == 0) part_max[threadIdx.x >> 5] = amax;
-    __syncthreads();
-    amax = fmaxf(fmaxf(part_max[0], part_max[1]), fmaxf(part_max[2], part_max[3]));
-    const float scale = c.kind == KV8_INT8 ? fmaxf(__fdiv_rn(amax, 127.0f), 7.888609052210118e-31f) : e4m3_scale(amax);
-    const float inv = __frcp_rn(scale);  // (of a power of two: exact)
-    uint8_t *const codes = (values ? c.v : c.k) + (unit * c.rows + (int64_t)j * block) * D;
-    if (threadIdx.x == 0) (values ? c.v_scale : c.k_scale)[unit * (c.rows / block) + j] = scale;
-#pragma unroll
-    for (int i = 0; i < CHUNKS; i++) {
-      const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
-      uint32_t out[2];
-#pragma unroll
-      for (int e = 0; e < 2; e++) {
-        float f[4] = {__uint_as_float(w[2 * e] << 16), __uint_as_float(w[2 * e] & 0xFFFF0000u), __uint_as_float(w[2 * e + 1] << 16), __uint_as_float(w[2 * e + 1] & 0xFFFF0000u)};
-        if (c.kind == KV8_INT8) {
-          out[e] = int8_code(f[0], scale, inv) | int8_code(f[1], scale, inv) << 8 | int8_code(f[2], scale, inv) << 16 | int8_code(f[3], scale, inv) << 24;
-        } else {
-#pragma unroll
-          for (int n = 0; n < 4; n++) f[n] = f[n] == f[n] ? f[n] * inv : 0.0f;
-          out[e] = (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(f[0], f[1]), __NV_SATFINITE, __NV_E4M3) | (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(f[2], f[3]), __NV_SATFINITE, __NV_E4M3) << 16;
-        }
-      }
-      *reinterpret_cast<uint2 *>(codes + ((int64_t)threadIdx.x + 128 * i) * 8) = make_uint2(out[0], out[1]);
-    }
-  }
+  const bool all = kv8_tokens(c, a.counts, a.tokens, b, held, brought);
+  if (!all && rel == 0 && h == 0 && !values && threadIdx.x == 0) atomicExch(&g_kv8_error, 1);
+  const int j = held / c.block + rel;
+  if (brought == 0 || j > (held + brought - 1) / c.block) return;
+  const bool v = values;
+  append_block<CHUNKS>(c, v, b, h, j, held, held + brought, v ? a.v + b * a.v_seq + h * a.v_head : a.k + b * a.k_seq + h * a.k_head, v ? a.v_token : a.k_token);
 }
 
 __global__ void __launch_bounds__(256) advance_kernel(const __grid_constant__ bn_kv8 c, int n, const int32_t *__restrict__ counts) {

@@ -20,7 +20,10 @@
 // A warp streams its own keys through a cp.async ring of its own: no barrier in the loop; the warps of a block
 // are joined at the end. The work is the tiles of all sequences and heads in a row, cut into equal
 // shares: sequences of unequal lengths load the SMs alike, and one long one spreads over all of them. A sequence and head
-// that is cut leaves partial sums, joined by a second kernel.
+// that is cut leaves partial sums; the block that finishes last joins them (it takes the last of the tickets), always in
+// the same order. The block with a sequence's last tile also appends the new tokens, reads them where they came from, and
+// codes the block that they fill before it reads it: a decode step is one launch. Several groups of rows (more than
+// 32, or 16 with heads of 256) read what an append kernel has written, and a second kernel joins them.
 //
 // Figures: at attend_launch.
 #include <cuda_bf16.h>
@@ -31,7 +34,11 @@
 namespace bn {
 namespace {
 
+__device__ int g_attend_error;  // 1: tokens were brought that the cache has no room for
+__device__ __forceinline__ void kv8_overflow() { atomicExch(&g_attend_error, 1); }
+
 constexpr int WARPS = 4;
+constexpr int MIN_SHARE = 1;
 constexpr float HEADROOM = 15.0f;  // weights may reach 2^15
 constexpr float NOTHING = -3.402823466e38f;  // a row's m while no key was visible: finite, so that a masked score less m stays -inf
 
@@ -42,6 +49,8 @@ struct AttendArgs {
   int64_t q_seq, q_token, q_head, o_seq, o_token, o_head;  // elements
   const int32_t *counts, *prefix;
   const float *slopes;
+  const uint16_t *k, *v;  // new tokens to append, or NULL
+  int64_t k_seq, k_token, k_head, v_seq, v_token, v_head;
   int tokens, heads, group;  // group: query heads of a key head
   int window, causal, zero_rest;
   float scale, cap;
@@ -66,22 +75,23 @@ struct Shape {
   static constexpr int PART = ROWS * (D + 2);          // floats of a partial result: sums, then maxima and weights
 };
 
-// Tiles of sequence b, its first key and full blocks' end. The last tile is the open block's, if it holds tokens.
+// Tiles of sequence b: of the blocks that are full before `split` from the first key on, then one of everything behind.
+// split is the end of the blocks that were full before the call where the call appends, else of those that are full now.
 struct Span {
-  int held, brought, L, full, start, quant, tiles;
+  int held, brought, L, full, split, start, quant, tiles;
 };
 __device__ __forceinline__ Span span_of(const AttendArgs &a, int64_t b, int tile) {
   Span s;
   kv8_tokens(a.c, a.counts, a.tokens, b, s.held, s.brought);
-  s.L = s.held + s.brought, s.full = s.L / a.c.block * a.c.block, s.start = 0;
+  const int log2 = 31 - __clz(a.c.block);
+  s.L = s.held + s.brought, s.full = s.L >> log2 << log2, s.split = a.k ? s.held >> log2 << log2 : s.full, s.start = 0;
   if (s.brought == 0) {
     s.quant = s.tiles = 0;
     return s;
   }
-  if (a.window > 0) s.start = max(0, s.held - a.window + 1) & ~15;  // the first query looks back furthest
-  s.start = min(s.start, s.full);
-  s.quant = (s.full - s.start + tile - 1) / tile;
-  s.tiles = s.quant + (s.L > s.full);
+  if (a.window > 0) s.start = min(max(0, s.held - a.window + 1) & ~15, s.split);  // the first query looks back furthest
+  s.quant = (s.split - s.start + tile - 1) / tile;
+  s.tiles = s.quant + (s.L > s.split);
   return s;
 }
 
@@ -247,17 +257,41 @@ __device__ __forceinline__ constexpr int dim_of(int t, int n) {
   return D == 64 ? 8 * n + t : 128 * (t / 16) + 16 * n + t % 16;
 }
 
+// Where the open block's tokens are read: from the tail, the new ones where they came from (if they come with the call).
+struct OpenRows {
+  const uint16_t *k_tail, *v_tail, *k, *v;  // tails less the block's first token; new ones less `from` tokens
+  int64_t k_step, v_step;
+  int D, from;
+  __device__ __forceinline__ const uint16_t *key(int j) const { return j >= from ? k + j * k_step : k_tail + (int64_t)j * D; }
+  __device__ __forceinline__ const uint16_t *value(int j) const { return j >= from ? v + j * v_step : v_tail + (int64_t)j * D; }
+};
+
+// New tokens of one sequence and head that fill a block, into the cache, by the block's 128 threads.
+template <int D>
+__device__ __noinline__ void append_filled(const AttendArgs &a, int64_t b, int h, int held, int L) {
+  const int first = held / a.c.block, last = (L - 1) / a.c.block;
+  for (int side = 0; side < 2; side++) {
+    const uint16_t *const in = side ? a.v + b * a.v_seq + h * a.v_head : a.k + b * a.k_seq + h * a.k_head;
+    const int64_t step = side ? a.v_token : a.k_token;
+    for (int j = first; j <= last; j++) {
+      if (a.c.block == 16) append_block<16 * D / 1024>(a.c, side, b, h, j, held, L, in, step);
+      else if (a.c.block == 32) append_block<32 * D / 1024>(a.c, side, b, h, j, held, L, in, step);
+      else append_block<64 * D / 1024>(a.c, side, b, h, j, held, L, in, step);
+    }
+  }
+  __syncthreads();
+}
+
 // The open block's 16 tokens from `key0` on, in BF16. Weights go in two BF16 halves (hi + lo: 2^-17), values times 2^-23
 // with 2^23 in the weights' exponent, so that no sum of 63 of them passes fp32. Where a value is not finite, a
 // weight of zero must not touch it: those go one by one.
 template <int D, int MT, bool PLAIN>
-__device__ void open_block(const AttendArgs &a, const uint16_t *const (&qrow)[MT][2], const uint16_t *ktail, const uint16_t *vtail, int full, int L, int key0, const Rows<MT> &r, State<D, MT> &st) {
+__device__ void open_block(const AttendArgs &a, const uint16_t *const (&qrow)[MT][2], const OpenRows &rows, int L, int key0, const Rows<MT> &r, State<D, MT> &st) {
   const uint32_t lane = lane_id(), n = lane >> 2, c = lane & 3u;
-  const int last = L - 1 - full, at = key0 - full;  // the last token's row, this piece's first
   float x[MT][2][4] = {};
   const uint16_t *k[2];
 #pragma unroll
-  for (int j = 0; j < 2; j++) k[j] = ktail + (int64_t)min(at + 4 * (int)(n >> 1) + 2 * j + (int)(n & 1), last) * D + 16 * c;
+  for (int j = 0; j < 2; j++) k[j] = rows.key(min(key0 + 4 * (int)(n >> 1) + 2 * j + (int)(n & 1), L - 1)) + 16 * c;
 #pragma unroll 1
   for (int g = 0; g < D / 64; g++)
 #pragma unroll
@@ -290,7 +324,7 @@ __device__ void open_block(const AttendArgs &a, const uint16_t *const (&qrow)[MT
   const uint16_t *v[4];
   bool odd = false;
 #pragma unroll
-  for (int i = 0; i < 4; i++) v[i] = vtail + (int64_t)min(at + 4 * (int)c + i, last) * D;
+  for (int i = 0; i < 4; i++) v[i] = rows.value(min(key0 + 4 * (int)c + i, L - 1));
 #pragma unroll
   for (int t = 0; t < Shape<D, MT>::NT; t += 2) {
     uint32_t w[4];  // dims dim_of(t, n) and the next
@@ -323,7 +357,7 @@ __device__ void open_block(const AttendArgs &a, const uint16_t *const (&qrow)[MT
   }
 #pragma unroll
   for (int key = 0; key < 16; key++) {
-    const uint16_t *const row = vtail + (int64_t)min(at + key, last) * D;
+    const uint16_t *const row = rows.value(min(key0 + key, L - 1));
     const uint32_t from = (lane & ~3u) | (key >> 2);
 #pragma unroll
     for (int mt = 0; mt < MT; mt++)
@@ -339,6 +373,46 @@ __device__ void open_block(const AttendArgs &a, const uint16_t *const (&qrow)[MT
   }
 }
 
+// The parts of one sequence and head together, by the block that finished last: four dimensions a thread, eight parts at
+// a time. Parts lie in the workspace, two slots a block of the grid; late: the first part is in its block's second slot.
+template <int D, int MT>
+__device__ __noinline__ void join_parts(const AttendArgs &a, int64_t b, int kv, int rows, int brought, int64_t first, int parts, bool late) {
+  using S = Shape<D, MT>;
+  for (int i = (int)threadIdx.x; i < rows * (D / 4); i += WARPS * 32) {
+    const int row = i / (D / 4), col = i % (D / 4) * 4;
+    float m = NOTHING, l = 0.0f;
+    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int p0 = 0; p0 < parts; p0 += 8) {
+      float pm[8], pl[8];
+      float4 v[8];
+#pragma unroll
+      for (int u = 0; u < 8; u++) {
+        const int p = min(p0 + u, parts - 1);
+        const float *const part = a.parts + ((first + p) * 2 + (p == 0 && late ? 1 : 0)) * S::PART;
+        pm[u] = __ldcg(part + S::ROWS * D + row), pl[u] = __ldcg(part + S::ROWS * D + S::ROWS + row);
+        v[u] = __ldcg(reinterpret_cast<const float4 *>(part + row * D + col));
+      }
+      float top = m;
+#pragma unroll
+      for (int u = 0; u < 8; u++) top = fmaxf(top, pm[u]);
+      const float keep = ex2(m - top);
+      m = top, l *= keep, o.x *= keep, o.y *= keep, o.z *= keep, o.w *= keep;
+#pragma unroll
+      for (int u = 0; u < 8; u++) {
+        if (p0 + u >= parts) break;
+        const float f = ex2(pm[u] - top);
+        l = fmaf(f, pl[u], l);
+        o.x = fmaf(f, v[u].x, o.x), o.y = fmaf(f, v[u].y, o.y), o.z = fmaf(f, v[u].z, o.z), o.w = fmaf(f, v[u].w, o.w);
+      }
+    }
+    const int t = row / a.group, head = kv * a.group + row % a.group;
+    uint16_t *const out = a.out + b * a.o_seq + t * a.o_token + head * a.o_head + col;
+    const float inv = 1.0f / l;
+    if (t < brought) *reinterpret_cast<uint2 *>(out) = make_uint2(pack_bf16(o.x * inv, o.y * inv), pack_bf16(o.z * inv, o.w * inv));
+    else if (a.zero_rest) *reinterpret_cast<uint2 *>(out) = make_uint2(0, 0);
+  }
+}
+
 template <int D, int KIND, int MT, bool PLAIN>
 __global__ void __launch_bounds__(WARPS * 32, (D == 64 && MT == 1) ? 4 : (MT * D <= 128) ? 3 : 2) attend_kernel(const __grid_constant__ AttendArgs a) {
   using S = Shape<D, MT>;
@@ -346,6 +420,7 @@ __global__ void __launch_bounds__(WARPS * 32, (D == 64 && MT == 1) ? 4 : (MT * D
   extern __shared__ __align__(128) uint8_t attend_smem[];
   __shared__ int64_t found[2];
   __shared__ int64_t warp_tiles[WARPS];
+  __shared__ bool last_ticket;
   __shared__ float join_m[WARPS][S::ROWS], join_l[WARPS][S::ROWS];
   __shared__ float scales[WARPS][S::STAGES][2][S::KS / 16];
   const uint32_t lane = lane_id(), warp = threadIdx.x >> 5, n = lane >> 2, c = lane & 3u;
@@ -358,7 +433,20 @@ __global__ void __launch_bounds__(WARPS * 32, (D == 64 && MT == 1) ? 4 : (MT * D
   const int per_thread = (int)((cache.batch + WARPS * 32 - 1) / (WARPS * 32));
   const int64_t b_from = min((int64_t)threadIdx.x * per_thread, cache.batch), b_to = min(b_from + per_thread, cache.batch);
   int64_t mine = 0;
-  for (int64_t b = b_from; b < b_to; b++) mine += span_of(a, b, S::TILE).tiles;
+  bool nothing = false;
+  for (int64_t b = b_from; b < b_to; b++) {
+    const Span s = span_of(a, b, S::TILE);
+    mine += s.tiles;
+    nothing |= s.brought == 0;
+    if (a.k && blockIdx.x == 0 && s.brought < (a.counts ? min(max(a.counts[b], 0), a.tokens) : a.tokens)) kv8_overflow();
+  }
+  if (__syncthreads_or(nothing && a.zero_rest))  // sequences that bring nothing have no tiles: their rows are zeroed here
+    for (int64_t b = blockIdx.x; b < cache.batch; b += gridDim.x)
+      if (span_of(a, b, S::TILE).brought == 0)
+        for (int i = (int)threadIdx.x; i < a.tokens * a.heads * (D / 8); i += WARPS * 32) {
+          const int row = i / (D / 8);
+          *reinterpret_cast<uint4 *>(a.out + b * a.o_seq + row / a.heads * a.o_token + row % a.heads * a.o_head + i % (D / 8) * 8) = make_uint4(0, 0, 0, 0);
+        }
   int64_t upto = mine;
 #pragma unroll
   for (int d = 1; d < 32; d <<= 1) {
@@ -373,7 +461,7 @@ __global__ void __launch_bounds__(WARPS * 32, (D == 64 && MT == 1) ? 4 : (MT * D
     if (w < (int)warp) before += warp_tiles[w];
     total += warp_tiles[w];
   }
-  const int64_t share = max((total * per_seq + a.blocks - 1) / a.blocks, (int64_t)1);
+  const int64_t share = max((total * per_seq + a.blocks - 1) / a.blocks, (int64_t)MIN_SHARE);
   int64_t x = (int64_t)blockIdx.x * share;
   const int64_t x_end = min(x + share, total * per_seq);
   for (int64_t b = b_from, at = before; b < b_to; b++) {
@@ -404,14 +492,19 @@ __global__ void __launch_bounds__(WARPS * 32, (D == 64 && MT == 1) ? 4 : (MT * D
     const uint8_t *const codes[2] = {cache.k + unit * cache.rows * D, cache.v + unit * cache.rows * D};
     const int64_t scale_at = unit * (cache.rows / cache.block);
 
+    // The block of the last tile appends: first, if the new tokens fill a block, which is then one more tile of codes
+    // (from `split` on); else beside the copies.
+    const bool appends = a.k && tile_end == s.tiles, fills = appends && s.full > s.split;
+    const int codes_end = fills ? s.quant + 1 : min(tile_end, s.quant);
+    auto key_of = [&](int t) { return (t < s.quant ? s.start + t * S::TILE : s.split) + (int)warp * S::KS; };
     // this warp's keys of tile t, 16 at a time: those of the full blocks come in whole pieces
     auto issue = [&](int t, int slot) {
-      if (t < min(tile_end, s.quant)) {
-        const int key0 = s.start + t * S::TILE + (int)warp * S::KS;
+      if (t < codes_end) {
+        const int key0 = key_of(t), end = t < s.quant ? s.split : s.full;
         const uint32_t to = ring + slot * S::STAGE_BYTES;
 #pragma unroll
         for (int sub = 0; sub < S::KS / 16; sub++) {
-          if (key0 + 16 * sub >= s.full) break;
+          if (key0 + 16 * sub >= end) break;
 #pragma unroll
           for (int side = 0; side < 2; side++) {
             const uint8_t *const from = codes[side] + (int64_t)(key0 + 16 * sub) * D + lane * 16;
@@ -427,8 +520,17 @@ __global__ void __launch_bounds__(WARPS * 32, (D == 64 && MT == 1) ? 4 : (MT * D
       }
       copies_commit();
     };
+    if (fills) append_filled<D>(a, b, kv, s.held, s.L);
 #pragma unroll
     for (int i = 0; i < S::STAGES - 1; i++) issue(tile + i, i);
+    if (appends && !fills) {  // rows of the open block, which nobody reads in this call: nothing waits for them
+      const int64_t to = ((unit * 2 + kv8_slot(cache, b, s.held, s.held >> block_log2)) * cache.block + (s.held & (cache.block - 1))) * D;
+      for (int i = (int)threadIdx.x; i < 2 * s.brought * (D / 8); i += WARPS * 32) {
+        const int side = i & 1, row = (i >> 1) / (D / 8), col = (i >> 1) % (D / 8) * 8;
+        const uint16_t *const from = side ? a.v + b * a.v_seq + row * a.v_token + kv * a.v_head : a.k + b * a.k_seq + row * a.k_token + kv * a.k_head;
+        *reinterpret_cast<uint4 *>((side ? cache.v_tail : cache.k_tail) + to + row * D + col) = *reinterpret_cast<const uint4 *>(from + col);
+      }
+    }
 
     // ---- the rows of this lane: n and n + 8 of each 16
     const int t_first = row0 / a.group, t_last = min((row0 + rows - 1) / a.group, s.brought - 1);
@@ -485,18 +587,18 @@ __global__ void __launch_bounds__(WARPS * 32, (D == 64 && MT == 1) ? 4 : (MT * D
 
     // ---- full blocks
     int slot = 0;
-    const int quant_end = min(tile_end, s.quant);
-    for (int t = tile; t < quant_end; t++) {
+    for (int t = tile; t < codes_end; t++) {
       copies_wait<S::STAGES - 2>();
       __syncwarp();  // this tile's copies of all lanes are there, and the slot of the tile before is read
       issue(t + S::STAGES - 1, slot == 0 ? S::STAGES - 1 : slot - 1);
       const uint32_t at = ring + slot * S::STAGE_BYTES;
 #pragma unroll
       for (int sub = 0; sub < S::KS / 16; sub++) {
-        const int key0 = s.start + t * S::TILE + (int)warp * S::KS + 16 * sub;
-        if (key0 >= s.full) break;
+        const int key0 = key_of(t) + 16 * sub;
+        if (key0 >= (t < s.quant ? s.split : s.full)) break;
         const float kscale = scales[warp][slot][0][sub], vscale = scales[warp][slot][1][sub];
         float x[MT][2][4] = {};
+        float x2[MT][2][4] = {};  // every other product, for shorter chains
 #pragma unroll
         for (int g = 0; g < D / 64; g++)
 #pragma unroll
@@ -508,9 +610,15 @@ __global__ void __launch_bounds__(WARPS * 32, (D == 64 && MT == 1) ? 4 : (MT * D
             for (int e = 0; e < 4; e++) {
               const uint32_t b0 = codes_f16<KIND, false>(w[e]), b1 = codes_f16<KIND, true>(w[e]);
 #pragma unroll
-              for (int mt = 0; mt < MT; mt++) mma_f16(x[mt][j], q[mt][4 * g + e], b0, b1);
+              for (int mt = 0; mt < MT; mt++) mma_f16(MT == 1 && (e & 1) ? x2[mt][j] : x[mt][j], q[mt][4 * g + e], b0, b1);
             }
           }
+        if constexpr (MT == 1) {
+#pragma unroll
+          for (int j = 0; j < 2; j++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) x[0][j][e] += x2[0][j][e];
+        }
         float vlog;
         asm("lg2.approx.f32 %0, %1;" : "=f"(vlog) : "f"(vscale));
         weigh<D, MT, PLAIN>(a, x, r, st, key0, kscale, vlog, __fdividef(1.0f, vscale), key0 < lo_most || key0 + 16 > hi_least);
@@ -538,8 +646,10 @@ __global__ void __launch_bounds__(WARPS * 32, (D == 64 && MT == 1) ? 4 : (MT * D
     }
     // ---- the open block
     if (tile_end == s.tiles && s.L > s.full) {
-      const int64_t tail_at = (unit * 2 + kv8_slot(cache, b, s.held, s.full / cache.block)) * cache.block * D;
-      for (int key0 = s.full + 16 * (int)warp; key0 < s.L; key0 += 16 * WARPS) open_block<D, MT, PLAIN>(a, qrow, cache.k_tail + tail_at, cache.v_tail + tail_at, s.full, s.L, key0, r, st);
+      const int64_t tail_at = ((unit * 2 + kv8_slot(cache, b, s.held, s.full / cache.block)) * cache.block - s.full) * D;
+      OpenRows rows{cache.k_tail + tail_at, cache.v_tail + tail_at, nullptr, nullptr, a.k_token, a.v_token, D, s.L};
+      if (a.k) rows.from = s.held, rows.k = a.k + b * a.k_seq + kv * a.k_head - s.held * a.k_token, rows.v = a.v + b * a.v_seq + kv * a.v_head - s.held * a.v_token;
+      for (int key0 = s.full + 16 * (int)warp; key0 < s.L; key0 += 16 * WARPS) open_block<D, MT, PLAIN>(a, qrow, rows, s.L, key0, r, st);
     }
 
     // ---- the warps' results together
@@ -590,6 +700,19 @@ __global__ void __launch_bounds__(WARPS * 32, (D == 64 && MT == 1) ? 4 : (MT * D
         if (col == 0) part[S::ROWS * D + row] = m, part[S::ROWS * D + S::ROWS + row] = l;
       }
     }
+    if (!whole && a.row_groups == 1) {  // the last block of this sequence and head joins
+      const int64_t from = x - tile;
+      const int64_t left = from / share, right = (from + s.tiles - 1) / share;
+      __syncthreads();
+      if (threadIdx.x == 0) {
+        __threadfence();
+        const uint32_t ticket = atomicAdd(cache.tickets + unit, 1u);
+        last_ticket = ticket == (uint32_t)(right - left);
+        if (last_ticket) cache.tickets[unit] = 0, __threadfence();
+      }
+      __syncthreads();
+      if (last_ticket) join_parts<D, MT>(a, b, kv, rows, s.brought, left, (int)(right - left) + 1, from != left * share);
+    }
     x += tile_end - tile;
     if (x >= x_end) return;
     __syncthreads();  // the join's shared memory is the ring's
@@ -602,8 +725,8 @@ __global__ void __launch_bounds__(WARPS * 32, (D == 64 && MT == 1) ? 4 : (MT * D
   }
 }
 
-// Joins what blocks left of a sequence and head that was cut, and zeroes the rows of sequences that brought nothing.
-// A block per query row: a thread has four dimensions of every few parts.
+// Joins what blocks left of a sequence and head that was cut, where there are several groups of rows. A block per query
+// row: a thread has four dimensions of every few parts.
 constexpr int JOIN_THREADS = 256;
 
 template <int D, int MT>
@@ -626,12 +749,7 @@ __global__ void __launch_bounds__(JOIN_THREADS) join_kernel(const __grid_constan
   if ((first + 1) * share <= from) first++;
   const int t = r / a.group, head = kv * a.group + r % a.group;
   uint16_t *const out = a.out + b * a.o_seq + t * a.o_token + head * a.o_head;
-  if (tiles == 0) {
-    if (a.zero_rest)
-      for (int i = (int)threadIdx.x; i < D / 8; i += JOIN_THREADS) *reinterpret_cast<uint4 *>(out + 8 * i) = make_uint4(0, 0, 0, 0);
-    return;
-  }
-  if ((first + 1) * share >= to) return;  // one block's: it wrote the output
+  if (tiles == 0 || (first + 1) * share >= to) return;  // nothing, or one block's, which wrote the output
   int parts = 1;
   while ((first + parts) * share < to) parts += max(1, (int)((to - (first + parts) * share) / share));
   auto part_of = [&](int p) { return a.parts + ((first + p) * 2 + (p == 0 && from != first * share ? 1 : 0)) * S::PART; };
@@ -712,6 +830,7 @@ int attend_launch(const AttendArgs &a, cudaStream_t stream) {
   cfg.gridDim = dim3((unsigned)a.blocks), cfg.blockDim = dim3(WARPS * 32), cfg.dynamicSmemBytes = S::SMEM, cfg.stream = stream, cfg.attrs = attr, cfg.numAttrs = 1;
   BN_CUDA(allow_smem(attend_kernel<D, KIND, MT, PLAIN>, S::SMEM));
   BN_CUDA(cudaLaunchKernelEx(&cfg, attend_kernel<D, KIND, MT, PLAIN>, a));
+  if (a.row_groups == 1) return launched("attend_kernel");
   cfg.gridDim = dim3((unsigned)(a.c.batch * a.heads * a.tokens)), cfg.blockDim = dim3(JOIN_THREADS), cfg.dynamicSmemBytes = 0;
   BN_CUDA(cudaLaunchKernelEx(&cfg, join_kernel<D, MT>, a));
   return launched("attend_kernel");
@@ -735,6 +854,18 @@ bool chunk_wins(const bn_kv8 *c, int64_t tokens, int64_t heads) {
 bool attend_sizes(const bn_kv8 *c, int64_t tokens, int64_t heads) { return tokens >= 0 && tokens <= 0x3FFFFFFF && heads >= 1 && heads <= 4096 && heads % c->kv_heads == 0; }
 
 }  // namespace
+
+int kv8_attend_status(int *status) {
+  BN_CUDA(cudaMemcpyFromSymbol(status, g_attend_error, sizeof(int)));
+  return BN_OK;
+}
+
+int kv8_attend_status_reset() {
+  const int zero = 0;
+  BN_CUDA(cudaMemcpyToSymbol(g_attend_error, &zero, sizeof(int)));
+  return BN_OK;
+}
+
 }  // namespace bn
 
 extern "C" uint64_t bn_kv8_workspace(const bn_kv8 *c, int64_t tokens, int64_t heads) {
@@ -759,9 +890,12 @@ extern "C" int bn_kv8_attend(const bn_kv8 *c, const uint16_t *q, int64_t q_seq, 
   }
   if (!workspace || (uintptr_t)workspace & 15 || workspace_bytes < p.bytes) return bn::fail(BN_ERR_CAPACITY, "bn_kv8_attend: the workspace is smaller than bn_kv8_workspace says, or not on 16 bytes");
   if (c->batch * heads * tokens > 0x7FFFFFFF) return bn::fail(BN_ERR_ARG, "bn_kv8_attend: too many rows for one call");
-  if (k)
+  if (k && (((uintptr_t)k | (uintptr_t)v) & 15 || (k_seq | k_token | k_head | v_seq | v_token | v_head) & 7)) return bn::fail(BN_ERR_ARG, "bn_kv8_attend: rows have to start on 16 bytes");
+  if (k && (p.row_groups > 1 || tokens > 16)) {  // (16 tokens fill one block at most)
     if (const int e = bn_kv8_append(c, k, k_seq, k_token, k_head, v, v_seq, v_token, v_head, tokens, counts, stream)) return e;
-  bn::AttendArgs a{*c, q, out, q_seq, q_token, q_head, o_seq, o_token, o_head, counts, prefix, scores->slopes, (int)tokens, (int)heads, (int)(heads / c->kv_heads), (int)scores->window, scores->causal, zero_rest, scores->scale, scores->softcap, (int64_t *)workspace, (float *)((uint8_t *)workspace + p.plan_bytes), p.row_groups, p.blocks};
+    k = v = nullptr;
+  }
+  bn::AttendArgs a{*c, q, out, q_seq, q_token, q_head, o_seq, o_token, o_head, counts, prefix, scores->slopes, k, v, k_seq, k_token, k_head, v_seq, v_token, v_head, (int)tokens, (int)heads, (int)(heads / c->kv_heads), (int)scores->window, scores->causal, zero_rest, scores->scale, scores->softcap, (int64_t *)workspace, (float *)((uint8_t *)workspace + p.plan_bytes), p.row_groups, p.blocks};
   const cudaStream_t s = (cudaStream_t)stream;
   if (scores->softcap == 0.0f && !scores->slopes) return c->kind == BN_KV8_INT8 ? bn::attend_kind<BN_KV8_INT8, true>(a, p.mt, s) : bn::attend_kind<BN_KV8_E4M3, true>(a, p.mt, s);
   return c->kind == BN_KV8_INT8 ? bn::attend_kind<BN_KV8_INT8, false>(a, p.mt, s) : bn::attend_kind<BN_KV8_E4M3, false>(a, p.mt, s);

@@ -639,6 +639,7 @@ extern "C" int bn_device_status_reset(void) {
   if (int e = bn::oct_rows_status_reset()) return e;
   if (int e = bn::mma_status_reset()) return e;
   if (int e = bn::kv8_status_reset()) return e;
+  if (int e = bn::kv8_attend_status_reset()) return e;
   if (int e = bn::attention_status_reset()) return e;
   if (int e = bn::kv8_chunk_status_reset()) return e;
   return bn::exchange_status_reset();
@@ -655,6 +656,8 @@ extern "C" int bn_device_status(int *status) {
   if (int e = bn::mma_status(&mma)) return e;
   if (int e = bn::exchange_status(&xch)) return e;
   if (int e = bn::kv8_status(&kv8)) return e;
+  if (int e = bn::kv8_attend_status(&oct)) return e;
+  kv8 |= oct;
   if (int e = bn::attention_status(&attention)) return e;
   if (int e = bn::kv8_chunk_status(&chunk)) return e;
   *status = stream | (mma << 8) | (xch << 16) | (kv8 << 24) | ((attention | chunk) << 28);

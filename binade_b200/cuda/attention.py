@@ -65,7 +65,7 @@ def overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
 
 def _out(out, like: torch.Tensor, device, *inputs) -> torch.Tensor:
     if out is None:
-        return torch.empty(like.shape, dtype=torch.bfloat16, device=like.device)
+        return torch.empty_like(like, memory_format=torch.contiguous_format)
     if not isinstance(out, torch.Tensor) or out.dtype != torch.bfloat16 or out.shape != like.shape or out.get_device() != device or out.requires_grad:
         raise ValueError("out has to be a bfloat16 tensor of q's shape on its device")
     if out.stride(-1) != 1 or out.data_ptr() % 16 or any(s % 8 or s == 0 for s, n in zip(out.stride()[:-1], out.shape[:-1]) if n > 1):
@@ -162,7 +162,8 @@ class KV8Cache:
         self.k_scale, self.v_scale = new(rows // block, dtype=torch.float32), new(rows // block, dtype=torch.float32)
         self.k_tail, self.v_tail = new(2, block, head_dim, dtype=torch.bfloat16), new(2, block, head_dim, dtype=torch.bfloat16)
         self.length, self._side = torch.zeros(batch, dtype=torch.int32, device=self.device), torch.zeros(batch, dtype=torch.int32, device=self.device)
-        self._structs = [_native.KV8Struct(*(t[i].data_ptr() for t in (self.k, self.v, self.k_scale, self.v_scale, self.k_tail, self.v_tail)), self.length.data_ptr(), self._side.data_ptr(), batch, kv_heads, rows, head_dim, max_seq, block, KINDS[kind]) for i in range(layers)]
+        self._tickets = torch.zeros(batch * kv_heads, dtype=torch.int32, device=self.device)
+        self._structs = [_native.KV8Struct(*(t[i].data_ptr() for t in (self.k, self.v, self.k_scale, self.v_scale, self.k_tail, self.v_tail)), self.length.data_ptr(), self._side.data_ptr(), self._tickets.data_ptr(), batch, kv_heads, rows, head_dim, max_seq, block, KINDS[kind]) for i in range(layers)]
 
     def bytes(self) -> int:
         """Device memory of the cache."""
@@ -224,8 +225,8 @@ class KV8Cache:
             need = self._work.get((tokens, heads))
             if need is None:
                 need = self._work[tokens, heads] = _native.load("cuda").bn_kv8_workspace(at, tokens, heads)
-            work = torch.empty(need, dtype=torch.uint8, device=self.device)
-            ck._call("bn_kv8_attend", at, q.data_ptr(), *_steps(q), *new, tokens, heads, ck._p(counts), ck._p(prefix), ctypes.byref(scores), y.data_ptr(), *_steps(y), int(out is None), work.data_ptr(), need)
+            work = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
+            ck._call("bn_kv8_attend", at, q.data_ptr(), *_steps(q), *new, tokens, heads, ck._p(counts), ck._p(prefix), ctypes.byref(scores), y.data_ptr(), *_steps(y), int(out is None), ck._p(work), need)
         return y
 
     def advance(self, n) -> None:

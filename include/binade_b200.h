@@ -325,6 +325,7 @@ typedef struct bn_kv8 {
   float *k_scale, *v_scale;
   uint16_t *k_tail, *v_tail;
   int32_t *length, *side;
+  uint32_t *tickets; /* [batch * kv_heads] zeros, for bn_kv8_attend, which leaves them so */
   int64_t batch, kv_heads, rows, D, max_seq;
   int block, kind;
 } bn_kv8;
@@ -339,7 +340,8 @@ int bn_kv8_append(const bn_kv8 *c, const uint16_t *k, int64_t k_seq, int64_t k_t
 /* Attention of those tokens over everything up to themselves, before `length` moves on. With k and v (NULL or not
  * together) they are appended first; otherwise bn_kv8_append did it. Query t of sequence b has position length[b] + t, its keys are the length[b] + counts[b] first.
  * prefix [batch] or NULL. Rows of tokens that are not real are zeroed if zero_rest, else left as they are.
- * workspace: bn_kv8_workspace bytes on 16 bytes, for this call alone. */
+ * workspace: bn_kv8_workspace bytes on 16 bytes, for this call alone (NULL if none). Calls on one cache must not
+ * overlap: they share its tickets. */
 uint64_t bn_kv8_workspace(const bn_kv8 *c, int64_t tokens, int64_t heads);
 int bn_kv8_attend(const bn_kv8 *c, const uint16_t *q, int64_t q_seq, int64_t q_token, int64_t q_head,
                   const uint16_t *k, int64_t k_seq, int64_t k_token, int64_t k_head, const uint16_t *v,

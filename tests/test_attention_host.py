@@ -12,7 +12,7 @@ BUF = 0x10000  # an aligned address that no call below gets to read
 
 
 def cache(**change):
-    c = _native.KV8Struct(*([BUF] * 8), 2, 2, 128, 128, 100, 32, 0)
+    c = _native.KV8Struct(*([BUF] * 9), 2, 2, 128, 128, 100, 32, 0)
     for k, v in change.items():
         setattr(c, k, v)
     return c
@@ -40,7 +40,7 @@ def test_attention_of_nothing():
     assert attention(T=0, q=None, k=None, v=None, out=None) == 0
 
 
-BAD_CACHES = [dict(k=None), dict(v_scale=None), dict(length=None), dict(side=None), dict(k=BUF + 4), dict(D=80), dict(block=8), dict(block=48), dict(kind=2), dict(batch=0), dict(kv_heads=0), dict(rows=64), dict(rows=100), dict(max_seq=0), dict(max_seq=1 << 31)]
+BAD_CACHES = [dict(k=None), dict(v_scale=None), dict(length=None), dict(side=None), dict(tickets=None), dict(k=BUF + 4), dict(D=80), dict(block=8), dict(block=48), dict(kind=2), dict(batch=0), dict(kv_heads=0), dict(rows=64), dict(rows=100), dict(max_seq=0), dict(max_seq=1 << 31)]
 
 
 @pytest.mark.parametrize("change", BAD_CACHES)

@@ -20,10 +20,10 @@
 // A warp streams its own keys through a cp.async ring of its own: no barrier in the loop; the warps of a block
 // are joined at the end. The work is the tiles of all sequences and heads in a row, cut into equal
 // shares: sequences of unequal lengths load the SMs alike, and one long one spreads over all of them. A sequence and head
-// that is cut leaves partial sums; the block that finishes last joins them (it takes the last of the tickets), always in
-// the same order. The block with a sequence's last tile also appends the new tokens, reads them where they came from, and
+// that is cut leaves partial sums; the block that finishes last joins them (it takes the last of the tickets), or, where
+// there may be many, a second kernel, always in the same order. The block with a sequence's last tile also appends the new tokens, reads them where they came from, and
 // codes the block that they fill before it reads it: a decode step is one launch. Several groups of rows (more than
-// 32, or 16 with heads of 256) read what an append kernel has written, and a second kernel joins them.
+// 32, or 16 with heads of 256) read what an append kernel has written.
 //
 // Figures: at attend_launch.
 #include <cuda_bf16.h>
@@ -59,6 +59,7 @@ struct AttendArgs {
   float *parts;
   int row_groups;
   int blocks;
+  bool join_here;  // by the block that finishes last; else by the join kernel
 };
 
 template <int D, int MT>
@@ -373,20 +374,21 @@ __device__ void open_block(const AttendArgs &a, const uint16_t *const (&qrow)[MT
   }
 }
 
-// The parts of one sequence and head together, by the block that finished last: four dimensions a thread, eight parts at
-// a time. Parts lie in the workspace, two slots a block of the grid; late: the first part is in its block's second slot.
+// The parts of one sequence and head together, by the block that finished last: four dimensions a thread, sixteen parts
+// at a time. Parts lie in the workspace, two slots a block of the grid; late: the first part is in its block's second slot.
 template <int D, int MT>
 __device__ __noinline__ void join_parts(const AttendArgs &a, int64_t b, int kv, int rows, int brought, int64_t first, int parts, bool late) {
   using S = Shape<D, MT>;
+  constexpr int U = 16;
   for (int i = (int)threadIdx.x; i < rows * (D / 4); i += WARPS * 32) {
     const int row = i / (D / 4), col = i % (D / 4) * 4;
     float m = NOTHING, l = 0.0f;
     float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    for (int p0 = 0; p0 < parts; p0 += 8) {
-      float pm[8], pl[8];
-      float4 v[8];
+    for (int p0 = 0; p0 < parts; p0 += U) {
+      float pm[U], pl[U];
+      float4 v[U];
 #pragma unroll
-      for (int u = 0; u < 8; u++) {
+      for (int u = 0; u < U; u++) {
         const int p = min(p0 + u, parts - 1);
         const float *const part = a.parts + ((first + p) * 2 + (p == 0 && late ? 1 : 0)) * S::PART;
         pm[u] = __ldcg(part + S::ROWS * D + row), pl[u] = __ldcg(part + S::ROWS * D + S::ROWS + row);
@@ -394,11 +396,11 @@ __device__ __noinline__ void join_parts(const AttendArgs &a, int64_t b, int kv, 
       }
       float top = m;
 #pragma unroll
-      for (int u = 0; u < 8; u++) top = fmaxf(top, pm[u]);
+      for (int u = 0; u < U; u++) top = fmaxf(top, pm[u]);
       const float keep = ex2(m - top);
       m = top, l *= keep, o.x *= keep, o.y *= keep, o.z *= keep, o.w *= keep;
 #pragma unroll
-      for (int u = 0; u < 8; u++) {
+      for (int u = 0; u < U; u++) {
         if (p0 + u >= parts) break;
         const float f = ex2(pm[u] - top);
         l = fmaf(f, pl[u], l);
@@ -700,7 +702,7 @@ __global__ void __launch_bounds__(WARPS * 32, (D == 64 && MT == 1) ? 4 : (MT * D
         if (col == 0) part[S::ROWS * D + row] = m, part[S::ROWS * D + S::ROWS + row] = l;
       }
     }
-    if (!whole && a.row_groups == 1) {  // the last block of this sequence and head joins
+    if (!whole && a.join_here) {  // the last block of this sequence and head joins
       const int64_t from = x - tile;
       const int64_t left = from / share, right = (from + s.tiles - 1) / share;
       __syncthreads();
@@ -725,8 +727,8 @@ __global__ void __launch_bounds__(WARPS * 32, (D == 64 && MT == 1) ? 4 : (MT * D
   }
 }
 
-// Joins what blocks left of a sequence and head that was cut, where there are several groups of rows. A block per query
-// row: a thread has four dimensions of every few parts.
+// Joins what blocks left of a sequence and head that was cut, where there are several groups of rows or may be many parts. A
+// block per query row: a thread has four dimensions of every few parts.
 constexpr int JOIN_THREADS = 256;
 
 template <int D, int MT>
@@ -801,6 +803,7 @@ int sm_count() {
 // Blocks of a launch, and bytes of its workspace.
 struct Plan {
   int mt, row_groups, blocks;
+  bool join_here;
   uint64_t plan_bytes, bytes;
 };
 template <int D>
@@ -814,6 +817,9 @@ Plan plan_of(const bn_kv8 *c, int64_t tokens, int64_t heads) {
   const int64_t most = c->batch * c->kv_heads * p.row_groups * ((c->max_seq + tile - 1) / tile + 1);
   const int64_t full = (int64_t)sm_count() * resident;
   p.blocks = (int)(most < full ? most : full);
+  // The block that finishes last reads a few parts faster than another kernel starts, many parts slower (us, 300 tokens,
+  // 6 parts at most: 12.4 / 14.4; 131073 tokens, 55 parts: 82 / 70).
+  p.join_here = p.row_groups == 1 && p.blocks <= 8 * c->batch * c->kv_heads;
   p.plan_bytes = ((uint64_t)(c->batch + 2) * 8 + 127) / 128 * 128;
   p.bytes = p.plan_bytes + (uint64_t)p.blocks * 2 * (16 * p.mt * (D + 2)) * 4;
   return p;
@@ -830,7 +836,7 @@ int attend_launch(const AttendArgs &a, cudaStream_t stream) {
   cfg.gridDim = dim3((unsigned)a.blocks), cfg.blockDim = dim3(WARPS * 32), cfg.dynamicSmemBytes = S::SMEM, cfg.stream = stream, cfg.attrs = attr, cfg.numAttrs = 1;
   BN_CUDA(allow_smem(attend_kernel<D, KIND, MT, PLAIN>, S::SMEM));
   BN_CUDA(cudaLaunchKernelEx(&cfg, attend_kernel<D, KIND, MT, PLAIN>, a));
-  if (a.row_groups == 1) return launched("attend_kernel");
+  if (a.join_here) return launched("attend_kernel");
   cfg.gridDim = dim3((unsigned)(a.c.batch * a.heads * a.tokens)), cfg.blockDim = dim3(JOIN_THREADS), cfg.dynamicSmemBytes = 0;
   BN_CUDA(cudaLaunchKernelEx(&cfg, join_kernel<D, MT>, a));
   return launched("attend_kernel");
@@ -895,7 +901,7 @@ extern "C" int bn_kv8_attend(const bn_kv8 *c, const uint16_t *q, int64_t q_seq, 
     if (const int e = bn_kv8_append(c, k, k_seq, k_token, k_head, v, v_seq, v_token, v_head, tokens, counts, stream)) return e;
     k = v = nullptr;
   }
-  bn::AttendArgs a{*c, q, out, q_seq, q_token, q_head, o_seq, o_token, o_head, counts, prefix, scores->slopes, k, v, k_seq, k_token, k_head, v_seq, v_token, v_head, (int)tokens, (int)heads, (int)(heads / c->kv_heads), (int)scores->window, scores->causal, zero_rest, scores->scale, scores->softcap, (int64_t *)workspace, (float *)((uint8_t *)workspace + p.plan_bytes), p.row_groups, p.blocks};
+  bn::AttendArgs a{*c, q, out, q_seq, q_token, q_head, o_seq, o_token, o_head, counts, prefix, scores->slopes, k, v, k_seq, k_token, k_head, v_seq, v_token, v_head, (int)tokens, (int)heads, (int)(heads / c->kv_heads), (int)scores->window, scores->causal, zero_rest, scores->scale, scores->softcap, (int64_t *)workspace, (float *)((uint8_t *)workspace + p.plan_bytes), p.row_groups, p.blocks, p.join_here};
   const cudaStream_t s = (cudaStream_t)stream;
   if (scores->softcap == 0.0f && !scores->slopes) return c->kind == BN_KV8_INT8 ? bn::attend_kind<BN_KV8_INT8, true>(a, p.mt, s) : bn::attend_kind<BN_KV8_E4M3, true>(a, p.mt, s);
   return c->kind == BN_KV8_INT8 ? bn::attend_kind<BN_KV8_INT8, false>(a, p.mt, s) : bn::attend_kind<BN_KV8_E4M3, false>(a, p.mt, s);

@@ -65,9 +65,10 @@ struct AttendArgs {
 template <int D, int MT>
 struct Shape {
   static constexpr int ROWS = 16 * MT;                 // query rows of a block
-  static constexpr int KS = D == 64 ? 32 : 16;         // keys of a warp's stage
+  static constexpr int P = MT * D <= 128 ? 2 : 1;      // pieces of 16 keys that a warp takes at once, where registers allow two: their chains of dependent instructions overlap
+  static constexpr int KS = 16 * P;                    // keys of a warp's stage
   static constexpr int TILE = KS * WARPS;              // keys of a block's step
-  static constexpr int STAGES = D == 256 ? 3 : 4;
+  static constexpr int STAGES = D == 256 ? 3 : P == 2 && D == 128 ? 2 : 4;
   static constexpr int STAGE_BYTES = 2 * KS * D;
   static constexpr int NT = D / 8;                     // n8 tiles of the output
   static constexpr int RING = WARPS * STAGES * STAGE_BYTES;
@@ -97,12 +98,12 @@ __device__ __forceinline__ Span span_of(const AttendArgs &a, int64_t b, int tile
 }
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ void mma_bf16x(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
@@ -170,55 +171,70 @@ struct Rows {
   int L, prefix;
 };
 
-// The scores of a 16-key piece into weights: x holds the raw sums and gets p' (tile j, column 2c + e: key key0 + 4c
-// + 2j + e). scale, vlog, vinv: K's scale, V's as a power of two and inverted. Updates the weights' sum; where a score passes
-// a row's m by the headroom, moves m and rescales the sums.
-template <int D, int MT, bool PLAIN>
-__device__ __forceinline__ void weigh(const AttendArgs &a, float (&x)[MT][2][4], const Rows<MT> &r, State<D, MT> &st, int key0, float scale, float vlog, float vinv, bool masked) {
-  const int first = key0 + 4 * (int)(lane_id() & 3u);
+// What goes with a 16-key piece: its first key, the first key that is not its stage's, K's scale, V's as a power of two and
+// inverted, whether some row does not see all of it.
+struct PieceOf16 {
+  int key0, end;
+  float scale, vlog, vinv;
+  bool masked;
+};
+
+// The scores of P pieces into weights: x holds the raw sums and gets p' (tile j, column 2c + e: key key0 + 4c + 2j + e).
+// Updates the weights' sum; where a score passes a row's m by the headroom, moves m and rescales the sums.
+template <int D, int MT, int P, bool PLAIN>
+__device__ __forceinline__ void weigh(const AttendArgs &a, float (&x)[P][MT][2][4], const Rows<MT> &r, State<D, MT> &st, const PieceOf16 (&pc)[P]) {
+  const int lane_key = 4 * (int)(lane_id() & 3u);
+  float top[MT][2];
 #pragma unroll
-  for (int mt = 0; mt < MT; mt++)
-#pragma unroll
-    for (int h = 0; h < 2; h++) {
-      const float f = fminf(scale * r.factor[mt][h], 3.0e38f);
-#pragma unroll
-      for (int j = 0; j < 2; j++)
-#pragma unroll
-        for (int e = 0; e < 2; e++) {
-          float &v = x[mt][j][2 * h + e];
-          if constexpr (PLAIN) {
-            v = fmaf(v, f, vlog);
-          } else {
-            v *= f;
-            if (a.cap > 0.0f) v = capped(v, a.cap * LOG2E);
-            v = fmaf(-r.slope[mt][h], (float)abs(r.i[mt][h] - (first + 2 * j + e)), v) + vlog;
-          }
-        }
-    }
-  if (masked) {
+  for (int p = 0; p < P; p++) {
+    const int first = pc[p].key0 + lane_key;
 #pragma unroll
     for (int mt = 0; mt < MT; mt++)
 #pragma unroll
       for (int h = 0; h < 2; h++) {
-        int lo = 0, hi = 0;
-        if (r.i[mt][h] >= 0) visible_keys(r.i[mt][h], r.L, r.prefix, a.window, a.causal, lo, hi);
+        const float f = fminf(pc[p].scale * r.factor[mt][h], 3.0e38f);
 #pragma unroll
         for (int j = 0; j < 2; j++)
 #pragma unroll
           for (int e = 0; e < 2; e++) {
-            const int key = first + 2 * j + e;
-            if (key < lo || key >= hi) x[mt][j][2 * h + e] = -CUDART_INF_F;
+            float &v = x[p][mt][j][2 * h + e];
+            if constexpr (PLAIN) {
+              v = fmaf(v, f, pc[p].vlog);
+            } else {
+              v *= f;
+              if (a.cap > 0.0f) v = capped(v, a.cap * LOG2E);
+              v = fmaf(-r.slope[mt][h], (float)abs(r.i[mt][h] - (first + 2 * j + e)), v) + pc[p].vlog;
+            }
           }
       }
+    if (pc[p].masked) {
+#pragma unroll
+      for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+          int lo = 0, hi = 0;
+          if (r.i[mt][h] >= 0) visible_keys(r.i[mt][h], r.L, r.prefix, a.window, a.causal, lo, hi);
+          hi = min(hi, pc[p].end);
+#pragma unroll
+          for (int j = 0; j < 2; j++)
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+              const int key = first + 2 * j + e;
+              if (key < lo || key >= hi) x[p][mt][j][2 * h + e] = -CUDART_INF_F;
+            }
+        }
+    }
   }
-  float top[MT][2];
   bool over = false;
 #pragma unroll
   for (int mt = 0; mt < MT; mt++)
 #pragma unroll
     for (int h = 0; h < 2; h++) {
-      top[mt][h] = fmaxf(fmaxf(x[mt][0][2 * h], x[mt][0][2 * h + 1]), fmaxf(x[mt][1][2 * h], x[mt][1][2 * h + 1]));
-      over |= top[mt][h] > st.m[mt][h] + HEADROOM;
+      float t = -CUDART_INF_F;
+#pragma unroll
+      for (int p = 0; p < P; p++) t = fmaxf(t, fmaxf(fmaxf(x[p][mt][0][2 * h], x[p][mt][0][2 * h + 1]), fmaxf(x[p][mt][1][2 * h], x[p][mt][1][2 * h + 1])));
+      top[mt][h] = t;
+      over |= t > st.m[mt][h] + HEADROOM;
     }
   if (__any_sync(BN_FULL, over)) {
 #pragma unroll
@@ -236,20 +252,22 @@ __device__ __forceinline__ void weigh(const AttendArgs &a, float (&x)[MT][2][4],
       }
   }
 #pragma unroll
-  for (int mt = 0; mt < MT; mt++)
+  for (int p = 0; p < P; p++)
 #pragma unroll
-    for (int h = 0; h < 2; h++) {
-      float sum = 0.0f;
+    for (int mt = 0; mt < MT; mt++)
 #pragma unroll
-      for (int j = 0; j < 2; j++)
+      for (int h = 0; h < 2; h++) {
+        float sum = 0.0f;
 #pragma unroll
-        for (int e = 0; e < 2; e++) {
-          float &v = x[mt][j][2 * h + e];
-          v = ex2(v - st.m[mt][h]);
-          sum += v;
-        }
-      st.l[mt][h] = fmaf(sum, vinv, st.l[mt][h]);
-    }
+        for (int j = 0; j < 2; j++)
+#pragma unroll
+          for (int e = 0; e < 2; e++) {
+            float &v = x[p][mt][j][2 * h + e];
+            v = ex2(v - st.m[mt][h]);
+            sum += v;
+          }
+        st.l[mt][h] = fmaf(sum, pc[p].vinv, st.l[mt][h]);
+      }
 }
 
 // The dimension of n8 tile t's column n.
@@ -289,7 +307,8 @@ __device__ __noinline__ void append_filled(const AttendArgs &a, int64_t b, int h
 template <int D, int MT, bool PLAIN>
 __device__ void open_block(const AttendArgs &a, const uint16_t *const (&qrow)[MT][2], const OpenRows &rows, int L, int key0, const Rows<MT> &r, State<D, MT> &st) {
   const uint32_t lane = lane_id(), n = lane >> 2, c = lane & 3u;
-  float x[MT][2][4] = {};
+  float x1[1][MT][2][4] = {};
+  auto &x = x1[0];
   const uint16_t *k[2];
 #pragma unroll
   for (int j = 0; j < 2; j++) k[j] = rows.key(min(key0 + 4 * (int)(n >> 1) + 2 * j + (int)(n & 1), L - 1)) + 16 * c;
@@ -312,7 +331,8 @@ __device__ void open_block(const AttendArgs &a, const uint16_t *const (&qrow)[MT
   Rows<MT> plain = r;  // the queries as they are: no power of two in the factor
 #pragma unroll
   for (int mt = 0; mt < MT; mt++) plain.factor[mt][0] = plain.factor[mt][1] = a.cap > 0.0f ? a.scale * (2.0f * LOG2E / a.cap) : a.scale * LOG2E;
-  weigh<D, MT, PLAIN>(a, x, plain, st, key0, 1.0f, 23.0f, 1.0f / (1 << 23), true);
+  const PieceOf16 piece[1] = {{key0, L, 1.0f, 23.0f, 1.0f / (1 << 23), true}};
+  weigh<D, MT, 1, PLAIN>(a, x1, plain, st, piece);
   uint32_t hi[MT][4], lo[MT][4];
 #pragma unroll
   for (int mt = 0; mt < MT; mt++)
@@ -506,7 +526,11 @@ __global__ void __launch_bounds__(WARPS * 32, (D == 64 && MT == 1) ? 4 : (MT * D
         const uint32_t to = ring + slot * S::STAGE_BYTES;
 #pragma unroll
         for (int sub = 0; sub < S::KS / 16; sub++) {
-          if (key0 + 16 * sub >= end) break;
+          if (key0 + 16 * sub >= end) {  // nothing there: zeros that the masks keep out
+            for (int i = 0; sub && i < 2 * (D / 32); i++) asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(to + (i & 1) * (S::KS * D) + sub * (16 * D) + (lane + 32 * (i >> 1)) * 16), "r"(0) : "memory");
+            if (lane < 2) scales[warp][slot][lane][sub] = 1.0f;
+            continue;
+          }
 #pragma unroll
           for (int side = 0; side < 2; side++) {
             const uint8_t *const from = codes[side] + (int64_t)(key0 + 16 * sub) * D + lane * 16;
@@ -594,55 +618,58 @@ __global__ void __launch_bounds__(WARPS * 32, (D == 64 && MT == 1) ? 4 : (MT * D
       __syncwarp();  // this tile's copies of all lanes are there, and the slot of the tile before is read
       issue(t + S::STAGES - 1, slot == 0 ? S::STAGES - 1 : slot - 1);
       const uint32_t at = ring + slot * S::STAGE_BYTES;
-#pragma unroll
-      for (int sub = 0; sub < S::KS / 16; sub++) {
-        const int key0 = key_of(t) + 16 * sub;
-        if (key0 >= (t < s.quant ? s.split : s.full)) break;
-        const float kscale = scales[warp][slot][0][sub], vscale = scales[warp][slot][1][sub];
-        float x[MT][2][4] = {};
-        float x2[MT][2][4] = {};  // every other product, for shorter chains
+      const int first = key_of(t), end = t < s.quant ? s.split : s.full;
+      if (first < end) {
+        constexpr int P = S::P;
+        float x[P][MT][2][4] = {};
+        PieceOf16 piece[P];
 #pragma unroll
         for (int g = 0; g < D / 64; g++)
 #pragma unroll
-          for (int j = 0; j < 2; j++) {
-            const uint32_t key = 16 * sub + 4 * (n >> 1) + 2 * j + (n & 1);
-            const uint4 w4 = lds16(at + key * D + k_piece<D>(key, 4 * g + c) * 16);
-            const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
+          for (int sub = 0; sub < P; sub++)
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-              const uint32_t b0 = codes_f16<KIND, false>(w[e]), b1 = codes_f16<KIND, true>(w[e]);
+            for (int j = 0; j < 2; j++) {
+              const uint32_t key = 16 * sub + 4 * (n >> 1) + 2 * j + (n & 1);
+              const uint4 w4 = lds16(at + key * D + k_piece<D>(key, 4 * g + c) * 16);
+              const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
 #pragma unroll
-              for (int mt = 0; mt < MT; mt++) mma_f16(MT == 1 && (e & 1) ? x2[mt][j] : x[mt][j], q[mt][4 * g + e], b0, b1);
+              for (int e = 0; e < 4; e++) {
+                const uint32_t b0 = codes_f16<KIND, false>(w[e]), b1 = codes_f16<KIND, true>(w[e]);
+#pragma unroll
+                for (int mt = 0; mt < MT; mt++) mma_f16(x[sub][mt][j], q[mt][4 * g + e], b0, b1);
+              }
             }
-          }
-        if constexpr (MT == 1) {
 #pragma unroll
-          for (int j = 0; j < 2; j++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) x[0][j][e] += x2[0][j][e];
+        for (int sub = 0; sub < P; sub++) {
+          const float vscale = scales[warp][slot][1][sub];
+          float vlog;
+          asm("lg2.approx.f32 %0, %1;" : "=f"(vlog) : "f"(vscale));
+          const int key0 = first + 16 * sub;
+          piece[sub] = {key0, end, scales[warp][slot][0][sub], vlog, __fdividef(1.0f, vscale), key0 < lo_most || key0 + 16 > min(hi_least, end)};
         }
-        float vlog;
-        asm("lg2.approx.f32 %0, %1;" : "=f"(vlog) : "f"(vscale));
-        weigh<D, MT, PLAIN>(a, x, r, st, key0, kscale, vlog, __fdividef(1.0f, vscale), key0 < lo_most || key0 + 16 > hi_least);
-        uint32_t p[MT][4];
+        weigh<D, MT, P, PLAIN>(a, x, r, st, piece);
 #pragma unroll
-        for (int mt = 0; mt < MT; mt++)
+        for (int sub = 0; sub < P; sub++) {
+          uint32_t p[MT][4];
 #pragma unroll
-          for (int f = 0; f < 4; f++) p[mt][f] = pack_f16(x[mt][f >> 1][2 * (f & 1)], x[mt][f >> 1][2 * (f & 1) + 1]);
-        const uint32_t vat = at + S::KS * D + (4 * sub + c) * (4 * D);
+          for (int mt = 0; mt < MT; mt++)
 #pragma unroll
-        for (int half = 0; half < (D + 127) / 128; half++)
+            for (int f = 0; f < 4; f++) p[mt][f] = pack_f16(x[sub][mt][f >> 1][2 * (f & 1)], x[sub][mt][f >> 1][2 * (f & 1) + 1]);
+          const uint32_t vat = at + S::KS * D + (4 * sub + c) * (4 * D);
 #pragma unroll
-          for (int i = 0; i < (D == 64 ? 2 : 4); i++) {
-            const uint4 w4 = lds16(vat + v_piece<D>(c, 32 * half + (D == 64 ? 2 : 4) * n + i) * 16);
-            const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
+          for (int half = 0; half < (D + 127) / 128; half++)
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-              const uint32_t b0 = codes_f16<KIND, false>(w[e]), b1 = codes_f16<KIND, true>(w[e]);
+            for (int i = 0; i < (D == 64 ? 2 : 4); i++) {
+              const uint4 w4 = lds16(vat + v_piece<D>(c, 32 * half + (D == 64 ? 2 : 4) * n + i) * 16);
+              const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
 #pragma unroll
-              for (int mt = 0; mt < MT; mt++) mma_f16(st.o[mt][16 * half + 4 * i + e], p[mt], b0, b1);
+              for (int e = 0; e < 4; e++) {
+                const uint32_t b0 = codes_f16<KIND, false>(w[e]), b1 = codes_f16<KIND, true>(w[e]);
+#pragma unroll
+                for (int mt = 0; mt < MT; mt++) mma_f16(st.o[mt][16 * half + 4 * i + e], p[mt], b0, b1);
+              }
             }
-          }
+        }
       }
       slot = slot + 1 == S::STAGES ? 0 : slot + 1;
     }

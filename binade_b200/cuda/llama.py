@@ -11,6 +11,10 @@ local, and four all-gathers per layer (attention output, o_proj, SwiGLU output, 
 one for the logits rebuild the full vectors, in row order, so outputs do not depend on the GPU
 count. The all-gathers are this library's peer-store kernel (dist.PushGather), or NCCL with
 BINADE_B200_GATHER=nccl.
+
+With cache="int8" or "e4m3" keys and values are held in 8 bits (attention.KV8Cache), a step's attention
+and its append are one launch, and a prompt goes through the layers in one pass (`prefill`); `generate` can
+put penalties, a bias and a grammar's mask on the logits (logits.process_logits).
 """
 
 from __future__ import annotations
@@ -22,6 +26,8 @@ import torch
 from torch import nn
 
 from . import r4
+from .attention import KV8Cache, attention
+from .logits import TokenCounts, process_logits
 from .dist import RowShardedLinear, make_exchange, row_range
 
 
@@ -56,9 +62,10 @@ def synthetic_weight(rows: int, cols: int, seed: int, device) -> torch.Tensor:
 
 
 class Decoder(nn.Module):
-    def __init__(self, shape: LlamaShape, kind: str = "r4", rank: int = 0, world: int = 1, group=None, device="cuda", seed: int = 0):
+    def __init__(self, shape: LlamaShape, kind: str = "r4", rank: int = 0, world: int = 1, group=None, device="cuda", seed: int = 0, cache: str = "bf16"):
         """kind: "r4" (R4Linear over from_dense) or "bf16" (DenseLinear). Weights are N(0, 0.02)
-        from fixed seeds, generated whole on every rank and cut to the rank's rows."""
+        from fixed seeds, generated whole on every rank and cut to the rank's rows. cache: "bf16", or "int8" or
+        "e4m3" for keys and values in 8 bits."""
         super().__init__()
         s = self.shape = shape
         if s.heads % world or s.kv_heads % world or s.ffn % world or s.hidden % world or s.vocab % world:
@@ -106,8 +113,12 @@ class Decoder(nn.Module):
             self.norm2.append(torch.ones(s.hidden, dtype=torch.bfloat16, device=dev))
         self.norm_f = torch.ones(s.hidden, dtype=torch.bfloat16, device=dev)
         self.lm_head = lin(rows_of(synthetic_weight(s.vocab, s.hidden, seed + 2, dev), s.vocab), s.vocab)
-        self.k_cache = torch.zeros((s.layers, self.hkv, s.max_seq, d), dtype=torch.bfloat16, device=dev)
-        self.v_cache = torch.zeros_like(self.k_cache)
+        if cache == "bf16":
+            self.cache = None
+            self.k_cache = torch.zeros((s.layers, self.hkv, s.max_seq, d), dtype=torch.bfloat16, device=dev)
+            self.v_cache = torch.zeros_like(self.k_cache)
+        else:
+            self.cache = KV8Cache(s.layers, 1, self.hkv, d, s.max_seq, kind=cache, device=device)
         inv = 1.0 / (s.rope_theta ** (torch.arange(0, d, 2, device=dev, dtype=torch.float32) / d))
         ang = torch.arange(s.max_seq, device=dev, dtype=torch.float32)[:, None] * inv[None, :]
         self.cos, self.sin = torch.cos(ang), torch.sin(ang)  # [max_seq, d/2]
@@ -116,7 +127,7 @@ class Decoder(nn.Module):
     def _sources(self):
         """(module, source weight) for every linear of this rank, weights regenerated one at a
         time from the construction seeds."""
-        s, d, dev = self.shape, self.shape.head_dim, self.k_cache.device
+        s, d, dev = self.shape, self.shape.head_dim, self.cos.device
         rows_of = lambda w, count: w[slice(*row_range(count, self.rank, self.world))]
         local = lambda m: m.local if isinstance(m, RowShardedLinear) else m
         for l in range(s.layers):
@@ -151,12 +162,20 @@ class Decoder(nn.Module):
             checked += 1
             hooks.append(m.register_forward_hook(compare))
             del w
-        dev = self.k_cache.device
+        dev = self.cos.device
+        self.reset()
         self.step(torch.zeros(1, dtype=torch.int64, device=dev), torch.zeros(1, dtype=torch.int64, device=dev))
         for h in hooks:
             h.remove()
-        self.k_cache.zero_(), self.v_cache.zero_()
+        self.reset()
         return {"linears_decoding_to_their_source": checked, "max_ulp_vs_fp32_product_step0": worst}
+
+    def reset(self) -> None:
+        """Forgets every token."""
+        if self.cache is not None:
+            self.cache.length.zero_()
+        else:
+            self.k_cache.zero_(), self.v_cache.zero_()
 
     def linear_bytes(self) -> int:
         """Weight bytes one decode step streams on this rank (R4 arrays or BF16 words)."""
@@ -181,19 +200,21 @@ class Decoder(nn.Module):
 
     @staticmethod
     def _rope(t: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor) -> torch.Tensor:
-        """t [heads, d] rotated by the position's cos / sin [1, d/2] (fp32 arithmetic)."""
+        """t [.., heads, d] rotated by its position's cos / sin [.., 1, d/2] (fp32 arithmetic)."""
         tf = t.float()
-        a, b = tf[:, : t.shape[1] // 2], tf[:, t.shape[1] // 2 :]
-        return torch.cat([a * cos - b * sin, a * sin + b * cos], dim=1).to(t.dtype)
+        a, b = tf[..., : t.shape[-1] // 2], tf[..., t.shape[-1] // 2 :]
+        return torch.cat([a * cos - b * sin, a * sin + b * cos], dim=-1).to(t.dtype)
 
     def step(self, token: torch.Tensor, pos: torch.Tensor) -> torch.Tensor:
         """One decode step: token, pos are device int64 tensors of one element -> logits [1, vocab].
         The glue between the linear layers is kept to few kernels (it is launch-bound at batch 1):
         the position's rotation is looked up once per step, q and k rotate together, attention is
-        one fused scaled-dot-product call over the static cache with a position mask."""
+        one fused scaled-dot-product call over the static cache with a position mask. Over a cache in 8
+        bits it is one call that appends too; the cache holds a token more afterwards, and `pos` has to be
+        what it held before."""
         s, d = self.shape, self.shape.head_dim
         x = self.embed(token) if isinstance(self.embed, r4.R4Embedding) else self.embed.index_select(0, token)  # [1, hidden]
-        mask = (self.positions <= pos)[None, None, None, :]  # [1, 1, 1, max_seq]
+        mask = (self.positions <= pos)[None, None, None, :] if self.cache is None else None  # [1, 1, 1, max_seq]
         cos, sin = self.cos.index_select(0, pos), self.sin.index_select(0, pos)  # [1, d/2]
         nqk = self.hq + self.hkv
         for l in range(s.layers):
@@ -201,31 +222,79 @@ class Decoder(nn.Module):
             qkv = self.qkv[l](h)[0]
             qk = self._rope(qkv[: nqk * d].view(nqk, d), cos, sin)
             v = qkv[nqk * d :].view(self.hkv, d)
-            self.k_cache[l].index_copy_(1, pos, qk[self.hq :, None, :])
-            self.v_cache[l].index_copy_(1, pos, v[:, None, :])
-            attn = torch.nn.functional.scaled_dot_product_attention(qk[None, : self.hq, None, :], self.k_cache[l][None], self.v_cache[l][None], attn_mask=mask, enable_gqa=True)  # [1, hq, 1, d]
+            if self.cache is not None:
+                attn = self.cache.attend(l, qk[None, None, : self.hq], qk[None, None, self.hq :], v[None, None])
+            else:
+                self.k_cache[l].index_copy_(1, pos, qk[self.hq :, None, :])
+                self.v_cache[l].index_copy_(1, pos, v[:, None, :])
+                attn = torch.nn.functional.scaled_dot_product_attention(qk[None, : self.hq, None, :], self.k_cache[l][None], self.v_cache[l][None], attn_mask=mask, enable_gqa=True)  # [1, hq, 1, d]
             x = x + self.o[l](self._gather(attn.reshape(1, self.hq * d), s.heads * d))
             h = torch.nn.functional.rms_norm(x, (s.hidden,), self.norm2[l], s.eps)
             gu = self.gate_up[l](h)[0]
             half = gu.shape[0] // 2
             act = (torch.nn.functional.silu(gu[:half].float()) * gu[half:].float()).to(torch.bfloat16)
             x = x + self.down[l](self._gather(act[None, :], s.ffn))
+        if self.cache is not None:
+            self.cache.advance(1)
         return self.lm_head(torch.nn.functional.rms_norm(x, (s.hidden,), self.norm_f, s.eps))
 
     @torch.no_grad()
-    def generate(self, prompt: torch.Tensor, n_new: int, use_graph: bool = True):
+    def prefill(self, tokens: torch.Tensor, more: bool = False) -> torch.Tensor:
+        """A prompt, int64 [P] on the device, through the layers in one pass -> logits [1, vocab] behind its last token; its
+        keys and values go to the cache (in 8 bits; one GPU). Without `more` the cache is emptied first and the prompt's tokens
+        see one another's keys as they are; with it the prompt goes behind what the cache holds, and sees what the
+        cache holds then."""
+        if self.cache is None or self.world > 1:
+            raise ValueError("prefill needs a cache in 8 bits and one GPU")
+        s, d, P = self.shape, self.shape.head_dim, tokens.numel()
+        if not 1 <= P <= s.max_seq:
+            raise ValueError(f"a prompt of {P} tokens, max_seq {s.max_seq}")
+        if not more:
+            self.reset()
+        x = self.embed(tokens) if isinstance(self.embed, r4.R4Embedding) else self.embed.index_select(0, tokens)  # [P, hidden]
+        at = torch.clamp(self.positions[:P] + self.cache.length.to(torch.int64) if more else self.positions[:P], max=s.max_seq - 1)
+        cos, sin = self.cos.index_select(0, at)[:, None, :], self.sin.index_select(0, at)[:, None, :]  # [P, 1, d/2]
+        nqk = self.hq + self.hkv
+        for l in range(s.layers):
+            h = torch.nn.functional.rms_norm(x, (s.hidden,), self.norm1[l], s.eps)
+            qkv = self.qkv[l](h)
+            qk = self._rope(qkv[:, : nqk * d].view(P, nqk, d), cos, sin)
+            q, k, v = qk[:, : self.hq], qk[:, self.hq :], qkv[:, nqk * d :].view(P, self.hkv, d)
+            if more:
+                attn = self.cache.attend(l, q[None], k[None], v[None])
+            else:
+                attn = attention(q, k, v)
+                self.cache.append(l, k[None], v[None])
+            x = x + self.o[l](attn.reshape(P, self.hq * d))
+            h = torch.nn.functional.rms_norm(x, (s.hidden,), self.norm2[l], s.eps)
+            gu = self.gate_up[l](h)
+            half = gu.shape[1] // 2
+            x = x + self.down[l]((torch.nn.functional.silu(gu[:, :half].float()) * gu[:, half:].float()).to(torch.bfloat16))
+        self.cache.advance(P)
+        return self.lm_head(torch.nn.functional.rms_norm(x[-1:], (s.hidden,), self.norm_f, s.eps))
+
+    @torch.no_grad()
+    def generate(self, prompt: torch.Tensor, n_new: int, use_graph: bool = True, rules: dict | None = None):
         """Greedy decoding. prompt: int64 [P] on the device. Returns (tokens int64 [n_new],
-        seconds spent on the n_new generated tokens, measured with CUDA events)."""
+        seconds spent on the n_new generated tokens, measured with CUDA events). rules: keyword arguments of
+        logits.process_logits (repetition, presence, frequency, bias, mask); a token of -1: nothing was allowed."""
         P = prompt.numel()
         if P + n_new > self.shape.max_seq:
             raise ValueError("prompt + new tokens exceed max_seq")
         token, pos = prompt[:1].clone(), torch.zeros(1, dtype=torch.int64, device=prompt.device)
         out = torch.zeros(n_new, dtype=torch.int64, device=prompt.device)
         nxt = torch.zeros(1, dtype=torch.int64, device=prompt.device)
+        said = TokenCounts(1, self.shape.vocab, prompt.device) if rules is not None else None
+
+        def choose(logits):
+            if said is None:
+                nxt.copy_(torch.argmax(logits[0].float(), dim=-1, keepdim=True))  # ties: lowest index
+            else:
+                nxt.copy_(process_logits(logits, said, **rules)[1])
+                said.add(nxt)
 
         def one():
-            logits = self.step(token, pos)
-            nxt.copy_(torch.argmax(logits[0].float(), dim=-1, keepdim=True))  # ties: lowest index
+            choose(self.step(token, pos))
             pos.add_(1)
 
         graph = None
@@ -241,14 +310,26 @@ class Decoder(nn.Module):
                     one()
             torch.cuda.synchronize()
             pos.zero_()
+        if self.cache is not None:
+            self.reset()
+        if said is not None:
+            said.clear()
+            said.add(prompt[None], prompt=True)
         run = graph.replay if graph else one
-        for i in range(P):  # the prompt, one token at a time through the same step
-            token.copy_(prompt[i : i + 1])
-            run()
+        if self.cache is not None and self.world == 1:
+            choose(self.prefill(prompt))
+            pos.fill_(P)
+        else:
+            for i in range(P):  # the prompt, one token at a time through the same step
+                token.copy_(prompt[i : i + 1])
+                run()
+                if said is not None and i + 1 < P:  # only what follows the whole prompt is part of the answer
+                    said.clear()
+                    said.add(prompt[None], prompt=True)
         e0, e1 = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
         e0.record()
         for i in range(n_new):
-            token.copy_(nxt)
+            token.copy_(nxt if said is None else nxt.clamp(min=0))
             out[i : i + 1].copy_(nxt)
             run()
         e1.record()

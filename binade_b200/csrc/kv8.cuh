@@ -61,6 +61,21 @@ __device__ __forceinline__ float finite_size(float x) {
   return s <= 3.4028235e38f ? s : 0.0f;
 }
 
+// Four finite values of a block (two words of BF16 pairs) as codes: the quotient is rounded by adding 1.5 x 2^23, whose last
+// byte is then code + 128; `close` is set where a quotient lies next to the middle of two codes (int8_code decides there).
+__device__ __forceinline__ uint32_t int8_codes(uint32_t lo, uint32_t hi, float inv, bool &close) {
+  constexpr float MAGIC = 12582912.0f + 128.0f;
+  const float x[4] = {__uint_as_float(lo << 16), __uint_as_float(lo & 0xFFFF0000u), __uint_as_float(hi << 16), __uint_as_float(hi & 0xFFFF0000u)};
+  uint32_t r[4];
+#pragma unroll
+  for (int e = 0; e < 4; e++) {
+    const float t = x[e] * inv, sum = t + MAGIC, off = t - (sum - MAGIC);
+    close |= fabsf(off) > 0.4995f;
+    r[e] = __float_as_uint(sum);
+  }
+  return __byte_perm(__byte_perm(r[0], r[1], 0x0040), __byte_perm(r[2], r[3], 0x0040), 0x5410);
+}
+
 // Block j of one sequence and head, keys or values, by 128 threads: a full block is scaled, coded and stored; the
 // tokens of the blocks that were open (the one at `held`) or stay open go to the tail in BF16. in: the new tokens'
 // rows, `step` elements apart. CHUNKS: pieces of eight values that a thread has: neighbours of one token, or for values
@@ -68,13 +83,13 @@ __device__ __forceinline__ float finite_size(float x) {
 // codes.
 template <int CHUNKS>
 __device__ __forceinline__ void append_block(const bn_kv8 &c, bool values, int64_t b, int h, int j, int held, int end, const uint16_t *__restrict__ in, int64_t step) {
-  __shared__ float part_max[4];
+  __shared__ uint32_t part_max[4];
   const int block = c.block, D = (int)c.D;
   const int64_t unit = b * c.kv_heads + h;
   const bool full = (j + 1) * (int64_t)block <= end, open = j == held / block || !full;  // the first block goes to its slot, full or not
   uint16_t *const tail = (values ? c.v_tail : c.k_tail) + (unit * 2 + (open ? kv8_slot(c, b, held, j) : 0)) * block * D;
   uint4 x[CHUNKS];
-  float amax = 0.0f;
+  uint32_t most = 0;  // largest magnitudes, as pairs of 16 bits
 #pragma unroll
   for (int i = 0; i < CHUNKS; i++) {
     const int chunk = (int)threadIdx.x + 128 * i;
@@ -95,17 +110,32 @@ __device__ __forceinline__ void append_block(const bn_kv8 &c, bool values, int64
       if (p < end && (full || p >= held)) x[i] = *reinterpret_cast<const uint4 *>(p < held ? tail + row * D + col : in + (int64_t)(p - held) * step + col);
       if (open && p >= held && p < end) *reinterpret_cast<uint4 *>(tail + row * D + col) = x[i];
     }
-    const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
-#pragma unroll
-    for (int e = 0; e < 4; e++) amax = fmaxf(amax, fmaxf(finite_size(__uint_as_float(w[e] << 16)), finite_size(__uint_as_float(w[e] & 0xFFFF0000u))));
+    most = __vmaxu2(__vmaxu2(most, x[i].x & 0x7FFF7FFFu), __vmaxu2(x[i].y & 0x7FFF7FFFu, __vmaxu2(x[i].z & 0x7FFF7FFFu, x[i].w & 0x7FFF7FFFu)));
   }
   if (!full) return;
 #pragma unroll
-  for (int d = 16; d; d >>= 1) amax = fmaxf(amax, __shfl_xor_sync(BN_FULL, amax, d));
+  for (int d = 16; d; d >>= 1) most = __vmaxu2(most, __shfl_xor_sync(BN_FULL, most, d));
   __syncthreads();  // (another block's maxima may still be read)
-  if (lane_id() == 0) part_max[threadIdx.x >> 5] = amax;
+  if (lane_id() == 0) part_max[threadIdx.x >> 5] = most;
   __syncthreads();
-  amax = fmaxf(fmaxf(part_max[0], part_max[1]), fmaxf(part_max[2], part_max[3]));
+  most = __vmaxu2(__vmaxu2(part_max[0], part_max[1]), __vmaxu2(part_max[2], part_max[3]));
+  float amax = __uint_as_float(max(most & 0xFFFFu, most >> 16) << 16);
+  const bool odd = !(amax <= 3.4e38f);  // a value that is not finite: the largest of the others then
+  if (odd) {
+    amax = 0.0f;
+#pragma unroll
+    for (int i = 0; i < CHUNKS; i++) {
+      const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+#pragma unroll
+      for (int e = 0; e < 4; e++) amax = fmaxf(amax, fmaxf(finite_size(__uint_as_float(w[e] << 16)), finite_size(__uint_as_float(w[e] & 0xFFFF0000u))));
+    }
+#pragma unroll
+    for (int d = 16; d; d >>= 1) amax = fmaxf(amax, __shfl_xor_sync(BN_FULL, amax, d));
+    __syncthreads();
+    if (lane_id() == 0) part_max[threadIdx.x >> 5] = __float_as_uint(amax);
+    __syncthreads();
+    amax = __uint_as_float(max(max(part_max[0], part_max[1]), max(part_max[2], part_max[3])));
+  }
   const float scale = c.kind == KV8_INT8 ? fmaxf(__fdiv_rn(amax, 127.0f), 7.888609052210118e-31f) : e4m3_scale(amax);
   const float inv = __frcp_rn(scale);  // (of a power of two: exact)
   uint8_t *const codes = (values ? c.v : c.k) + (unit * c.rows + (int64_t)j * block) * D;
@@ -114,15 +144,19 @@ __device__ __forceinline__ void append_block(const bn_kv8 &c, bool values, int64
   for (int i = 0; i < CHUNKS; i++) {
     const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
     uint32_t out[2];
+    bool slow = odd;
+    if (c.kind == KV8_INT8 && !odd) out[0] = int8_codes(w[0], w[1], inv, slow), out[1] = int8_codes(w[2], w[3], inv, slow);
+    if (c.kind != KV8_INT8 || slow) {
 #pragma unroll
-    for (int e = 0; e < 2; e++) {
-      float f[4] = {__uint_as_float(w[2 * e] << 16), __uint_as_float(w[2 * e] & 0xFFFF0000u), __uint_as_float(w[2 * e + 1] << 16), __uint_as_float(w[2 * e + 1] & 0xFFFF0000u)};
-      if (c.kind == KV8_INT8) {
-        out[e] = int8_code(f[0], scale, inv) | int8_code(f[1], scale, inv) << 8 | int8_code(f[2], scale, inv) << 16 | int8_code(f[3], scale, inv) << 24;
-      } else {
+      for (int e = 0; e < 2; e++) {
+        float f[4] = {__uint_as_float(w[2 * e] << 16), __uint_as_float(w[2 * e] & 0xFFFF0000u), __uint_as_float(w[2 * e + 1] << 16), __uint_as_float(w[2 * e + 1] & 0xFFFF0000u)};
+        if (c.kind == KV8_INT8) {
+          out[e] = int8_code(f[0], scale, inv) | int8_code(f[1], scale, inv) << 8 | int8_code(f[2], scale, inv) << 16 | int8_code(f[3], scale, inv) << 24;
+        } else {
 #pragma unroll
-        for (int n = 0; n < 4; n++) f[n] = f[n] == f[n] ? f[n] * inv : 0.0f;
-        out[e] = (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(f[0], f[1]), __NV_SATFINITE, __NV_E4M3) | (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(f[2], f[3]), __NV_SATFINITE, __NV_E4M3) << 16;
+          for (int n = 0; n < 4; n++) f[n] = f[n] == f[n] ? f[n] * inv : 0.0f;
+          out[e] = (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(f[0], f[1]), __NV_SATFINITE, __NV_E4M3) | (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(f[2], f[3]), __NV_SATFINITE, __NV_E4M3) << 16;
+        }
       }
     }
     *reinterpret_cast<uint2 *>(codes + ((int64_t)threadIdx.x + 128 * i) * 8) = make_uint2(out[0], out[1]);

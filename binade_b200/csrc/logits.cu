@@ -51,7 +51,7 @@ __device__ __forceinline__ uint32_t four_bits(const uint32_t *__restrict__ words
 // has 16-byte boundaries (rows of an odd vocabulary start anywhere); the input is read in one piece
 // where its row has them at the same places. Counts are read only where a token was said.
 template <typename T, int THREADS, int U>
-__global__ void __launch_bounds__(THREADS) logits_kernel(const __grid_constant__ LogitsArgs a) {
+__global__ void __launch_bounds__(THREADS, U == 1 ? 4 : 2) logits_kernel(const __grid_constant__ LogitsArgs a) {
   namespace cg = cooperative_groups;
   cg::cluster_group cluster = cg::this_cluster();
   const int64_t b = blockIdx.y;
@@ -175,10 +175,11 @@ extern "C" int bn_logits(const void *x, int fp32, int64_t x_row, int64_t batch, 
   if (batch < 0 || batch > 65535 || V < 1 || V > 0x3FFFFFFF) return bn::fail(BN_ERR_ARG, "bn_logits: bad size");
   if (!rules || (batch && (!x || !out || !token)) || (rules && rules->seen && !rules->counts)) return bn::fail(BN_ERR_ARG, "bn_logits: null pointer");
   if (batch == 0) return BN_OK;
-  constexpr int threads = 512, quads = 2;
+  constexpr int threads = 512;
+  const int quads = batch <= 8 ? 2 : 1;
   bn::LogitsArgs a{x, out, token, x_row, out_row, (int)V, *rules};
   // blocks of a row: up to 8 (the portable cluster size), 16 where the rows are few
-  const int64_t need = (V + 4 * threads * quads - 1) / (4 * threads * quads);
+  const int64_t need = (V + 4 * threads - 1) / (4 * threads);
   const unsigned most = batch <= 8 ? 16 : 8;
   unsigned blocks = 1;
   while (blocks < most && blocks < need) blocks *= 2;
@@ -188,7 +189,7 @@ extern "C" int bn_logits(const void *x, int fp32, int64_t x_row, int64_t batch, 
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = blocks, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr, cfg.numAttrs = 1;
-  auto kern = fp32 ? bn::logits_kernel<float, threads, quads> : bn::logits_kernel<uint16_t, threads, quads>;
+  auto kern = quads == 2 ? (fp32 ? bn::logits_kernel<float, threads, 2> : bn::logits_kernel<uint16_t, threads, 2>) : fp32 ? bn::logits_kernel<float, threads, 1> : bn::logits_kernel<uint16_t, threads, 1>;
   if (blocks > 8) BN_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
   BN_CUDA(cudaLaunchKernelEx(&cfg, kern, a));
   return bn::launched("logits_kernel");

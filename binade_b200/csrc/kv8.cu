@@ -1,6 +1,8 @@
 // Writing and reading back the 8-bit key/value cache (bn_kv8).
 #include <stdio.h>
 
+#include <type_traits>
+
 #include "kv8.cuh"
 
 namespace bn {
@@ -18,25 +20,21 @@ struct AppendArgs {
 };
 
 // A block per block of tokens, keys or values. The read of the new rows and the write of the codes bound it.
-template <int CHUNKS>
+template <int D, int CHUNKS>
 __global__ void __launch_bounds__(128) append_kernel(const __grid_constant__ AppendArgs a) {
   const bn_kv8 &c = a.c;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");  // what made the tokens, and what read the cache before
-  uint32_t at = blockIdx.x;
-  const bool values = at & 1;
-  at >>= 1;
-  const int rel = (int)(at % a.rel);
-  at /= a.rel;
-  const int h = (int)(at % (uint32_t)c.kv_heads);
-  const int64_t b = at / (uint32_t)c.kv_heads;
+  const bool values = blockIdx.x & 1;
+  const int rel = (int)(blockIdx.x >> 1), h = (int)blockIdx.y;
+  const int64_t b = blockIdx.z;
   int held, brought;
   const bool all = kv8_tokens(c, a.counts, a.tokens, b, held, brought);
   if (!all && rel == 0 && h == 0 && !values && threadIdx.x == 0) atomicExch(&g_kv8_error, 1);
   const int j = held / c.block + rel;
   if (brought == 0 || j > (held + brought - 1) / c.block) return;
   const bool v = values;
-  append_block<CHUNKS>(c, v, b, h, j, held, held + brought, v ? a.v + b * a.v_seq + h * a.v_head : a.k + b * a.k_seq + h * a.k_head, v ? a.v_token : a.k_token);
+  append_block<D, CHUNKS>(c, v, b, h, j, held, held + brought, v ? a.v + b * a.v_seq + h * a.v_head : a.k + b * a.k_seq + h * a.k_head, v ? a.v_token : a.k_token);
 }
 
 __global__ void __launch_bounds__(256) advance_kernel(const __grid_constant__ bn_kv8 c, int n, const int32_t *__restrict__ counts) {
@@ -120,15 +118,16 @@ extern "C" int bn_kv8_append(const bn_kv8 *c, const uint16_t *k, int64_t k_seq, 
   if (tokens == 0) return BN_OK;
   bn::AppendArgs a{*c, k, v, k_seq, k_token, k_head, v_seq, v_token, v_head, counts, (int)tokens, 0};
   a.rel = (int)((tokens + c->block - 1) / c->block) + 1;  // a run of tokens that starts inside a block touches one more
-  const int64_t blocks = c->batch * c->kv_heads * a.rel * 2;
-  if (blocks > 0x7FFFFFFF) return bn::fail(BN_ERR_ARG, "bn_kv8_append: too many tokens for one call");
-  const int chunks = (int)(c->block * c->D / 1024);
-  auto kern = chunks == 1 ? bn::append_kernel<1> : chunks == 2 ? bn::append_kernel<2> : chunks == 4 ? bn::append_kernel<4> : chunks == 8 ? bn::append_kernel<8> : bn::append_kernel<16>;
+  auto pick = [&](auto d) {
+    constexpr int D = decltype(d)::value;
+    return c->block == 16 ? bn::append_kernel<D, 16 * D / 1024> : c->block == 32 ? bn::append_kernel<D, 32 * D / 1024> : bn::append_kernel<D, 64 * D / 1024>;
+  };
+  auto kern = c->D == 64 ? pick(std::integral_constant<int, 64>()) : c->D == 128 ? pick(std::integral_constant<int, 128>()) : pick(std::integral_constant<int, 256>());
   cudaLaunchConfig_t cfg{};
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.gridDim = dim3((unsigned)blocks), cfg.blockDim = dim3(128), cfg.stream = (cudaStream_t)stream, cfg.attrs = attr, cfg.numAttrs = 1;
+  cfg.gridDim = dim3((unsigned)a.rel * 2, (unsigned)c->kv_heads, (unsigned)c->batch), cfg.blockDim = dim3(128), cfg.stream = (cudaStream_t)stream, cfg.attrs = attr, cfg.numAttrs = 1;
   BN_CUDA(cudaLaunchKernelEx(&cfg, kern, a));
   return bn::launched("append_kernel");
 }

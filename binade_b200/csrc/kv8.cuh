@@ -27,7 +27,7 @@ __device__ __forceinline__ int kv8_slot(const bn_kv8 &c, int64_t b, int held, in
 template <int KIND>
 __device__ __forceinline__ float kv8_code(uint32_t byte) {
   if constexpr (KIND == KV8_INT8) {
-    return (float)((int)byte - 128);
+    return __uint_as_float(0x4B000000u | byte) - 8388736.0f;  // 2^23 + code + 128, less both
   } else {
     __nv_fp8_e4m3 f;
     f.__x = (__nv_fp8_storage_t)byte;
@@ -35,13 +35,13 @@ __device__ __forceinline__ float kv8_code(uint32_t byte) {
   }
 }
 // The nearest code to x / scale, ties to the even one, for finite x; 0 for NaN, the largest code for an infinity.
-// As stored, with 128 added. x times the inverse is off by at most 2^-15 in a quotient of up to 127: only next to the
+// As stored, with 128 added. x times the inverse is off by at most 127 * 2^-23 in a quotient of up to 127: only next to the
 // middle of two codes the real quotient decides, by the sign of x - middle * scale, which one rounding keeps.
 __device__ __forceinline__ uint32_t int8_code(float x, float scale, float inv) {
   const float t = x * inv;
   int q = __float2int_rn(t);  // NaN: 0
   const float off = t - (float)q;
-  if (fabsf(fabsf(off) - 0.5f) < 0.0005f) {
+  if (fabsf(fabsf(off) - 0.5f) < 0.0001f) {
     const float middle = (float)q + (off > 0.0f ? 0.5f : -0.5f), side = fmaf(-middle, scale, x);
     const int below = (int)floorf(middle);
     q = side > 0.0f ? below + 1 : side < 0.0f ? below : below + (below & 1);
@@ -70,7 +70,7 @@ __device__ __forceinline__ uint32_t int8_codes(uint32_t lo, uint32_t hi, float i
 #pragma unroll
   for (int e = 0; e < 4; e++) {
     const float t = x[e] * inv, sum = t + MAGIC, off = t - (sum - MAGIC);
-    close |= fabsf(off) > 0.4995f;
+    close |= fabsf(off) > 0.49998f;  // (the quotient is off by at most 127 * 2^-23)
     r[e] = __float_as_uint(sum);
   }
   return __byte_perm(__byte_perm(r[0], r[1], 0x0040), __byte_perm(r[2], r[3], 0x0040), 0x5410);
@@ -81,37 +81,56 @@ __device__ __forceinline__ uint32_t int8_codes(uint32_t lo, uint32_t hi, float i
 // rows, `step` elements apart. CHUNKS: pieces of eight values that a thread has: neighbours of one token, or for values
 // two neighbours of four tokens, whose codes lie together. A block stays in registers between its maximum and its
 // codes.
-template <int CHUNKS>
+template <int D, int CHUNKS>
 __device__ __forceinline__ void append_block(const bn_kv8 &c, bool values, int64_t b, int h, int j, int held, int end, const uint16_t *__restrict__ in, int64_t step) {
   __shared__ uint32_t part_max[4];
-  const int block = c.block, D = (int)c.D;
+  const int block = c.block;
   const int64_t unit = b * c.kv_heads + h;
   const bool full = (j + 1) * (int64_t)block <= end, open = j == held / block || !full;  // the first block goes to its slot, full or not
   uint16_t *const tail = (values ? c.v_tail : c.k_tail) + (unit * 2 + (open ? kv8_slot(c, b, held, j) : 0)) * block * D;
   uint4 x[CHUNKS];
   uint32_t most = 0;  // largest magnitudes, as pairs of 16 bits
+  if (full && !open) {  // most blocks of a prompt: every token is new, and none goes to the tail
+    in += (int64_t)(j * block - held) * step;
 #pragma unroll
-  for (int i = 0; i < CHUNKS; i++) {
-    const int chunk = (int)threadIdx.x + 128 * i;
-    if (values) {
-      const int row = chunk / (D / 2) * 4, col = chunk % (D / 2) * 2;
-      uint32_t w[4] = {};
+    for (int i = 0; i < CHUNKS; i++) {
+      const int chunk = (int)threadIdx.x + 128 * i;
+      if (values) {
+        const uint16_t *const at = in + (int64_t)(chunk / (D / 2) * 4) * step + chunk % (D / 2) * 2;
+        uint32_t w[4];
 #pragma unroll
-      for (int e = 0; e < 4; e++) {
-        const int p = j * block + row + e;
-        if (p < end && (full || p >= held)) w[e] = *reinterpret_cast<const uint32_t *>(p < held ? tail + (row + e) * D + col : in + (int64_t)(p - held) * step + col);
-        if (open && p >= held && p < end) *reinterpret_cast<uint32_t *>(tail + (row + e) * D + col) = w[e];
+        for (int e = 0; e < 4; e++) w[e] = *reinterpret_cast<const uint32_t *>(at + e * step);
+        x[i] = make_uint4(__byte_perm(w[0], w[1], 0x5410), __byte_perm(w[2], w[3], 0x5410), __byte_perm(w[0], w[1], 0x7632), __byte_perm(w[2], w[3], 0x7632));
+      } else {
+        x[i] = *reinterpret_cast<const uint4 *>(in + (int64_t)(chunk / (D / 8)) * step + chunk % (D / 8) * 8);
       }
-      // dimension by dimension: the order in which the codes lie
-      x[i] = make_uint4(__byte_perm(w[0], w[1], 0x5410), __byte_perm(w[2], w[3], 0x5410), __byte_perm(w[0], w[1], 0x7632), __byte_perm(w[2], w[3], 0x7632));
-    } else {
-      const int row = chunk / (D / 8), col = chunk % (D / 8) * 8, p = j * block + row;
-      x[i] = make_uint4(0, 0, 0, 0);
-      if (p < end && (full || p >= held)) x[i] = *reinterpret_cast<const uint4 *>(p < held ? tail + row * D + col : in + (int64_t)(p - held) * step + col);
-      if (open && p >= held && p < end) *reinterpret_cast<uint4 *>(tail + row * D + col) = x[i];
     }
-    most = __vmaxu2(__vmaxu2(most, x[i].x & 0x7FFF7FFFu), __vmaxu2(x[i].y & 0x7FFF7FFFu, __vmaxu2(x[i].z & 0x7FFF7FFFu, x[i].w & 0x7FFF7FFFu)));
+  } else {
+#pragma unroll
+    for (int i = 0; i < CHUNKS; i++) {
+      const int chunk = (int)threadIdx.x + 128 * i;
+      if (values) {
+        const int row = chunk / (D / 2) * 4, col = chunk % (D / 2) * 2;
+        uint32_t w[4] = {};
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          const int p = j * block + row + e;
+          if (p < end && (full || p >= held)) w[e] = *reinterpret_cast<const uint32_t *>(p < held ? tail + (row + e) * D + col : in + (int64_t)(p - held) * step + col);
+          if (open && p >= held && p < end) *reinterpret_cast<uint32_t *>(tail + (row + e) * D + col) = w[e];
+        }
+        // dimension by dimension: the order in which the codes lie
+        x[i] = make_uint4(__byte_perm(w[0], w[1], 0x5410), __byte_perm(w[2], w[3], 0x5410), __byte_perm(w[0], w[1], 0x7632), __byte_perm(w[2], w[3], 0x7632));
+      } else {
+        const int row = chunk / (D / 8), col = chunk % (D / 8) * 8, p = j * block + row;
+        x[i] = make_uint4(0, 0, 0, 0);
+        if (p < end && (full || p >= held)) x[i] = *reinterpret_cast<const uint4 *>(p < held ? tail + row * D + col : in + (int64_t)(p - held) * step + col);
+        if (open && p >= held && p < end) *reinterpret_cast<uint4 *>(tail + row * D + col) = x[i];
+      }
+    }
   }
+#pragma unroll
+  for (int i = 0; i < CHUNKS; i++)
+    most = __vmaxu2(__vmaxu2(most, x[i].x & 0x7FFF7FFFu), __vmaxu2(x[i].y & 0x7FFF7FFFu, __vmaxu2(x[i].z & 0x7FFF7FFFu, x[i].w & 0x7FFF7FFFu)));
   if (!full) return;
 #pragma unroll
   for (int d = 16; d; d >>= 1) most = __vmaxu2(most, __shfl_xor_sync(BN_FULL, most, d));

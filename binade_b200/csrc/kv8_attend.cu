@@ -293,9 +293,9 @@ __device__ __noinline__ void append_filled(const AttendArgs &a, int64_t b, int h
     const uint16_t *const in = side ? a.v + b * a.v_seq + h * a.v_head : a.k + b * a.k_seq + h * a.k_head;
     const int64_t step = side ? a.v_token : a.k_token;
     for (int j = first; j <= last; j++) {
-      if (a.c.block == 16) append_block<16 * D / 1024>(a.c, side, b, h, j, held, L, in, step);
-      else if (a.c.block == 32) append_block<32 * D / 1024>(a.c, side, b, h, j, held, L, in, step);
-      else append_block<64 * D / 1024>(a.c, side, b, h, j, held, L, in, step);
+      if (a.c.block == 16) append_block<D, 16 * D / 1024>(a.c, side, b, h, j, held, L, in, step);
+      else if (a.c.block == 32) append_block<D, 32 * D / 1024>(a.c, side, b, h, j, held, L, in, step);
+      else append_block<D, 64 * D / 1024>(a.c, side, b, h, j, held, L, in, step);
     }
   }
   __syncthreads();

@@ -72,7 +72,7 @@ __global__ void __launch_bounds__(THREADS, U == 1 ? 4 : 2) logits_kernel(const _
   for (int k0 = blockIdx.x * THREADS + threadIdx.x; k0 < quads; k0 += U * stride) {
     float y[U][4], add[U][4];
     uint32_t said[U], open[U];
-    int n[U][4];
+    int n[U];  // the count of the first token of the quad that was said
 #pragma unroll
     for (int u = 0; u < U; u++) {
       const int t = 4 * (k0 + u * stride) - shift;
@@ -110,24 +110,25 @@ __global__ void __launch_bounds__(THREADS, U == 1 ? 4 : 2) logits_kernel(const _
 #pragma unroll
     for (int u = 0; u < U; u++) {
       const int t = 4 * (k0 + u * stride) - shift;
-#pragma unroll
-      for (int e = 0; e < 4; e++) {
-        if (t + e < 0 || t + e >= V) said[u] &= ~(1u << e);
-        n[u][e] = (said[u] >> e) & 1u ? counts[t + e] : 0;
-      }
+      said[u] &= t < 0 ? 15u << -t : t + 3 >= V ? 15u >> (t + 4 - V) : 15u;
+      n[u] = said[u] ? counts[t + __ffs((int)said[u]) - 1] : 0;
     }
 #pragma unroll
     for (int u = 0; u < U; u++) {
       const int t = 4 * (k0 + u * stride) - shift;
       if (k0 + u * stride >= quads) break;
+      // every operation rounds by itself, in the order of the definition: a plain evaluation gives the same bits
+      for (uint32_t left = said[u]; left; left &= left - 1) {  // few tokens are: a loop over those
+        const int e = __ffs((int)left) - 1, count = left == said[u] ? n[u] : counts[t + e];
+        float z = e & 2 ? (e & 1 ? y[u][3] : y[u][2]) : (e & 1 ? y[u][1] : y[u][0]);
+        z = z > 0.0f ? __fdiv_rn(z, repetition) : __fmul_rn(z, repetition);
+        if (count > 0) z = __fsub_rn(z, __fadd_rn(__fmul_rn(frequency, (float)count), presence));
+#pragma unroll
+        for (int i = 0; i < 4; i++) y[u][i] = i == e ? z : y[u][i];
+      }
 #pragma unroll
       for (int e = 0; e < 4; e++) {
-        // every operation rounds by itself, in the order of the definition: a plain evaluation gives the same bits
         float &z = y[u][e];
-        if ((said[u] >> e) & 1u) {
-          z = z > 0.0f ? __fdiv_rn(z, repetition) : __fmul_rn(z, repetition);
-          if (n[u][e] > 0) z = __fsub_rn(z, __fadd_rn(__fmul_rn(frequency, (float)n[u][e]), presence));
-        }
         if (bias) z = __fadd_rn(z, add[u][e]);
         if (!((open[u] >> e) & 1u)) z = -CUDART_INF_F;
         if (z > best.value && t + e >= 0 && t + e < V) best = {z, t + e};  // (NaN is never chosen)

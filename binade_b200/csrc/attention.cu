@@ -12,7 +12,7 @@ int attention_launch(const PromptArgs &a, cudaStream_t stream) {
   if (!rows_map(&q_map, a.q, D, a.heads, a.T, 1, a.q_head, a.q_token, 0, group, 128 / group, 4) || !rows_map(&k_map, a.k, D, a.kv_heads, a.T, 1, a.k_head, a.k_token, 0, 1, G::BN, 3) || !rows_map(&v_map, a.v, D, a.kv_heads, a.T, 1, a.v_head, a.v_token, 0, 1, G::BN, 3))
     return fail(BN_ERR_ARG, "bn_attention: no tensor map for these strides");
   const int64_t blocks = ((int64_t)a.T * group / G::ROWS + a.docs + 1) * (a.heads / group);
-  if (blocks > 0x7FFFFFFF) return fail(BN_ERR_ARG, "bn_attention: too many rows");
+  if (blocks > 0x7FFFFFFF || (int64_t)a.T * group > 0x3FFFFFFF) return fail(BN_ERR_ARG, "bn_attention: too many rows");
   return prompt_launch<D, FROM_BF16>(a, q_map, k_map, v_map, blocks, log2, stream);
 }
 

@@ -38,7 +38,6 @@ __device__ int g_attend_error;  // 1: tokens were brought that the cache has no 
 __device__ __forceinline__ void kv8_overflow() { atomicExch(&g_attend_error, 1); }
 
 constexpr int WARPS = 4;
-constexpr int MIN_SHARE = 1;
 constexpr float HEADROOM = 15.0f;  // weights may reach 2^15
 constexpr float NOTHING = -3.402823466e38f;  // a row's m while no key was visible: finite, so that a masked score less m stays -inf
 
@@ -483,7 +482,7 @@ __global__ void __launch_bounds__(WARPS * 32, (D == 64 && MT == 1) ? 4 : (MT * D
     if (w < (int)warp) before += warp_tiles[w];
     total += warp_tiles[w];
   }
-  const int64_t share = max((total * per_seq + a.blocks - 1) / a.blocks, (int64_t)MIN_SHARE);
+  const int64_t share = max((total * per_seq + a.blocks - 1) / a.blocks, (int64_t)1);
   int64_t x = (int64_t)blockIdx.x * share;
   const int64_t x_end = min(x + share, total * per_seq);
   for (int64_t b = b_from, at = before; b < b_to; b++) {

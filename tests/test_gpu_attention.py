@@ -295,6 +295,71 @@ def test_chunks_over_the_cache(kind, D, heads, kv, block, options):
     h.check_attend([256, 300, 0], heads, g, slopes=slopes_of(heads), prefixes=[10, 500, 3], **options)
 
 
+@pytest.mark.parametrize("kind", ["int8", "e4m3"])
+@pytest.mark.parametrize("D,block", [(64, 64), (128, 16), (256, 32)])
+@pytest.mark.parametrize("options", [{}, dict(softcap=10.0), dict(window=90), dict(scale=-0.1)])
+def test_wide_batches_of_chunks(kind, D, block, options):
+    """Many rows, enough of them for the kernel that reads the keys once: blocks that end inside a tile of keys, sequences
+    without tokens, heads of a group that is no power of two, and values that are not finite in the open block."""
+    g = gen(D + block)
+    h = History(5, 8, D, 900, kind, block)
+    h.append([0, 3, 200, 129, 500], g)
+    h.check_attend([150, 97, 1, 0, 64], 24, g, **options)
+    h.check_attend([64, 130, 33, 200, 128], 24, g, apart=True, **options)
+    h.check_attend([30, 100, 97, 10, 3], 8, g, **options)
+    q, k, v = normal((5, 100, 16, D), g), normal((5, 100, 8, D), g), normal((5, 100, 8, D), g)
+    held = h.cache.length.tolist()
+    at = [max(0, (n + 100) // block * block - n) for n in held]  # the first token of each sequence that stays in the open block
+    for b in range(5):
+        if at[b] < 100:
+            k[b, at[b], 2], v[b, at[b], 3, 5] = math.nan, math.inf
+    got = h.cache.attend(0, q, k, v, **options)
+    for b in range(5):
+        if at[b] >= 100:
+            continue
+        clean = [torch.cat([x, y[b]]) for x, y in ((h.k[b], k), (h.v[b], v))]
+        stored = [ref.stored(torch.nan_to_num(x.float(), nan=0.0, posinf=0.0).to(torch.bfloat16), kind, block) for x in clean]
+        want, bound = ref.attend(q[b], *stored, held[b], **options)
+        touched = torch.zeros((100, 16), dtype=torch.bool, device="cuda")
+        end = at[b] + (options.get("window") or 1000)
+        touched[at[b] : end, 4:8] = True  # heads of key heads 2 and 3
+        close(got[b][~touched], want[~touched], bound[~touched])
+        assert torch.isnan(got[b, at[b] : end, 4:6]).all() and (got[b, at[b] : end, 6:8, 5] == math.inf).all()
+        close(got[b, at[b] : end, 6:8, 6:], want[at[b] : end, 6:8, 6:], bound[at[b] : end, 6:8, 6:])
+
+
+@pytest.mark.parametrize("heads,kv", [(40, 1), (64, 1), (24, 2), (12, 12)])
+def test_groups_of_many_sizes(heads, kv):
+    check_prompt([70, 130], heads, kv, 128, seed=heads)
+    g = gen(heads)
+    h = History(2, kv, 128, 400, "int8", 32)
+    h.append([70, 200], g)
+    for counts in ([1, 1], [2, 1], [16, 9], [17, 3], [1, 0]):
+        h.check_attend(counts, heads, g)
+
+
+def test_steps_over_block_borders_equal_append_and_attend():
+    """A step that appends inside the attention's launch gives what append and attend apart give, bit for bit in what
+    is stored, at every place of a block, drafts that fill one among them."""
+    from binade_b200.cuda.attention import KV8Cache
+
+    g = gen(60)
+    for block, D, kind in ((16, 64, "int8"), (64, 128, "e4m3"), (32, 256, "int8")):
+        a, b = (KV8Cache(1, 3, 2, D, 600, kind=kind, block=block) for _ in range(2))
+        for step in range(60):
+            n = 1 + step * 7 % 16
+            q, k, v = normal((3, n, 4, D), g), normal((3, n, 2, D), g), normal((3, n, 2, D), g)
+            counts = torch.tensor([n, max(0, n - 3), step % 2], device="cuda")
+            x = a.attend(0, q, k, v, counts)
+            b.append(0, k, v, counts)
+            y = b.attend(0, q, counts=counts)
+            a.advance(counts), b.advance(counts)
+            assert torch.allclose(x.float(), y.float(), atol=2e-2, rtol=2e-2)
+            for s, t in ((a.k, b.k), (a.v, b.v), (a.k_scale, b.k_scale), (a.v_scale, b.v_scale), (a.k_tail, b.k_tail), (a.v_tail, b.v_tail), (a.length, b.length), (a._side, b._side)):
+                assert torch.equal(s, t)
+            assert not a._tickets.any()
+
+
 def test_decode_long_and_wide():
     """A cache of more than 2^31 codes in one array, its last sequence behind that border."""
     g = gen(32)

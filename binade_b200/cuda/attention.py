@@ -24,24 +24,31 @@ BLOCKS = (16, 32, 64)
 KINDS = {"int8": 0, "e4m3": 1}  # BN_KV8_INT8, BN_KV8_E4M3
 
 
-def _rows(t: torch.Tensor, name: str, dims: int, device) -> torch.Tensor:
+def _rows(t: torch.Tensor, name: str, dims: int, device, apart: bool = False):
     """Checks a BF16 tensor of rows (its last dimension a head's) on CUDA device number `device` and gives it with
-    rows that the kernels can read: neighbouring elements, every row on 16 bytes."""
+    rows that the kernels can read (neighbouring elements, every row on 16 bytes; apart: no two the same), and the
+    strides of its leading dimensions, 0 for one that is not stepped."""
     if not isinstance(t, torch.Tensor) or t.dtype is not torch.bfloat16 or t.dim() != dims:
         raise ValueError(f"{name} has to be a bfloat16 tensor of {dims} dimensions")
     if t.get_device() != device:
         raise ValueError(f"{name} is on {t.device}, the call on cuda:{device}")
     if t.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{name} asks for a gradient: attention here has none (use torch.no_grad)")
-    if t.data_ptr() % 16 == 0 and (t.is_contiguous() or (t.stride(-1) == 1 and not any(s % 8 for s, n in zip(t.stride()[:-1], t.shape[:-1]) if n > 1))):
-        return t  # (a contiguous tensor's rows lie on 16 bytes: a head has 64 dimensions at least)
-    t = t.contiguous()
-    return t if t.data_ptr() % 16 == 0 else t.clone()
+    if t.is_contiguous() and t.data_ptr() % 16 == 0:
+        return t, t.stride()[:-1]
+    steps = _steps(t)
+    fits = t.stride(-1) == 1 and t.data_ptr() % 16 == 0
+    for s, n in zip(steps, t.shape):
+        fits = fits and not s % 8 and (s or n <= 1 or not apart)
+    if not fits:
+        t = t.contiguous() if not t.is_contiguous() else t.clone()
+        steps = _steps(t)
+    return t, steps
 
 
 def _steps(t: torch.Tensor):
     """Strides of the leading dimensions; of one that is not stepped, 0."""
-    return [s if n > 1 else 0 for s, n in zip(t.stride()[:-1], t.shape[:-1])]
+    return [s if n > 1 else 0 for s, n in zip(t.stride(), t.shape)][:-1]
 
 
 def _numbers(t, name: str, n: int, device, dtype=torch.int32) -> torch.Tensor | None:
@@ -49,7 +56,7 @@ def _numbers(t, name: str, n: int, device, dtype=torch.int32) -> torch.Tensor | 
         return None
     if not isinstance(t, torch.Tensor) or t.get_device() != device or t.dim() != 1 or t.numel() != n or (dtype == torch.int32 and t.is_floating_point()):
         raise ValueError(f"{name} has to be a tensor of {n} {'whole ' if dtype == torch.int32 else ''}numbers on cuda:{device}")
-    return t.to(dtype).contiguous()
+    return t if t.dtype is dtype and t.is_contiguous() else t.to(dtype).contiguous()
 
 
 def extent(t: torch.Tensor):
@@ -114,10 +121,10 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets: torch.
     it, but for the first prefix[n] of its document n. window: only keys at a distance below it. scale
     defaults to 1 / sqrt(D). Nothing is read on the host: the call can be captured in a graph."""
     dev = _device(q)
-    q = _rows(q, "q", 3, dev)
+    q, q_steps = _rows(q, "q", 3, dev, apart=True)
+    k, k_steps = _rows(k, "k", 3, dev, apart=True)
+    v, v_steps = _rows(v, "v", 3, dev, apart=True)
     T, heads, D = q.shape
-    k, v = _rows(k, "k", 3, dev), _rows(v, "v", 3, dev)
-    q, k, v = (t.contiguous() if 0 in t.stride() else t for t in (q, k, v))  # (expanded rows)
     kv = k.shape[1]
     if D not in HEAD_DIMS or k.shape != (T, kv, D) or v.shape != k.shape or kv < 1 or heads < 1 or heads % kv:
         raise ValueError(f"q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}: heads of 64, 128 or 256, query heads a multiple of key heads, the same tokens")
@@ -131,7 +138,7 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets: torch.
     scores, slopes = _scores(D, heads, dev, scale, softcap, window, slopes, causal)
     y = _out(out, q, dev, q, k, v)
     if T:
-        ck._call("bn_attention", ck._p(q), *_steps(q), ck._p(k), *_steps(k), ck._p(v), *_steps(v), T, heads, kv, D, ck._p(offsets), docs, ck._p(prefix), ctypes.byref(scores), ck._p(y), *_steps(y), int(out is None))
+        ck._call("bn_attention", q.data_ptr(), *q_steps, k.data_ptr(), *k_steps, v.data_ptr(), *v_steps, T, heads, kv, D, ck._p(offsets), docs, ck._p(prefix), ctypes.byref(scores), y.data_ptr(), *(y.stride()[:-1] if out is None else _steps(y)), int(out is None))
     return y
 
 
@@ -176,11 +183,11 @@ class KV8Cache:
             raise ValueError(f"the cache is on {self.device}, the current device is another one")
         return ctypes.byref(self._structs[layer])
 
-    def _new(self, t, name: str, heads: int | None = None) -> torch.Tensor:
-        t = _rows(t, name, 4, self._index)
+    def _new(self, t, name: str, heads: int | None = None, apart: bool = False):
+        t, steps = _rows(t, name, 4, self._index, apart)
         if t.shape[0] != self.batch or t.shape[3] != self.head_dim or (heads is not None and t.shape[2] != heads):
             raise ValueError(f"{name} {tuple(t.shape)}: [batch {self.batch}, tokens, {'heads' if heads is None else heads}, {self.head_dim}] expected")
-        return t
+        return t, steps
 
     def append(self, layer: int, k: torch.Tensor, v: torch.Tensor, counts: torch.Tensor | None = None) -> None:
         """New tokens k, v [batch, tokens, kv_heads, D] bfloat16 behind what the sequences hold; counts (whole
@@ -188,12 +195,12 @@ class KV8Cache:
         `length` stays until `advance`: until then a second append writes the same places again. Tokens
         beyond max_seq are dropped, and bn_device_status tells (bits 24..27)."""
         at = self._layer(layer)
-        k, v = self._new(k, "k", self.kv_heads), self._new(v, "v", self.kv_heads)
+        (k, k_steps), (v, v_steps) = self._new(k, "k", self.kv_heads), self._new(v, "v", self.kv_heads)
         if k.shape != v.shape:
             raise ValueError(f"k {tuple(k.shape)} and v {tuple(v.shape)} differ")
         counts = _numbers(counts, "counts", self.batch, self._index)
         if k.shape[1]:
-            ck._call("bn_kv8_append", at, ck._p(k), *_steps(k), ck._p(v), *_steps(v), k.shape[1], ck._p(counts))
+            ck._call("bn_kv8_append", at, k.data_ptr(), *k_steps, v.data_ptr(), *v_steps, k.shape[1], ck._p(counts))
 
     def attend(self, layer: int, q: torch.Tensor, k: torch.Tensor | None = None, v: torch.Tensor | None = None, counts: torch.Tensor | None = None, *, causal: bool = True, scale: float | None = None, softcap: float | None = None, window: int | None = None, slopes: torch.Tensor | None = None, prefix: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
         """Attention of new tokens q [batch, tokens, heads, D] bfloat16 over what their sequences hold and
@@ -202,9 +209,7 @@ class KV8Cache:
         length[b] + counts[b] if not causal; options as in `attention`, prefix [batch]). Rows behind a sequence's
         counts come back as zeros, or, with `out` given, stay as they are."""
         at = self._layer(layer)
-        q = self._new(q, "q")
-        if 0 in q.stride():  # (expanded rows)
-            q = q.contiguous()
+        q, q_steps = self._new(q, "q", apart=True)
         tokens, heads = q.shape[1], q.shape[2]
         if heads < 1 or heads % self.kv_heads:
             raise ValueError(f"{heads} query heads over {self.kv_heads} key heads")
@@ -217,16 +222,16 @@ class KV8Cache:
         if k is None:
             new = (None, 0, 0, 0, None, 0, 0, 0)
         else:
-            k, v = self._new(k, "k", self.kv_heads), self._new(v, "v", self.kv_heads)
+            (k, k_steps), (v, v_steps) = self._new(k, "k", self.kv_heads), self._new(v, "v", self.kv_heads)
             if k.shape[1] != tokens or v.shape[1] != tokens:
                 raise ValueError(f"k {tuple(k.shape)} and v {tuple(v.shape)} for {tokens} tokens")
-            new = (k.data_ptr(), *_steps(k), v.data_ptr(), *_steps(v))
+            new = (k.data_ptr(), *k_steps, v.data_ptr(), *v_steps)
         if tokens:
             need = self._work.get((tokens, heads))
             if need is None:
                 need = self._work[tokens, heads] = _native.load("cuda").bn_kv8_workspace(at, tokens, heads)
             work = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
-            ck._call("bn_kv8_attend", at, q.data_ptr(), *_steps(q), *new, tokens, heads, ck._p(counts), ck._p(prefix), ctypes.byref(scores), y.data_ptr(), *_steps(y), int(out is None), ck._p(work), need)
+            ck._call("bn_kv8_attend", at, q.data_ptr(), *q_steps, *new, tokens, heads, ck._p(counts), ck._p(prefix), ctypes.byref(scores), y.data_ptr(), *(y.stride()[:-1] if out is None else _steps(y)), int(out is None), ck._p(work), need)
         return y
 
     def advance(self, n) -> None:

@@ -60,7 +60,7 @@ def _penalty(p, name: str, batch: int, device):
     if isinstance(p, torch.Tensor):
         if p.device != device or p.shape != (batch,):
             raise ValueError(f"{name} has to be a number or a tensor of {batch} on {device}")
-        return p.to(torch.float32).contiguous(), 0.0
+        return p if p.dtype is torch.float32 and p.is_contiguous() else p.to(torch.float32).contiguous(), 0.0
     return None, float(p)
 
 
@@ -108,7 +108,7 @@ def process_logits(logits: torch.Tensor, said: TokenCounts | None = None, *, rep
         setattr(rules, name, ck._p(t))
         setattr(rules, name + "_row", width if t.dim() == 2 else 0)
     if out is None:
-        out = torch.empty((batch, vocab), dtype=torch.float32, device=dev)
+        out = torch.empty(batch, vocab, dtype=torch.float32, device=dev)
     elif not isinstance(out, torch.Tensor) or out.dtype != torch.float32 or out.shape != logits.shape or out.device != dev or out.requires_grad or (vocab > 1 and out.stride(1) != 1) or (batch > 1 and out.stride(0) < vocab):
         raise ValueError("out has to be float32 of the logits' shape with rows of neighbouring elements that do not overlap")
     elif overlap(out, logits) and not (out.data_ptr() == logits.data_ptr() and out.dtype == logits.dtype and (batch == 1 or out.stride(0) == logits.stride(0))):

@@ -199,11 +199,12 @@ __device__ __forceinline__ bool piece_of(const PromptArgs &a, int group, int64_t
   int64_t first = 0;
   if (a.offsets) {
     auto start = [&](int n) { return (int64_t)min(max(a.offsets[n], 0), a.T) * group / ROWS + n; };
-    int lo = 0, hi = a.docs;  // the last n with start(n) <= slot
+    int lo = 0, hi = a.docs;  // the last n with start(n) <= slot, by a warp's 32 looks at a time
     while (lo < hi) {
-      const int m = (lo + hi + 1) >> 1;
-      if (start(m) <= slot) lo = m;
-      else hi = m - 1;
+      const int step = (hi - lo + 31) / 32, look = lo + step * ((int)lane_id() + 1);
+      const uint32_t below = __ballot_sync(BN_FULL, look <= hi && start(look) <= slot);
+      const int some = __popc(below);
+      hi = min(hi, lo + step * (some + 1) - 1), lo += step * some;
     }
     if (lo >= a.docs) return false;
     doc = lo, first = start(lo);
@@ -287,12 +288,15 @@ __global__ void __launch_bounds__(Roles<SRC>::WARPS * 32, 1) prompt_kernel(const
   using G = Tiles<D>;
   constexpr int NQ = G::NQ, BN = G::BN, ST = G::STAGES, TMA_WARP = Roles<SRC>::TMA_WARP, MMA_WARP = Roles<SRC>::MMA_WARP;
   constexpr bool CODES = SRC != FROM_BF16;
+  // Weights to the sums in two halves: worth it where the softmax is what the products wait for (us, chunk of 2 x 500 tokens
+  // over 9000: 263 / 280 in one piece), not where the products of the other tile would start instead (8192 tokens: 540 / 477).
+  constexpr bool HALVES = NQ == 2 && CODES;
   extern __shared__ uint8_t prompt_smem[];
   const uint32_t lane = lane_id(), warp = threadIdx.x >> 5;
   const int group = 1 << group_log2;
   const uint32_t base = (smem_addr(prompt_smem) + 1023u) & ~1023u;
   const uint32_t q_at = base, ring_at = q_at + NQ * G::Q_BYTES, bars = ring_at + ST * G::TILE_BYTES;
-  const uint32_t q_full = bars, s_full = bars + 16, p_full = bars + 32, o_done = bars + 48, ring_full = bars + 64, ring_empty = ring_full + 8 * ST, scale_full = ring_empty + 8 * ST, raw_full = scale_full + 8 * SCALES_AHEAD, raw_empty = raw_full + 16, tmem_slot = raw_empty + 16, scales_at = bars + G::BARS, told_at = scales_at + G::SCALES, raw_at = told_at + G::TOLD;
+  const uint32_t q_full = bars, s_full = bars + 16, p_full = bars + 32, o_done = bars + 48, ring_full = bars + 64, ring_empty = ring_full + 8 * ST, scale_full = ring_empty + 8 * ST, raw_full = scale_full + 8 * SCALES_AHEAD, raw_empty = raw_full + 16, p_half = raw_empty + 16, tmem_slot = p_half + 16, scales_at = bars + G::BARS, told_at = scales_at + G::SCALES, raw_at = told_at + G::TOLD;
   if (base + (CODES ? G::WINDOW_CODES : G::WINDOW) > smem_addr(prompt_smem) + (CODES ? G::SMEM_CODES : G::SMEM)) {
     if (threadIdx.x == 0) atomicExch(&g_prompt_error, 2);
     return;
@@ -300,7 +304,7 @@ __global__ void __launch_bounds__(Roles<SRC>::WARPS * 32, 1) prompt_kernel(const
 
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (threadIdx.x == 0) {
-    for (int i = 0; i < 2; i++) mm_bar_init(q_full + 8 * i, 1), mm_bar_init(s_full + 8 * i, 1), mm_bar_init(p_full + 8 * i, NQ == 2 ? 128 : 256), mm_bar_init(o_done + 8 * i, 1);
+    for (int i = 0; i < 2; i++) mm_bar_init(q_full + 8 * i, 1), mm_bar_init(s_full + 8 * i, 1), mm_bar_init(p_full + 8 * i, NQ == 2 ? 128 : 256), mm_bar_init(p_half + 8 * i, 128), mm_bar_init(o_done + 8 * i, 1);
     for (int i = 0; i < ST; i++) mm_bar_init(ring_full + 8 * i, CODES ? CODE_WARPS : 1), mm_bar_init(ring_empty + 8 * i, 1);
     for (int i = 0; i < SCALES_AHEAD; i++) mm_bar_init(scale_full + 8 * i, CODE_WARPS);
     for (int i = 0; i < 2; i++) mm_bar_init(raw_full + 8 * i, 1), mm_bar_init(raw_empty + 8 * i, CODE_WARPS);
@@ -420,12 +424,21 @@ __global__ void __launch_bounds__(Roles<SRC>::WARPS * 32, 1) prompt_kernel(const
     };
     auto sums = [&](int i, int j, uint32_t v_tile) {
       const int n = j - j0[i], buf = NQ == 2 ? i : n & 1;
+      const uint64_t dv = smem_desc_columns(v_tile, BN * 128);
+      auto steps = [&](int from, int to) {
+#pragma unroll
+        for (int s = from; s < to; s++) mma_bf16_tmem(tmem + G::O_AT + i * D, tmem + G::S_AT + buf * BN + 8 * s, dv + s * (2048 >> 4), O_DESC, (n | s) != 0);
+      };
+      if constexpr (HALVES) {  // the first half of the keys while the other half's weights are made
+        if (ok) ok = prompt_wait_warp(p_half + 8 * buf, n & 1);
+        tc_fence_after();
+        if (lead && ok) steps(0, BN / 32);
+        __syncwarp();
+      }
       if (ok) ok = prompt_wait_warp(p_full + 8 * buf, NQ == 2 ? n & 1 : (n >> 1) & 1);
       tc_fence_after();
       if (lead && ok) {
-        const uint64_t dv = smem_desc_columns(v_tile, BN * 128);
-#pragma unroll
-        for (int s = 0; s < BN / 16; s++) mma_bf16_tmem(tmem + G::O_AT + i * D, tmem + G::S_AT + buf * BN + 8 * s, dv + s * (2048 >> 4), O_DESC, (n | s) != 0);
+        steps(HALVES ? BN / 32 : 0, BN / 16);
         mma_commit(o_done + 8 * buf);
       }
       __syncwarp();
@@ -677,13 +690,16 @@ __global__ void __launch_bounds__(Roles<SRC>::WARPS * 32, 1) prompt_kernel(const
         if constexpr (CODES) p01 = mul_f32x2(p01, vv), p23 = mul_f32x2(p23, vv);
         split_f32(p01, e0, e1), split_f32(p23, e2, e3);
         s[x / 2] = bf16_pair(e0, e1), s[x / 2 + 1] = bf16_pair(e2, e3);
+        if (HALVES && x == CN / 2 - 4) {  // half of the keys
+          tmem_store32(s_at, s);
+          tmem_wait_stores();
+          tc_fence_before();
+          mm_bar_arrive(p_half + 8 * buf);
+        }
       }
-      if constexpr (NQ == 2) {
-#pragma unroll
-        for (int x = 0; x < CN / 2; x += 32) tmem_store32(s_at + x, s + x);
-      } else {
-        tmem_store16(s_at + col0 / 2, s);
-      }
+      if constexpr (NQ == 2 && !HALVES) tmem_store32(s_at, s);
+      if constexpr (NQ == 2) tmem_store32(s_at + CN / 4, s + CN / 4);
+      else tmem_store16(s_at + col0 / 2, s);
       float s0, s1;
       split_f32(add_f32x2(sum, sum2), s0, s1);
       l += s0 + s1;

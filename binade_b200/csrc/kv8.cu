@@ -46,44 +46,44 @@ __global__ void __launch_bounds__(256) advance_kernel(const __grid_constant__ bn
   if (now / c.block != held / c.block) c.side[b] ^= 1;
 }
 
-// Eight values a thread, of keys eight of a token, of values two of four tokens, as the codes lie; tokens that the
-// cache does not hold as zeros. Blocks: pieces of a sequence and head, those, and keys or values.
+// Sixteen codes a thread at a time, as they lie: of keys sixteen dimensions of a token, of values four of four tokens. Tokens
+// that the cache does not hold as zeros. Blocks: pieces of a sequence and head, those, and keys or values.
 template <int KIND, int D>
 __global__ void __launch_bounds__(256) dense_kernel(const __grid_constant__ bn_kv8 c, float *__restrict__ k, float *__restrict__ v) {
   const bool values = blockIdx.z;
-  const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x, units = c.batch * c.kv_heads;
-  const int row = (int)(values ? at / (D / 2) * 4 : at / (D / 8)), col = (int)(values ? at % (D / 2) * 2 : at % (D / 8) * 8);
-  if (row >= c.max_seq) return;
-  const int block_log2 = 31 - __clz(c.block);
-  for (int64_t unit = blockIdx.y; unit < units; unit += gridDim.y) {
-    const int64_t b = (int)unit / (int)c.kv_heads;
+  const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t from_row = values ? at / (D / 4) * 4 : at / (D / 16);
+  if (from_row >= c.max_seq) return;
+  const int row = (int)from_row, col = (int)(values ? at % (D / 4) * 4 : at % (D / 16) * 16), block_log2 = 31 - __clz(c.block);
+  const unsigned heads = (unsigned)c.kv_heads, units = (unsigned)c.batch * heads;
+  for (unsigned unit = blockIdx.y; unit < units; unit += gridDim.y) {
+    const unsigned b = unit / heads;
     const int length = min(max(c.length[b], 0), (int)c.max_seq), full = length >> block_log2 << block_log2;
-    float x[8] = {};
+    float x[16] = {};
     if (row < full) {  // (a block has whole rows of four)
-      const float scale = (values ? c.v_scale : c.k_scale)[unit * (c.rows >> block_log2) + (row >> block_log2)];
-      const uint2 w = *reinterpret_cast<const uint2 *>((values ? c.v : c.k) + (unit * c.rows + row) * D + (values ? 4 : 1) * col);
+      const float scale = (values ? c.v_scale : c.k_scale)[(int64_t)unit * (c.rows >> block_log2) + (row >> block_log2)];
+      const uint4 w4 = *reinterpret_cast<const uint4 *>((values ? c.v : c.k) + ((int64_t)unit * c.rows + row) * D + (values ? 4 : 1) * col);
+      const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
 #pragma unroll
-      for (int e = 0; e < 8; e++) x[e] = kv8_code<KIND>(((e < 4 ? w.x : w.y) >> (8 * (e & 3))) & 0xFFu) * scale;
+      for (int e = 0; e < 16; e++) x[e] = kv8_code<KIND>((w[e >> 2] >> (8 * (e & 3))) & 0xFFu) * scale;
     } else if (row < length) {
-      const uint16_t *const tail = (values ? c.v_tail : c.k_tail) + ((unit * 2 + (c.side[b] & 1)) * c.block + row - full) * D + col;
+      const uint16_t *const tail = (values ? c.v_tail : c.k_tail) + (((int64_t)unit * 2 + (c.side[b] & 1)) * c.block + row - full) * D + col;
 #pragma unroll
-      for (int e = 0; e < 8; e++)
+      for (int e = 0; e < 16; e++)
         if (row + (values ? e & 3 : 0) < length) x[e] = bf16_to_f32(tail[values ? (e & 3) * D + (e >> 2) : e]);
     }
-    if (values) {
+    float *const out = (values ? v : k) + ((int64_t)unit * c.max_seq + row) * D + col;
 #pragma unroll
-      for (int e = 0; e < 4; e++)
-        if (row + e < c.max_seq) *reinterpret_cast<float2 *>(v + (unit * c.max_seq + row + e) * D + col) = make_float2(x[e], x[4 + e]);
-    } else {
-      float4 *const out = reinterpret_cast<float4 *>(k + (unit * c.max_seq + row) * D + col);
-      out[0] = make_float4(x[0], x[1], x[2], x[3]), out[1] = make_float4(x[4], x[5], x[6], x[7]);
+    for (int e = 0; e < 4; e++) {
+      if (!values) *reinterpret_cast<float4 *>(out + 4 * e) = make_float4(x[4 * e], x[4 * e + 1], x[4 * e + 2], x[4 * e + 3]);
+      else if (row + e < c.max_seq) *reinterpret_cast<float4 *>(out + e * D) = make_float4(x[e], x[4 + e], x[8 + e], x[12 + e]);
     }
   }
 }
 
 template <int KIND>
 int dense_launch(const bn_kv8 &c, float *k, float *v, cudaStream_t s) {
-  const int64_t units = c.batch * c.kv_heads, pieces = ((c.max_seq + 3) / 4 * 4 * (c.D / 8) + 255) / 256;
+  const int64_t units = c.batch * c.kv_heads, pieces = ((c.max_seq + 3) / 4 * 4 * (c.D / 16) + 255) / 256;
   const dim3 grid((unsigned)pieces, (unsigned)(units < 65535 ? units : 65535), 2);
   auto kern = c.D == 64 ? dense_kernel<KIND, 64> : c.D == 128 ? dense_kernel<KIND, 128> : dense_kernel<KIND, 256>;
   kern<<<grid, 256, 0, s>>>(c, k, v);

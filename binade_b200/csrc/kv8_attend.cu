@@ -191,7 +191,7 @@ __device__ __forceinline__ void weigh(const AttendArgs &a, float (&x)[P][MT][2][
     for (int mt = 0; mt < MT; mt++)
 #pragma unroll
       for (int h = 0; h < 2; h++) {
-        const float f = fminf(pc[p].scale * r.factor[mt][h], 3.0e38f);
+        const float f = fmaxf(fminf(pc[p].scale * r.factor[mt][h], 3.0e38f), -3.0e38f);
 #pragma unroll
         for (int j = 0; j < 2; j++)
 #pragma unroll

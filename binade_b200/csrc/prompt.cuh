@@ -289,8 +289,10 @@ __global__ void __launch_bounds__(Roles<SRC>::WARPS * 32, 1) prompt_kernel(const
   constexpr int NQ = G::NQ, BN = G::BN, ST = G::STAGES, TMA_WARP = Roles<SRC>::TMA_WARP, MMA_WARP = Roles<SRC>::MMA_WARP;
   constexpr bool CODES = SRC != FROM_BF16;
   // Weights to the sums in two halves: worth it where the softmax is what the products wait for (us, chunk of 2 x 500 tokens
-  // over 9000: 263 / 280 in one piece), not where the products of the other tile would start instead (8192 tokens: 540 / 477).
-  constexpr bool HALVES = NQ == 2 && CODES;
+  // over 9000: 263 / 280 in one piece; 6001 tokens with a bias: 55 / 57), not where the products of the other tile would
+  // start instead (8192 tokens: 540 / 477). Key tiles of 64 with two S buffers a query tile instead: 734 there, since a product
+  // of half the columns takes more than half the time.
+  constexpr bool HALVES = NQ == 2 && (CODES || !PLAIN);
   extern __shared__ uint8_t prompt_smem[];
   const uint32_t lane = lane_id(), warp = threadIdx.x >> 5;
   const int group = 1 << group_log2;

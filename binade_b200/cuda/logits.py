@@ -52,6 +52,8 @@ class TokenCounts:
 
     def clear(self, row=None) -> None:
         """Forgets everything, or one sequence's tokens (row: a number)."""
+        if row is not None and (not isinstance(row, int) or isinstance(row, bool) or not 0 <= row < self.batch):
+            raise ValueError(f"row {row!r} of {self.batch}")
         (self._all if row is None else self._all[row]).zero_()
 
 

@@ -577,6 +577,8 @@ def test_refusals():
         lambda: counts.add(torch.zeros((2, 1), device="cuda")),
         lambda: counts.add(torch.zeros((2, 1), dtype=torch.int64)),
         lambda: counts.add(torch.zeros((2, 1), dtype=torch.int64, device="cuda"), lengths=torch.ones(3, dtype=torch.int32, device="cuda")),
+        lambda: counts.clear(2),
+        lambda: counts.clear(torch.tensor([0])),
         lambda: TokenCounts(0, 5),
         lambda: TokenCounts(1, 5, device="cpu"),
     ):

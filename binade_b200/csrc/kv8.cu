@@ -19,7 +19,8 @@ struct AppendArgs {
   int tokens, rel;  // tokens a sequence brings at most; blocks of the cache that those can touch
 };
 
-// A block per block of tokens, keys or values. The read of the new rows and the write of the codes bound it.
+// A block per block of tokens, keys or values. 4 x 2000 tokens, 8 heads of 128 (49 MB): 24 us; the instructions of the
+// rounding (20 a value) come before the bytes.
 template <int D, int CHUNKS>
 __global__ void __launch_bounds__(128) append_kernel(const __grid_constant__ AppendArgs a) {
   const bn_kv8 &c = a.c;

@@ -25,7 +25,9 @@
 // codes the block that they fill before it reads it: a decode step is one launch. Several groups of rows (more than
 // 32, or 16 with heads of 256) read what an append kernel has written.
 //
-// Figures: at attend_launch.
+// Measured: 64 sequences of up to 8192 tokens, 8 key heads of 128, int8, 637 MB: 171 us, 3.7 TB/s, 57 % of the copy rate;
+// one sequence of 131073, 269 MB: 68 us; one of 300: 12 us in a graph. What bounds the long ones: 64 M warp
+// instructions (410 a piece of 16 keys; 44 % of the issue slots) at 12 warps an SM, fixed-latency waits first.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 

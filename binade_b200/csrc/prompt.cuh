@@ -20,6 +20,10 @@
 // fit its 8 bits) straight into the ring, the open block's tokens as they are. The scales stay apart: K's multiply
 // the scores of their 16 keys or more, V's the weights, before these are rounded.
 //
+// Measured: 8192 tokens, 32 / 8 heads of 128, causal: 477 us at full clocks, 1.15 PFLOP/s, 69 % of the measured cuBLAS
+// rate (552 us under the power cap). Tensor pipe 53 %, ex2's 53 %: a tile's S, softmax, P and O in a row are twice as long as either,
+// and two tiles are what tensor memory holds. Chunk of 2 x 500 tokens over up to 9000, int8: 265 us.
+//
 // Every wait is bounded: a wait that gives up sets the device status, and the block still ends.
 #pragma once
 

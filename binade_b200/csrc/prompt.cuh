@@ -194,6 +194,17 @@ __device__ __forceinline__ bool prompt_wait(uint32_t bar, uint32_t parity) {
 }
 __device__ __forceinline__ bool prompt_wait_warp(uint32_t bar, uint32_t parity) { return __all_sync(BN_FULL, prompt_wait(bar, parity)); }
 
+// True in one lane of the warp, all of which has to get here: ahead of any wait.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t one;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(one));
+  return one != 0;
+}
+
 // Slot s of the launch: document n owns slots floor(offsets[n] Gp / ROWS) + n and on, at least as many as it has
 // tiles, so that no prefix sum over the documents is needed. False: the slot is empty.
 template <int ROWS>

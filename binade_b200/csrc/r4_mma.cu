@@ -66,6 +66,19 @@ __device__ __forceinline__ bool mm_bar_wait(uint32_t bar, uint32_t parity) {
 // The wait of a whole warp: every lane learns when some lane's gave up, so that the warp stays
 // together for what has to be executed by all of it (elect.sync, tcgen05.ld).
 __device__ __forceinline__ bool mm_bar_wait_warp(uint32_t bar, uint32_t parity) { return __all_sync(BN_FULL, mm_bar_wait(bar, parity)); }
+// True in one lane of the warp, all of which has to get here: ahead of any wait. Instructions that
+// a single thread issues (MMAs, commits, bulk copies) take their operands from uniform registers;
+// behind `lane == 0` the compiler has to assume divergent values and wraps each of them in code that
+// makes them uniform.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t one;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(one));
+  return one != 0;
+}
 struct MmaArgs {
   bn_r4 w;
   uint16_t *y;

@@ -32,19 +32,6 @@ __device__ __forceinline__ bool mm_bar_test(uint32_t bar, uint32_t parity) {
       : "memory");
   return ok != 0;
 }
-// True in one lane of the warp, all of which has to get here: ahead of any wait. Instructions that
-// a single thread issues (MMAs, commits, bulk copies) take their operands from uniform registers;
-// behind `lane == 0` the compiler has to assume divergent values and wraps each of them in code that
-// makes them uniform.
-__device__ __forceinline__ bool elect_one() {
-  uint32_t one;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "elect.sync _|p, 0xffffffff;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(one));
-  return one != 0;
-}
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }

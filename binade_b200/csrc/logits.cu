@@ -45,6 +45,12 @@ __device__ __forceinline__ uint32_t four_bits(const uint32_t *__restrict__ words
   return (t & 31) > 28 && hi > lo ? __funnelshift_r(a, b, t & 31) : a >> (t & 31);
 }
 
+// The cluster's barrier in two halves: a block's shared memory may be written from outside once that block is known
+// to run, which its arrival tells. Arriving at the start and waiting before the store hides the barrier behind the pass.
+// (Relaxed: no memory goes with it.)
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.aligned;" ::: "memory"); }
+
 // A cluster of blocks per row: the blocks take pieces of the vocabulary in turn, four tokens a thread, and the
 // first of them joins their choices through distributed shared memory. One launch, whatever the batch: 8 us in a graph for
 // one row of 128256 (the latency of a few loads in a row), 36 us for 64 rows of 151937 fp32 (2.2 TB/s: 130 instructions a
@@ -55,6 +61,7 @@ template <typename T, int THREADS, int U>
 __global__ void __launch_bounds__(THREADS, U == 1 ? 4 : 2) logits_kernel(const __grid_constant__ LogitsArgs a) {
   namespace cg = cooperative_groups;
   cg::cluster_group cluster = cg::this_cluster();
+  cluster_arrive();
   const int64_t b = blockIdx.y;
   const T *const x = reinterpret_cast<const T *>(a.x) + b * a.x_row;
   float *const out = a.out + b * a.out_row;
@@ -148,6 +155,7 @@ __global__ void __launch_bounds__(THREADS, U == 1 ? 4 : 2) logits_kernel(const _
   __shared__ Best warps[32], blocks[16];
   if (lane_id() == 0) warps[threadIdx.x >> 5] = best;
   __syncthreads();
+  cluster_wait();
   if (threadIdx.x < 32) {
     best = threadIdx.x < THREADS / 32 ? warps[threadIdx.x] : Best{-CUDART_INF_F, -1};
 #pragma unroll

@@ -8,14 +8,15 @@
 //                  permute and lose the 1152 by one subtraction; e4m3 converts in hardware
 //   queries        to f16 after a power of two per row that puts its largest value in [1, 2): exact down to
 //                  2^-24 of that value, below which a product does not show in an fp32 sum of scores
-//   scores         K's scale multiplies the sum; V's scale 2^v goes into the exponent: p' = 2^(s + v - m) with m
-//                  near the running maximum of s + v, so p' fits f16 (rounded to 11 bits, 2^-12) however far apart
-//                  the blocks' scales lie, and the sum of weights takes p' / 2^v, in fp32
+//   scores         K's scale multiplies the sum. A weight is p = 2^(s - m), m near the row's largest s, and goes to the sum
+//                  of weights as it is; to the product with V's codes goes p' = p vscale 2^d in f16, d near m less
+//                  the row's largest s + log2(vscale). Two maxima, since either sum must keep what weighs in it however
+//                  far apart the blocks' scales lie: a block of zeros (scale 2^-100) weighs in the first alone
 //   order of k     a dot product may take its dimensions, and the sum over keys its keys, in any order: each
 //                  thread reads 16 neighbouring bytes of a key and calls them the elements that the
 //                  fragments want. V's codes lie four keys at a time, dimension by dimension, since its fragments pair
 //                  keys: a word is one dimension of the thread's four keys
-//   maximum        a row's m moves only when a score passes it by 2^15, the room that f16 leaves above 1: a
+//   maxima         m and d move only when a p or a p' passes 2^15, the room that f16 leaves above 1: a
 //                  vote per 16 keys in place of shuffles and a rescaling of the sums
 // A warp streams its own keys through a cp.async ring of its own: no barrier in the loop; the warps of a block
 // are joined at the end. The work is the tiles of all sequences and heads in a row, cut into equal
@@ -40,7 +41,8 @@ __device__ int g_attend_error;  // 1: tokens were brought that the cache has no 
 __device__ __forceinline__ void kv8_overflow() { atomicExch(&g_attend_error, 1); }
 
 constexpr int WARPS = 4;
-constexpr float HEADROOM = 15.0f;  // weights may reach 2^15
+constexpr float MOST = 15.0f;  // p and p' may reach 2^15
+constexpr float AIM = 0.0f;    // where the largest p' of a row starts, in powers of two
 constexpr float NOTHING = -3.402823466e38f;  // a row's m while no key was visible: finite, so that a masked score less m stays -inf
 
 struct AttendArgs {
@@ -75,7 +77,7 @@ struct Shape {
   static constexpr int RING = WARPS * STAGES * STAGE_BYTES;
   static constexpr int JOIN = WARPS * ROWS * (D + 4) * 4;
   static constexpr int SMEM = RING > JOIN ? RING : JOIN;
-  static constexpr int PART = ROWS * (D + 2);          // floats of a partial result: sums, then maxima and weights
+  static constexpr int PART = ROWS * (D + 3);          // floats of a partial result: sums, then m, d and sums of weights
 };
 
 // Tiles of sequence b: of the blocks that are full before `split` from the first key on, then one of everything behind.
@@ -157,11 +159,11 @@ __device__ __forceinline__ uint32_t v_piece(uint32_t four, uint32_t col) {
   return D == 64 ? col ^ ((four & 1u) | ((four & 2u) << 1)) : col ^ (four & 3u);
 }
 
-// What a warp has so far: sums, running maxima (of s + v, in powers of two) and weights of its lane's rows.
+// What a warp has so far of its lane's rows: sums of p' times codes, m and d (powers of two), sums of p.
 template <int D, int MT>
 struct State {
   float o[MT][Shape<D, MT>::NT][4];
-  float m[MT][2], l[MT][2];
+  float m[MT][2], d[MT][2], l[MT][2];
 };
 
 // What a lane's rows need: positions (-1: no row), the factor from a sum of products to a score, the bias.
@@ -172,20 +174,19 @@ struct Rows {
   int L, prefix;
 };
 
-// What goes with a 16-key piece: its first key, the first key that is not its stage's, K's scale, V's as a power of two and
-// inverted, whether some row does not see all of it.
+// What goes with a 16-key piece: its first key, the first key that is not its stage's, K's scale, V's and that as a power of
+// two, whether some row does not see all of it.
 struct PieceOf16 {
   int key0, end;
-  float scale, vlog, vinv;
+  float scale, vscale, vlog;
   bool masked;
 };
 
 // The scores of P pieces into weights: x holds the raw sums and gets p' (tile j, column 2c + e: key key0 + 4c + 2j + e).
-// Updates the weights' sum; where a score passes a row's m by the headroom, moves m and rescales the sums.
+// Updates the sum of weights; where a p or a p' would pass 2^MOST, moves m and d and rescales the sums.
 template <int D, int MT, int P, bool PLAIN>
 __device__ __forceinline__ void weigh(const AttendArgs &a, float (&x)[P][MT][2][4], const Rows<MT> &r, State<D, MT> &st, const PieceOf16 (&pc)[P]) {
   const int lane_key = 4 * (int)(lane_id() & 3u);
-  float top[MT][2];
 #pragma unroll
   for (int p = 0; p < P; p++) {
     const int first = pc[p].key0 + lane_key;
@@ -199,12 +200,10 @@ __device__ __forceinline__ void weigh(const AttendArgs &a, float (&x)[P][MT][2][
 #pragma unroll
           for (int e = 0; e < 2; e++) {
             float &v = x[p][mt][j][2 * h + e];
-            if constexpr (PLAIN) {
-              v = fmaf(v, f, pc[p].vlog);
-            } else {
-              v *= f;
+            v *= f;
+            if constexpr (!PLAIN) {
               if (a.cap > 0.0f) v = capped(v, a.cap * LOG2E);
-              v = fmaf(-r.slope[mt][h], (float)abs(r.i[mt][h] - (first + 2 * j + e)), v) + pc[p].vlog;
+              v = fmaf(-r.slope[mt][h], (float)abs(r.i[mt][h] - (first + 2 * j + e)), v);
             }
           }
       }
@@ -226,38 +225,44 @@ __device__ __forceinline__ void weigh(const AttendArgs &a, float (&x)[P][MT][2][
         }
     }
   }
+  float top[MT][2], top_v[MT][2];  // largest s and s + log2(vscale)
   bool over = false;
 #pragma unroll
   for (int mt = 0; mt < MT; mt++)
 #pragma unroll
     for (int h = 0; h < 2; h++) {
-      float t = -CUDART_INF_F;
+      top[mt][h] = top_v[mt][h] = -CUDART_INF_F;
 #pragma unroll
-      for (int p = 0; p < P; p++) t = fmaxf(t, fmaxf(fmaxf(x[p][mt][0][2 * h], x[p][mt][0][2 * h + 1]), fmaxf(x[p][mt][1][2 * h], x[p][mt][1][2 * h + 1])));
-      top[mt][h] = t;
-      over |= t > st.m[mt][h] + HEADROOM;
+      for (int p = 0; p < P; p++) {
+        const float t = fmaxf(fmaxf(x[p][mt][0][2 * h], x[p][mt][0][2 * h + 1]), fmaxf(x[p][mt][1][2 * h], x[p][mt][1][2 * h + 1]));
+        top[mt][h] = fmaxf(top[mt][h], t), top_v[mt][h] = fmaxf(top_v[mt][h], t + pc[p].vlog);
+      }
+      over |= top[mt][h] - st.m[mt][h] > MOST || top_v[mt][h] - st.m[mt][h] + st.d[mt][h] > MOST;
     }
   if (__any_sync(BN_FULL, over)) {
 #pragma unroll
     for (int mt = 0; mt < MT; mt++)
 #pragma unroll
       for (int h = 0; h < 2; h++) {
-        float t = top[mt][h];
-        t = fmaxf(t, __shfl_xor_sync(BN_FULL, t, 1));
-        t = fmaxf(t, __shfl_xor_sync(BN_FULL, t, 2));
+        float t = top[mt][h], u = top_v[mt][h];
+        t = fmaxf(t, __shfl_xor_sync(BN_FULL, t, 1)), u = fmaxf(u, __shfl_xor_sync(BN_FULL, u, 1));
+        t = fmaxf(t, __shfl_xor_sync(BN_FULL, t, 2)), u = fmaxf(u, __shfl_xor_sync(BN_FULL, u, 2));
         t = fmaxf(t, st.m[mt][h]);
-        const float keep = ex2(st.m[mt][h] - t);
-        st.m[mt][h] = t, st.l[mt][h] *= keep;
+        const float rise = t - st.m[mt][h], d = floorf(fminf(st.d[mt][h] + rise, AIM - (u - t)));  // (whole: 2^d is exact)
+        const float keep = ex2(-rise), keep_o = ex2(d - st.d[mt][h] - rise);
+        st.m[mt][h] = t, st.d[mt][h] = d, st.l[mt][h] *= keep;
 #pragma unroll
-        for (int n = 0; n < Shape<D, MT>::NT; n++) st.o[mt][n][2 * h] *= keep, st.o[mt][n][2 * h + 1] *= keep;
+        for (int n = 0; n < Shape<D, MT>::NT; n++) st.o[mt][n][2 * h] *= keep_o, st.o[mt][n][2 * h + 1] *= keep_o;
       }
   }
 #pragma unroll
-  for (int p = 0; p < P; p++)
+  for (int mt = 0; mt < MT; mt++)
 #pragma unroll
-    for (int mt = 0; mt < MT; mt++)
+    for (int h = 0; h < 2; h++) {
+      const float to_v = ex2(st.d[mt][h]);
 #pragma unroll
-      for (int h = 0; h < 2; h++) {
+      for (int p = 0; p < P; p++) {
+        const float g = fminf(pc[p].vscale * to_v, 3.0e38f);  // (where the product passes fp32, p is zero)
         float sum = 0.0f;
 #pragma unroll
         for (int j = 0; j < 2; j++)
@@ -266,9 +271,11 @@ __device__ __forceinline__ void weigh(const AttendArgs &a, float (&x)[P][MT][2][
             float &v = x[p][mt][j][2 * h + e];
             v = ex2(v - st.m[mt][h]);
             sum += v;
+            v *= g;
           }
-        st.l[mt][h] = fmaf(sum, pc[p].vinv, st.l[mt][h]);
+        st.l[mt][h] += sum;
       }
+    }
 }
 
 // The dimension of n8 tile t's column n.
@@ -303,7 +310,7 @@ __device__ __noinline__ void append_filled(const AttendArgs &a, int64_t b, int h
 }
 
 // The open block's 16 tokens from `key0` on, in BF16. Weights go in two BF16 halves (hi + lo: 2^-17), values times 2^-23
-// with 2^23 in the weights' exponent, so that no sum of 63 of them passes fp32. Where a value is not finite, a
+// with 2^23 as V's scale, so that no sum of 63 of them passes fp32. Where a value is not finite, a
 // weight of zero must not touch it: those go one by one.
 template <int D, int MT, bool PLAIN>
 __device__ void open_block(const AttendArgs &a, const uint16_t *const (&qrow)[MT][2], const OpenRows &rows, int L, int key0, const Rows<MT> &r, State<D, MT> &st) {
@@ -332,7 +339,7 @@ __device__ void open_block(const AttendArgs &a, const uint16_t *const (&qrow)[MT
   Rows<MT> plain = r;  // the queries as they are: no power of two in the factor
 #pragma unroll
   for (int mt = 0; mt < MT; mt++) plain.factor[mt][0] = plain.factor[mt][1] = a.cap > 0.0f ? a.scale * (2.0f * LOG2E / a.cap) : a.scale * LOG2E;
-  const PieceOf16 piece[1] = {{key0, L, 1.0f, 23.0f, 1.0f / (1 << 23), true}};
+  const PieceOf16 piece[1] = {{key0, L, 1.0f, (float)(1 << 23), 23.0f, true}};
   weigh<D, MT, 1, PLAIN>(a, x1, plain, st, piece);
   uint32_t hi[MT][4], lo[MT][4];
 #pragma unroll
@@ -395,6 +402,12 @@ __device__ void open_block(const AttendArgs &a, const uint16_t *const (&qrow)[MT
   }
 }
 
+// Four outputs of a row: sums of p' times codes by the sum of weights, without the 2^d that p' has more than p.
+__device__ __forceinline__ uint2 quotients(float4 o, float l, float d) {
+  const float inv = 1.0f / l, back = ex2(-d);  // (o / l first: it is never small where back is)
+  return make_uint2(pack_bf16(o.x * inv * back, o.y * inv * back), pack_bf16(o.z * inv * back, o.w * inv * back));
+}
+
 // The parts of one sequence and head together, by the block that finished last: four dimensions a thread, sixteen parts
 // at a time. Parts lie in the workspace, two slots a block of the grid; late: the first part is in its block's second slot.
 template <int D, int MT>
@@ -403,35 +416,39 @@ __device__ __noinline__ void join_parts(const AttendArgs &a, int64_t b, int kv, 
   constexpr int U = 16;
   for (int i = (int)threadIdx.x; i < rows * (D / 4); i += WARPS * 32) {
     const int row = i / (D / 4), col = i % (D / 4) * 4;
-    float m = NOTHING, l = 0.0f;
+    float m = NOTHING, d = 0.0f, l = 0.0f;
     float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     for (int p0 = 0; p0 < parts; p0 += U) {
-      float pm[U], pl[U];
+      float pm[U], pd[U], pl[U];
       float4 v[U];
 #pragma unroll
       for (int u = 0; u < U; u++) {
         const int p = min(p0 + u, parts - 1);
         const float *const part = a.parts + ((first + p) * 2 + (p == 0 && late ? 1 : 0)) * S::PART;
-        pm[u] = __ldcg(part + S::ROWS * D + row), pl[u] = __ldcg(part + S::ROWS * D + S::ROWS + row);
+        pm[u] = __ldcg(part + S::ROWS * D + row), pd[u] = __ldcg(part + S::ROWS * (D + 1) + row), pl[u] = __ldcg(part + S::ROWS * (D + 2) + row);
         v[u] = __ldcg(reinterpret_cast<const float4 *>(part + row * D + col));
       }
       float top = m;
 #pragma unroll
       for (int u = 0; u < U; u++) top = fmaxf(top, pm[u]);
-      const float keep = ex2(m - top);
-      m = top, l *= keep, o.x *= keep, o.y *= keep, o.z *= keep, o.w *= keep;
+      const float had = (top - m) + d;
+      d = had;
+#pragma unroll
+      for (int u = 0; u < U; u++) pd[u] += top - pm[u], d = fminf(d, pd[u]);  // (a part that stands for several here counts once)
+      const float keep = ex2(d - had);
+      l *= ex2(m - top), o.x *= keep, o.y *= keep, o.z *= keep, o.w *= keep;
+      m = top;
 #pragma unroll
       for (int u = 0; u < U; u++) {
         if (p0 + u >= parts) break;
-        const float f = ex2(pm[u] - top);
-        l = fmaf(f, pl[u], l);
+        const float f = ex2(d - pd[u]);
+        l = fmaf(ex2(pm[u] - top), pl[u], l);
         o.x = fmaf(f, v[u].x, o.x), o.y = fmaf(f, v[u].y, o.y), o.z = fmaf(f, v[u].z, o.z), o.w = fmaf(f, v[u].w, o.w);
       }
     }
     const int t = row / a.group, head = kv * a.group + row % a.group;
     uint16_t *const out = a.out + b * a.o_seq + t * a.o_token + head * a.o_head + col;
-    const float inv = 1.0f / l;
-    if (t < brought) *reinterpret_cast<uint2 *>(out) = make_uint2(pack_bf16(o.x * inv, o.y * inv), pack_bf16(o.z * inv, o.w * inv));
+    if (t < brought) *reinterpret_cast<uint2 *>(out) = quotients(o, l, d);
     else if (a.zero_rest) *reinterpret_cast<uint2 *>(out) = make_uint2(0, 0);
   }
 }
@@ -444,7 +461,7 @@ __global__ void __launch_bounds__(WARPS * 32, (D == 64 && MT == 1) ? 4 : (MT * D
   __shared__ int64_t found[2];
   __shared__ int64_t warp_tiles[WARPS];
   __shared__ bool last_ticket;
-  __shared__ float join_m[WARPS][S::ROWS], join_l[WARPS][S::ROWS];
+  __shared__ float join_m[WARPS][S::ROWS], join_d[WARPS][S::ROWS], join_l[WARPS][S::ROWS];
   __shared__ float scales[WARPS][S::STAGES][2][S::KS / 16];
   const uint32_t lane = lane_id(), warp = threadIdx.x >> 5, n = lane >> 2, c = lane & 3u;
   const bn_kv8 &cache = a.c;
@@ -580,7 +597,7 @@ __global__ void __launch_bounds__(WARPS * 32, (D == 64 && MT == 1) ? 4 : (MT * D
         qrow[mt][h] = real ? a.q + b * a.q_seq + t * a.q_token + head * a.q_head : nullptr;
         r.i[mt][h] = real ? s.held + t : -1;
         r.slope[mt][h] = real && a.slopes ? a.slopes[head] * LOG2E : 0.0f;
-        st.m[mt][h] = NOTHING, st.l[mt][h] = 0.0f;
+        st.m[mt][h] = NOTHING, st.d[mt][h] = st.l[mt][h] = 0.0f;
         uint32_t most = 0;
 #pragma unroll
         for (int g = 0; g < D / 64; g++)
@@ -646,7 +663,7 @@ __global__ void __launch_bounds__(WARPS * 32, (D == 64 && MT == 1) ? 4 : (MT * D
           float vlog;
           asm("lg2.approx.f32 %0, %1;" : "=f"(vlog) : "f"(vscale));
           const int key0 = first + 16 * sub;
-          piece[sub] = {key0, end, scales[warp][slot][0][sub], vlog, __fdividef(1.0f, vscale), key0 < lo_most || key0 + 16 > min(hi_least, end)};
+          piece[sub] = {key0, end, scales[warp][slot][0][sub], vscale, vlog, key0 < lo_most || key0 + 16 > min(hi_least, end)};
         }
         weigh<D, MT, P, PLAIN>(a, x, r, st, piece);
 #pragma unroll
@@ -694,7 +711,7 @@ __global__ void __launch_bounds__(WARPS * 32, (D == 64 && MT == 1) ? 4 : (MT * D
         l += __shfl_xor_sync(BN_FULL, l, 1);
         l += __shfl_xor_sync(BN_FULL, l, 2);
         const int row = 16 * mt + 8 * h + (int)n;
-        if (c == 0) join_m[warp][row] = st.m[mt][h], join_l[warp][row] = l;
+        if (c == 0) join_m[warp][row] = st.m[mt][h], join_d[warp][row] = st.d[mt][h], join_l[warp][row] = l;
         float *const to = join + (warp * S::ROWS + row) * (D + 4);
         constexpr int RUN = D == 64 ? 8 : 16;  // neighbouring dimensions of a column
 #pragma unroll
@@ -710,24 +727,26 @@ __global__ void __launch_bounds__(WARPS * 32, (D == 64 && MT == 1) ? 4 : (MT * D
       float m = join_m[0][row], l = 0.0f, o[4] = {};
 #pragma unroll
       for (int w = 1; w < WARPS; w++) m = fmaxf(m, join_m[w][row]);
+      float d = (m - join_m[0][row]) + join_d[0][row];
+#pragma unroll
+      for (int w = 1; w < WARPS; w++) d = fminf(d, (m - join_m[w][row]) + join_d[w][row]);
 #pragma unroll
       for (int w = 0; w < WARPS; w++) {
-        const float f = ex2(join_m[w][row] - m);
+        const float f = ex2(d - ((m - join_m[w][row]) + join_d[w][row]));
         const float4 v = *reinterpret_cast<const float4 *>(join + (w * S::ROWS + row) * (D + 4) + col);
-        l = fmaf(f, join_l[w][row], l);
+        l = fmaf(ex2(join_m[w][row] - m), join_l[w][row], l);
         o[0] = fmaf(f, v.x, o[0]), o[1] = fmaf(f, v.y, o[1]), o[2] = fmaf(f, v.z, o[2]), o[3] = fmaf(f, v.w, o[3]);
       }
       if (whole) {
         const int t = (row0 + row) / a.group, head = kv * a.group + (row0 + row) % a.group;
         if (t < s.brought) {
-          const float inv = 1.0f / l;
-          *reinterpret_cast<uint2 *>(a.out + b * a.o_seq + t * a.o_token + head * a.o_head + col) = make_uint2(pack_bf16(o[0] * inv, o[1] * inv), pack_bf16(o[2] * inv, o[3] * inv));
+          *reinterpret_cast<uint2 *>(a.out + b * a.o_seq + t * a.o_token + head * a.o_head + col) = quotients(make_float4(o[0], o[1], o[2], o[3]), l, d);
         } else if (a.zero_rest) {
           *reinterpret_cast<uint2 *>(a.out + b * a.o_seq + t * a.o_token + head * a.o_head + col) = make_uint2(0, 0);
         }
       } else {
         *reinterpret_cast<float4 *>(part + row * D + col) = make_float4(o[0], o[1], o[2], o[3]);
-        if (col == 0) part[S::ROWS * D + row] = m, part[S::ROWS * D + S::ROWS + row] = l;
+        if (col == 0) part[S::ROWS * D + row] = m, part[S::ROWS * (D + 1) + row] = d, part[S::ROWS * (D + 2) + row] = l;
       }
     }
     if (!whole && a.join_here) {  // the last block of this sequence and head joins
@@ -763,7 +782,7 @@ template <int D, int MT>
 __global__ void __launch_bounds__(JOIN_THREADS) join_kernel(const __grid_constant__ AttendArgs a) {
   using S = Shape<D, MT>;
   constexpr int COLS = D / 4, GROUPS = JOIN_THREADS / COLS;
-  __shared__ float tops[JOIN_THREADS / 32], weights[16];
+  __shared__ float tops[JOIN_THREADS / 32], least[JOIN_THREADS / 32], weights[16];
   __shared__ float4 sums[JOIN_THREADS];
   const int all_rows = a.group * a.tokens, per_seq = (int)a.c.kv_heads * a.row_groups;
   const int unit = (int)(blockIdx.x / (unsigned)all_rows), r = (int)(blockIdx.x % (unsigned)all_rows);
@@ -791,15 +810,23 @@ __global__ void __launch_bounds__(JOIN_THREADS) join_kernel(const __grid_constan
   __syncthreads();
 #pragma unroll
   for (int w = 0; w < JOIN_THREADS / 32; w++) m = fmaxf(m, tops[w]);
+  float d = CUDART_INF_F;
+  for (int p = (int)threadIdx.x; p < parts; p += JOIN_THREADS) d = fminf(d, (m - part_of(p)[S::ROWS * D + row]) + part_of(p)[S::ROWS * (D + 1) + row]);
+#pragma unroll
+  for (int k = 16; k; k >>= 1) d = fminf(d, __shfl_xor_sync(BN_FULL, d, k));
+  if (lane_id() == 0) least[threadIdx.x >> 5] = d;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < JOIN_THREADS / 32; w++) d = fminf(d, least[w]);
   const int g = (int)threadIdx.x / COLS, col = (int)threadIdx.x % COLS * 4;
   float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   float l = 0.0f;
 #pragma unroll 4
   for (int p = g; p < parts; p += GROUPS) {
     const float *const part = part_of(p);
-    const float f = ex2(part[S::ROWS * D + row] - m);
+    const float pm = part[S::ROWS * D + row], f = ex2(d - ((m - pm) + part[S::ROWS * (D + 1) + row]));
     const float4 v = *reinterpret_cast<const float4 *>(part + row * D + col);
-    l = fmaf(f, part[S::ROWS * D + S::ROWS + row], l);
+    l = fmaf(ex2(pm - m), part[S::ROWS * (D + 2) + row], l);
     o.x = fmaf(f, v.x, o.x), o.y = fmaf(f, v.y, o.y), o.z = fmaf(f, v.z, o.z), o.w = fmaf(f, v.w, o.w);
   }
   sums[threadIdx.x] = o;
@@ -814,8 +841,7 @@ __global__ void __launch_bounds__(JOIN_THREADS) join_kernel(const __grid_constan
   int held, brought;
   kv8_tokens(a.c, a.counts, a.tokens, b, held, brought);
   if (t < brought) {
-    const float inv = 1.0f / l;
-    *reinterpret_cast<uint2 *>(out + col) = make_uint2(pack_bf16(o.x * inv, o.y * inv), pack_bf16(o.z * inv, o.w * inv));
+    *reinterpret_cast<uint2 *>(out + col) = quotients(o, l, d);
   } else if (a.zero_rest) {
     *reinterpret_cast<uint2 *>(out + col) = make_uint2(0, 0);
   }
@@ -849,7 +875,7 @@ Plan plan_of(const bn_kv8 *c, int64_t tokens, int64_t heads) {
   // 6 parts at most: 12.4 / 14.4; 131073 tokens, 55 parts: 82 / 70).
   p.join_here = p.row_groups == 1 && p.blocks <= 8 * c->batch * c->kv_heads;
   p.plan_bytes = ((uint64_t)(c->batch + 2) * 8 + 127) / 128 * 128;
-  p.bytes = p.plan_bytes + (uint64_t)p.blocks * 2 * (16 * p.mt * (D + 2)) * 4;
+  p.bytes = p.plan_bytes + (uint64_t)p.blocks * 2 * (16 * p.mt * (D + 3)) * 4;
   return p;
 }
 Plan plan_of(const bn_kv8 *c, int64_t tokens, int64_t heads) { return c->D == 64 ? plan_of<64>(c, tokens, heads) : c->D == 128 ? plan_of<128>(c, tokens, heads) : plan_of<256>(c, tokens, heads); }

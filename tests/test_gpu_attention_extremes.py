@@ -1,0 +1,78 @@
+"""Attention at the ends of its range: blocks of zeros, sinks, infinities beside masked NaN, caps of all sizes, rows that torch
+calls contiguous whatever their stride. Against the definition in 64 bits (attention_reference.py)."""
+
+import math
+
+import pytest
+import torch
+
+import attention_reference as ref
+from test_gpu_attention import close, gen, normal
+
+pytestmark = pytest.mark.gpu
+
+
+def constant(n, kv, D, value):
+    return torch.full((n, kv, D), float(value), dtype=torch.bfloat16, device="cuda")
+
+
+def check_decode(keys, values, heads, kind, block, new=1, batch=1, **options):
+    """keys, values [L, kv, D]: all but the last `new` tokens are held; queries of ones (with scale = 1 / D a
+    key's score is its mean) against the definition."""
+    from binade_b200.cuda.attention import KV8Cache
+
+    L, kv, D = keys.shape
+    cache = KV8Cache(1, batch, kv, D, L, kind=kind, block=block)
+    held = L - new
+    many = lambda x: x[None].expand(batch, -1, -1, -1)  # noqa: E731
+    if held:
+        cache.append(0, many(keys[:held]), many(values[:held]))
+        cache.advance(held)
+    q = torch.ones((batch, new, heads, D), dtype=torch.bfloat16, device="cuda")
+    got = cache.attend(0, q, many(keys[held:]), many(values[held:]), scale=1.0 / D, **options)
+    want, bound = ref.attend(q[0], ref.stored(keys, kind, block), ref.stored(values, kind, block), held, scale=1.0 / D, **options)
+    for b in range(batch):
+        close(got[b], want, bound)
+
+
+# ------------------------------------------------------------------------- values whose scales lie far apart
+@pytest.mark.parametrize("kind", ["int8", "e4m3"])
+@pytest.mark.parametrize("D,heads,kv,block", [(64, 4, 1, 16), (128, 8, 2, 32), (256, 2, 1, 64)])
+@pytest.mark.parametrize("gap", [-20, -4, 0, 2, 3, 4, 8, 12, 20])
+def test_decode_over_blocks_of_zero_values(kind, D, heads, kv, block, gap):
+    """Keys of weight whose values are all zero stay in the sum of weights: before an open block, before, between and
+    behind stored blocks, in one warp and in four, whole and cut into parts."""
+    zeros, one = (lambda n: constant(n, kv, D, 0)), (lambda n: constant(n, kv, D, 1))
+    for held, new in ((block, 1), (128, 1), (128, 3), (640, 2), (6000 // block * block, 1)):
+        check_decode(torch.cat([zeros(held), constant(new, kv, D, gap)]), torch.cat([zeros(held), one(new)]), heads, kind, block, new=new)
+    for before, behind in ((128, 0), (0, 256), (320, 704), (4096, 4096)):
+        keys = torch.cat([zeros(before), constant(block, kv, D, gap), zeros(behind + 1)])
+        values = torch.cat([zeros(before), one(block), zeros(behind + 1)])
+        check_decode(keys, values, heads, kind, block)
+        check_decode(keys, values, heads, kind, block, softcap=30.0)
+
+
+@pytest.mark.parametrize("kind", ["int8", "e4m3"])
+def test_decode_over_blocks_of_zero_values_in_many_parts_and_batches(kind):
+    zeros = lambda n: constant(n, 8, 128, 0)  # noqa: E731
+    for L, batch in ((70_016, 1), (2048, 3), (500, 40)):
+        for gap in (-3, 3, 9, 15):
+            keys = torch.cat([zeros(L), constant(2, 8, 128, gap)])
+            values = torch.cat([zeros(L), constant(2, 8, 128, -2)])
+            check_decode(keys, values, 32, kind, 32, new=1, batch=batch)
+            keys[L // 64 * 32 : L // 64 * 32 + 32] = gap - 2
+            values[L // 64 * 32 : L // 64 * 32 + 32] = 3
+            check_decode(keys, values, 32, kind, 32, new=2, batch=batch)
+
+
+@pytest.mark.parametrize("kind", ["int8", "e4m3"])
+@pytest.mark.parametrize("D,heads,kv", [(64, 4, 2), (128, 12, 1), (256, 4, 1)])
+def test_decode_values_from_the_smallest_to_the_largest(kind, D, heads, kv):
+    """Neighbouring blocks of values from 1e-30 to 1e30 with scores that make up for the difference, or do not."""
+    g = gen(70)
+    for slope in (0.0, -1.0, 1.0):  # nats a factor of e
+        keys, values = [], []
+        for e in (0, -30, 20, -10, 30, 5, -20, 10, -5, 25):
+            keys.append(constant(32, kv, D, slope * e * math.log(10)))
+            values.append((normal((32, kv, D), g).float() * 10.0**e).to(torch.bfloat16))
+        check_decode(torch.cat(keys + [constant(3, kv, D, 0)]), torch.cat(values + [normal((3, kv, D), g)]), heads, kind, 16, new=2)

@@ -16,8 +16,11 @@
 //                  thread reads 16 neighbouring bytes of a key and calls them the elements that the
 //                  fragments want. V's codes lie four keys at a time, dimension by dimension, since its fragments pair
 //                  keys: a word is one dimension of the thread's four keys
-//   maxima         m and d move only when a p or a p' passes 2^15, the room that f16 leaves above 1: a
-//                  vote per 16 keys in place of shuffles and a rescaling of the sums
+//   rounding       of p' to f16, 2^-11 of it. A row's largest p' starts in 2^12 .. 2^13, so that this holds down to 2^-26 of the
+//                  largest, and what is below 2^-37 of it is zero: where one key takes nearly all the weight and has no value,
+//                  the others are the output
+//   maxima         m and d move only when a p or a p' passes 2^15 (f16 ends at 2^16): a vote per 16 keys
+//                  in place of shuffles and a rescaling of the sums
 // A warp streams its own keys through a cp.async ring of its own: no barrier in the loop; the warps of a block
 // are joined at the end. The work is the tiles of all sequences and heads in a row, cut into equal
 // shares: sequences of unequal lengths load the SMs alike, and one long one spreads over all of them. A sequence and head
@@ -42,7 +45,7 @@ __device__ __forceinline__ void kv8_overflow() { atomicExch(&g_attend_error, 1);
 
 constexpr int WARPS = 4;
 constexpr float MOST = 15.0f;  // p and p' may reach 2^15
-constexpr float AIM = 0.0f;    // where the largest p' of a row starts, in powers of two
+constexpr float AIM = 13.0f;   // where a row's largest p' starts, in powers of two: that leaves 26 below it before f16 loses bits
 constexpr float NOTHING = -3.402823466e38f;  // a row's m while no key was visible: finite, so that a masked score less m stays -inf
 
 struct AttendArgs {

@@ -76,3 +76,17 @@ def test_decode_values_from_the_smallest_to_the_largest(kind, D, heads, kv):
             keys.append(constant(32, kv, D, slope * e * math.log(10)))
             values.append((normal((32, kv, D), g).float() * 10.0**e).to(torch.bfloat16))
         check_decode(torch.cat(keys + [constant(3, kv, D, 0)]), torch.cat(values + [normal((3, kv, D), g)]), heads, kind, 16, new=2)
+
+
+@pytest.mark.parametrize("kind", ["int8", "e4m3"])
+@pytest.mark.parametrize("D,heads,kv,L", [(64, 4, 1, 4100), (128, 4, 1, 9001), (128, 24, 1, 4100), (256, 4, 2, 4100), (128, 4, 1, 300)])
+@pytest.mark.parametrize("gap", [6.0, 12.0, 17.0, 18.0])
+def test_decode_behind_a_sink(kind, D, heads, kv, L, gap):
+    """The first key takes nearly all the weight and has no value: what the others add up to is the output."""
+    g = gen(71)
+    keys, values = normal((L, kv, D), g, 0.5), (normal((L, kv, D), g) + 1).to(torch.bfloat16)
+    keys[0], values[0] = gap, 0
+    for block in (16, 64):
+        check_decode(keys, values, heads, kind, block)
+    order = torch.arange(L, device="cuda").roll(L // 2)  # and in the middle
+    check_decode(keys[order], values[order], heads, kind, 32)

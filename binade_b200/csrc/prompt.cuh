@@ -52,6 +52,7 @@ struct PromptArgs {
   int64_t q_seq, o_seq;
 };
 
+constexpr float NOTHING = -3.402823466e38f;  // m before the first visible key: finite, so that -inf (a masked score, or a key's own) less m stays that
 constexpr int FROM_BF16 = -1;  // SRC: where keys and values come from; else the kind of a cache's codes
 
 template <int E>
@@ -101,7 +102,7 @@ __device__ __noinline__ void attend_row(const PromptArgs &a, const Piece &p, int
   const int full = SRC == FROM_BF16 ? 0 : p.L / a.c.block * a.c.block, slot = SRC == FROM_BF16 ? 0 : kv8_slot(a.c, p.b, p.held, p.L / a.c.block);
   int lo, hi;
   visible_keys(i, p.L, p.prefix, a.window, a.causal, lo, hi);
-  float q[E], o[E] = {}, m = -CUDART_INF_F, l = 0.0f;
+  float q[E], o[E] = {}, m = NOTHING, l = 0.0f;
   load_row<E>(a.q + p.b * a.q_seq + (p.from + t) * a.q_token + head * a.q_head + lane * E, q);
   const float slope = a.slopes ? a.slopes[head] * LOG2E : 0.0f;
   auto row = [&](bool values, int j, float (&x)[E]) {
@@ -157,7 +158,6 @@ __device__ __forceinline__ void fewer_registers() {
 }
 constexpr uint32_t PROMPT_SPINS = 1u << 22;
 constexpr float RISE = 8.0f;                   // how far, in powers of two, a row's maximum may pass m
-constexpr float NOTHING = -3.402823466e38f;    // m before the first visible key: finite, so that a masked score less m stays -inf
 
 template <int D>
 struct Tiles {

@@ -90,3 +90,29 @@ def test_decode_behind_a_sink(kind, D, heads, kv, L, gap):
         check_decode(keys, values, heads, kind, block)
     order = torch.arange(L, device="cuda").roll(L // 2)  # and in the middle
     check_decode(keys[order], values[order], heads, kind, 32)
+
+
+# ------------------------------------------------------------------------- rows that are computed again
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("softcap", [None, 20.0])
+def test_a_score_of_minus_infinity_beside_masked_values_that_are_not_finite(D, softcap):
+    """The first visible key has weight 0 whatever a key that is not seen holds."""
+    from binade_b200.cuda.attention import KV8Cache, attention
+
+    g = gen(72)
+    T = 60
+    q, k, v = normal((T, 24, D), g).abs() + 0.5, normal((T, 8, D), g), normal((T, 8, D), g)
+    q = q.to(torch.bfloat16)
+    k[0, :, 3] = -math.inf
+    want, bound = ref.attend(q, k, v, softcap=softcap)
+    first = 0 if softcap else 1  # (alone, that key has no weight to give; a cap makes its score finite)
+    clean = v.clone()
+    v[T - 1, :, 5], v[T - 1, :, D - 2] = math.nan, math.inf
+    got = attention(q, k, v, softcap=softcap)
+    close(got[first : T - 1], want[first : T - 1], bound[first : T - 1])
+    close(attention(q, k, clean, softcap=softcap)[first:], want[first:], bound[first:])
+    for batch in (1, 6):  # few rows a key head at a time, and many
+        cache = KV8Cache(1, batch, 8, D, 64, block=64)
+        got = cache.attend(0, *(x[None].expand(batch, -1, -1, -1).contiguous() for x in (q, k, v)), softcap=softcap)
+        for b in range(batch):
+            close(got[b, first : T - 1], want[first : T - 1], bound[first : T - 1])

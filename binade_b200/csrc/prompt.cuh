@@ -92,9 +92,10 @@ struct Piece {
 };
 
 // One query of one head by a warp, keys one after the other; a lane has E = D / 32 neighbouring dimensions.
-// Two passes, so that the values are weighted by shares of one: no sum of theirs can pass the largest of them.
+// Two passes, so that the values are weighted by shares of one: no sum of theirs can pass the largest of them. Writes
+// dimensions from .. to - 1, which are the calling warp's: the row's other half may be another's.
 template <int D, int SRC>
-__device__ __noinline__ void attend_row(const PromptArgs &a, const Piece &p, int t, int head) {
+__device__ __noinline__ void attend_row(const PromptArgs &a, const Piece &p, int t, int head, int from, int to) {
   constexpr int E = D / 32;
   const uint32_t lane = lane_id();
   const int kv = head / (a.heads / a.kv_heads), i = p.held + t;
@@ -134,6 +135,7 @@ __device__ __noinline__ void attend_row(const PromptArgs &a, const Piece &p, int
     for (int e = 0; e < E; e++) o[e] = fmaf(w, x[e], o[e]);
   }
   uint16_t *const out = a.out + p.b * a.o_seq + (p.from + t) * a.o_token + head * a.o_head + lane * E;
+  if ((int)lane * E < from || (int)lane * E >= to) return;
 #pragma unroll
   for (int e = 0; e < E; e++) out[e] = f32_to_bf16_bits(o[e]);
 }
@@ -755,9 +757,11 @@ __global__ void __launch_bounds__(Roles<SRC>::WARPS * 32, 1) prompt_kernel(const
             if (real) *reinterpret_cast<uint4 *>(out + x + e) = make_uint4(w[0], w[1], w[2], w[3]);
           }
         }
-        for (uint32_t again = __ballot_sync(BN_FULL, odd && real); again; again &= again - 1) {
+        uint32_t again = __ballot_sync(BN_FULL, odd && real);
+        __syncwarp();  // what is written again comes behind what the row's own lane wrote
+        for (; again; again &= again - 1) {
           const int other_row = p.row0 + 128 * i + (int)(warp & 3) * 32 + __ffs((int)again) - 1;
-          attend_row<D, SRC>(a, p, other_row >> group_log2, head0 + (other_row & (group - 1)));
+          attend_row<D, SRC>(a, p, other_row >> group_log2, head0 + (other_row & (group - 1)), part * OD, part * OD + OD);
         }
       }
     }

@@ -116,3 +116,18 @@ def test_a_score_of_minus_infinity_beside_masked_values_that_are_not_finite(D, s
         got = cache.attend(0, *(x[None].expand(batch, -1, -1, -1).contiguous() for x in (q, k, v)), softcap=softcap)
         for b in range(batch):
             close(got[b, first : T - 1], want[first : T - 1], bound[first : T - 1])
+
+
+def test_rows_computed_again_repeat_bit_for_bit():
+    """Heads of 256: the halves of a row belong to two warps, and a masked infinity may show to one of them alone."""
+    from binade_b200.cuda.attention import attention
+
+    g = gen(73)
+    T = 700
+    q, k, v = normal((T, 4, 256), g), normal((T, 2, 256), g), normal((T, 2, 256), g)
+    want, bound = ref.attend(q, k, v)
+    v[T - 1, 0, 5], v[T - 1, 1, 200] = math.inf, math.nan
+    first = attention(q, k, v)
+    close(first[: T - 1], want[: T - 1], bound[: T - 1])
+    for _ in range(50):
+        assert torch.equal(first[: T - 1], attention(q, k, v)[: T - 1])

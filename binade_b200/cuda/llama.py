@@ -302,6 +302,8 @@ class Decoder(nn.Module):
             side = torch.cuda.Stream()
             side.wait_stream(torch.cuda.current_stream())
             with torch.cuda.stream(side):
+                if self.cache is not None:
+                    self.reset()  # the last generation may have filled the cache: the warm-up needs room for a token
                 one()  # warm-up outside capture (also sets up lazy state)
                 side.synchronize()
                 pos.zero_()

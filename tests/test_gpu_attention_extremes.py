@@ -12,6 +12,16 @@ from test_gpu_attention import close, gen, normal
 pytestmark = pytest.mark.gpu
 
 
+def status():
+    import ctypes
+
+    from binade_b200 import _native
+
+    st = ctypes.c_int(-1)
+    _native.call("cuda", "bn_device_status", ctypes.byref(st))
+    return st.value
+
+
 def constant(n, kv, D, value):
     return torch.full((n, kv, D), float(value), dtype=torch.bfloat16, device="cuda")
 

@@ -105,6 +105,7 @@ class PushGather:
     back to the library collective)."""
 
     HEADER = 256
+    NO_WAIT = 0xF << 24  # bits of the device status that tell of no wait: tokens that a key/value cache did not take
 
     def __init__(self, group=None, max_bytes: int = 1 << 20):
         import ctypes
@@ -141,7 +142,7 @@ class PushGather:
 
         st = ctypes.c_int(0)
         _native.call("cuda", "bn_device_status", ctypes.byref(st))
-        flag = torch.tensor([st.value], device=self.out.device, dtype=torch.int32)
+        flag = torch.tensor([st.value & ~self.NO_WAIT], device=self.out.device, dtype=torch.int32)
         dist.all_reduce(flag, op=dist.ReduceOp.MAX, group=self.group)
         if int(flag.item()):
             self.dead = True

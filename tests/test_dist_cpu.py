@@ -195,3 +195,33 @@ def test_expert_parallel_two_gloo_ranks(tmp_path):
     for r in range(world):
         mine = slice(r * x.shape[0] // world, (r + 1) * x.shape[0] // world)
         assert torch.equal(torch.load(tmp_path / f"y{r}.pt"), want[mine]), r
+
+
+def test_exchange_is_retired_for_lost_waits_only(monkeypatch):
+    """What a key/value cache had no room for (bits 24..27 of the device status) is no lost exchange."""
+    import torch.distributed as dist
+
+    from binade_b200 import _native
+
+    state = {"status": 0, "resets": 0}
+
+    def call(which, name, *args):
+        if name == "bn_device_status":
+            args[0]._obj.value = state["status"]
+        else:
+            assert name == "bn_device_status_reset"
+            state["resets"] += 1
+
+    monkeypatch.setattr(_native, "call", call)
+    monkeypatch.setattr(dist, "all_reduce", lambda *a, **k: None)
+    ex = bd.PushGather.__new__(bd.PushGather)
+    ex.out, ex.group, ex.dead = torch.zeros(1), None, False
+    for harmless in (0, 1 << 24, 2 << 24, 3 << 24):
+        state["status"] = harmless
+        ex.check()
+        assert not ex.dead and state["resets"] == 0
+    for lost in (1, 4, 1 << 8, 1 << 16, 1 << 28, 2 << 28, 1 << 24 | 1 << 16):
+        ex.dead, state["status"], state["resets"] = False, lost, 0
+        with pytest.raises(RuntimeError, match="retired"):
+            ex.check()
+        assert ex.dead and state["resets"] == 1

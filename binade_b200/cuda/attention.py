@@ -35,7 +35,10 @@ def _rows(t: torch.Tensor, name: str, dims: int, device, apart: bool = False):
     if t.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{name} asks for a gradient: attention here has none (use torch.no_grad)")
     if t.is_contiguous() and t.data_ptr() % 16 == 0:
-        return t, t.stride()[:-1]
+        steps, bits = t.stride()[:-1], 0
+        for step in steps:
+            bits |= step
+        return t, _steps(t) if bits & 7 else steps  # (of a dimension of one element torch takes any stride for contiguous)
     steps = _steps(t)
     fits = t.stride(-1) == 1 and t.data_ptr() % 16 == 0
     for s, n in zip(steps, t.shape):

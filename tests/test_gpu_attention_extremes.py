@@ -141,3 +141,28 @@ def test_rows_computed_again_repeat_bit_for_bit():
     close(first[: T - 1], want[: T - 1], bound[: T - 1])
     for _ in range(50):
         assert torch.equal(first[: T - 1], attention(q, k, v)[: T - 1])
+
+
+# ------------------------------------------------------------------------- strides
+def test_one_token_of_rows_with_an_odd_stride():
+    """torch calls a tensor contiguous whatever the stride of a dimension of one element."""
+    from binade_b200.cuda.attention import KV8Cache, attention
+
+    g = gen(76)
+    wide = normal((5, 260), g)
+    x = wide[:, :256].unflatten(1, (2, 128))
+    for n in (1, 2, 5):
+        got = attention(x[:n], x[:n], x[:n])
+        want, bound = ref.attend(x[:n], x[:n], x[:n])
+        close(got, want, bound)
+    for first in (x[:1], x[2:3]):
+        cache = KV8Cache(1, 1, 2, 128, 64)
+        new = first[None]
+        got = cache.attend(0, new, new, new)
+        assert torch.equal(got[0], first)
+    one = x[:5, None]  # [5, 1, 2, 128]: a batch of single tokens, copied
+    cache = KV8Cache(1, 5, 2, 128, 64)
+    assert torch.equal(cache.attend(0, one, one, one), one)
+    out = torch.empty((1, 260), dtype=torch.bfloat16, device="cuda")[:, :256].unflatten(1, (2, 128))
+    attention(x[:1], x[:1], x[:1], out=out)
+    assert torch.equal(out, x[:1])

@@ -91,8 +91,9 @@ _score_structs: dict = {}  # bn_scores of calls without slopes, by their options
 def _scores(dim: int, heads: int, device, scale, softcap, window, slopes, causal):
     """The bn_scores of a call, and the slopes that it points at."""
     options = (dim, scale, softcap, window, causal)
-    if slopes is None and options in _score_structs:
-        return _score_structs[options], None
+    made = _score_structs.get(options) if slopes is None else None  # (one look: another thread may clear the table)
+    if made is not None:
+        return made, None
     if softcap is not None and not (softcap > 0 and math.isfinite(softcap)):
         raise ValueError("softcap has to be a positive number")
     if window is not None and not 1 <= window < 1 << 30:

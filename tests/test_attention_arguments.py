@@ -3,7 +3,7 @@ number is -1)."""
 
 import torch
 
-from binade_b200.cuda import attention
+from binade_b200.cuda import attention, logits
 
 CPU = -1
 
@@ -16,3 +16,18 @@ def test_rows_of_one_token_take_no_stride():
         t, steps = attention._rows(x[:n], "q", 3, CPU, apart=True)
         assert torch.equal(t, x[:n]) and all(s % 8 == 0 for s in steps)
     assert attention._rows(x[:1], "q", 3, CPU, apart=True)[0].data_ptr() == wide.data_ptr()  # and is read in place
+
+
+def test_options_of_a_call_survive_another_thread(monkeypatch):
+    """Between a look and a read another thread may empty the table."""
+
+    class Emptied(dict):
+        def __contains__(self, key):
+            there = super().__contains__(key)
+            self.clear()
+            return there
+
+    monkeypatch.setattr(attention, "_score_structs", Emptied())
+    for _ in range(3):
+        made, _ = attention._scores(128, 4, CPU, None, 20.0, 7, None, True)
+        assert (made.softcap, made.window, made.causal) == (20.0, 7, 1)

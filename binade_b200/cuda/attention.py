@@ -15,6 +15,7 @@ import ctypes
 import math
 
 import torch
+from torch.autograd import forward_ad
 
 from .. import _native
 from . import kernels as ck
@@ -22,6 +23,12 @@ from . import kernels as ck
 HEAD_DIMS = (64, 128, 256)
 BLOCKS = (16, 32, 64)
 KINDS = {"int8": 0, "e4m3": 1}  # BN_KV8_INT8, BN_KV8_E4M3
+
+
+def refuse_gradient(t: torch.Tensor, name: str) -> None:
+    """The calls here have no gradients, backward or forward: what asks for one is told so."""
+    if t.requires_grad and torch.is_grad_enabled() or forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None:
+        raise ValueError(f"{name} asks for a gradient: there is none here (use torch.no_grad)")
 
 
 def _rows(t: torch.Tensor, name: str, dims: int, device, apart: bool = False):
@@ -32,8 +39,7 @@ def _rows(t: torch.Tensor, name: str, dims: int, device, apart: bool = False):
         raise ValueError(f"{name} has to be a bfloat16 tensor of {dims} dimensions")
     if t.get_device() != device:
         raise ValueError(f"{name} is on {t.device}, the call on cuda:{device}")
-    if t.requires_grad and torch.is_grad_enabled():
-        raise ValueError(f"{name} asks for a gradient: attention here has none (use torch.no_grad)")
+    refuse_gradient(t, name)
     if t.is_contiguous() and t.data_ptr() % 16 == 0:
         steps, bits = t.stride()[:-1], 0
         for step in steps:
@@ -59,6 +65,8 @@ def _numbers(t, name: str, n: int, device, dtype=torch.int32) -> torch.Tensor | 
         return None
     if not isinstance(t, torch.Tensor) or t.get_device() != device or t.dim() != 1 or t.numel() != n or (dtype == torch.int32 and t.is_floating_point()):
         raise ValueError(f"{name} has to be a tensor of {n} {'whole ' if dtype == torch.int32 else ''}numbers on cuda:{device}")
+    if dtype == torch.float32:
+        refuse_gradient(t, name)
     return t if t.dtype is dtype and t.is_contiguous() else t.to(dtype).contiguous()
 
 
@@ -78,6 +86,7 @@ def _out(out, like: torch.Tensor, device, *inputs) -> torch.Tensor:
         return torch.empty_like(like, memory_format=torch.contiguous_format)
     if not isinstance(out, torch.Tensor) or out.dtype != torch.bfloat16 or out.shape != like.shape or out.get_device() != device or out.requires_grad:
         raise ValueError("out has to be a bfloat16 tensor of q's shape on its device")
+    refuse_gradient(out, "out")
     if out.stride(-1) != 1 or out.data_ptr() % 16 or any(s % 8 or s == 0 for s, n in zip(out.stride()[:-1], out.shape[:-1]) if n > 1):
         raise ValueError("out's rows have to lie apart, each of neighbouring elements from a 16-byte boundary on")
     if any(t is not None and overlap(out, t) for t in inputs):

@@ -12,7 +12,7 @@ import torch
 
 from .. import _native
 from . import kernels as ck
-from .attention import overlap
+from .attention import overlap, refuse_gradient
 
 
 class TokenCounts:
@@ -62,6 +62,7 @@ def _penalty(p, name: str, batch: int, device):
     if isinstance(p, torch.Tensor):
         if p.device != device or p.shape != (batch,):
             raise ValueError(f"{name} has to be a number or a tensor of {batch} on {device}")
+        refuse_gradient(p, name)
         return p if p.dtype is torch.float32 and p.is_contiguous() else p.to(torch.float32).contiguous(), 0.0
     return None, float(p)
 
@@ -78,8 +79,7 @@ def process_logits(logits: torch.Tensor, said: TokenCounts | None = None, *, rep
     if not isinstance(logits, torch.Tensor) or logits.dtype not in (torch.bfloat16, torch.float32) or logits.dim() != 2 or not logits.is_cuda or logits.get_device() != torch._C._cuda_getDevice():
         raise ValueError(f"logits have to be bfloat16 or float32 [batch, vocab] on the current device, {ck.require_cuda()}")
     dev = logits.device
-    if logits.requires_grad and torch.is_grad_enabled():
-        raise ValueError("logits ask for a gradient: there is none here (use torch.no_grad)")
+    refuse_gradient(logits, "logits")
     batch, vocab = logits.shape
     if not 1 <= vocab < 1 << 30 or batch > 65535:
         raise ValueError(f"logits {tuple(logits.shape)}")
@@ -105,6 +105,7 @@ def process_logits(logits: torch.Tensor, said: TokenCounts | None = None, *, rep
             continue
         if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.device != dev or t.shape not in ((width,), (batch, width)):
             raise ValueError(f"{name} has to be {dtype} of [{width}] or [{batch}, {width}] on {dev}")
+        refuse_gradient(t, name)
         t = t.contiguous()
         keep.append(t)
         setattr(rules, name, ck._p(t))
@@ -115,6 +116,7 @@ def process_logits(logits: torch.Tensor, said: TokenCounts | None = None, *, rep
         raise ValueError("out has to be float32 of the logits' shape with rows of neighbouring elements that do not overlap")
     elif overlap(out, logits) and not (out.data_ptr() == logits.data_ptr() and out.dtype == logits.dtype and (batch == 1 or out.stride(0) == logits.stride(0))):
         raise ValueError("out may be logits (float32), but not lie across them")
+    refuse_gradient(out, "out")
     tokens = torch.empty(batch, dtype=torch.int64, device=dev)
     if batch:
         ck._call("bn_logits", ck._p(logits), int(logits.dtype == torch.float32), logits.stride(0), batch, vocab, ctypes.byref(rules), ck._p(out), out.stride(0), ck._p(tokens))

@@ -1,7 +1,9 @@
 """Checks of arguments that need no GPU: the helpers behind the attention and logits calls, on CPU tensors (whose device
 number is -1)."""
 
+import pytest
 import torch
+from torch.autograd import forward_ad
 
 from binade_b200.cuda import attention, logits
 
@@ -31,3 +33,31 @@ def test_options_of_a_call_survive_another_thread(monkeypatch):
     for _ in range(3):
         made, _ = attention._scores(128, 4, CPU, None, 20.0, 7, None, True)
         assert (made.softcap, made.window, made.causal) == (20.0, 7, 1)
+
+
+def test_what_asks_for_a_gradient_is_refused():
+    asks = torch.ones(4, requires_grad=True)
+    for bad in (
+        lambda: attention._scores(128, 4, CPU, None, None, None, asks, True),
+        lambda: logits._penalty(asks, "presence", 4, asks.device),
+        lambda: logits._penalty(asks.double(), "presence", 4, asks.device),
+    ):
+        with pytest.raises(ValueError, match="gradient"):
+            bad()
+        with torch.no_grad():
+            bad()
+
+
+def test_what_carries_a_tangent_is_refused():
+    x = torch.ones((4, 2, 64), dtype=torch.bfloat16)
+    with forward_ad.dual_level():
+        dual, p = forward_ad.make_dual(x, x), forward_ad.make_dual(torch.ones(4), torch.ones(4))
+        for bad in (
+            lambda: attention._rows(dual, "q", 3, CPU),
+            lambda: attention._scores(128, 4, CPU, None, None, None, p, True),
+            lambda: logits._penalty(p, "presence", 4, p.device),
+        ):
+            with pytest.raises(ValueError, match="gradient"):
+                bad()
+        attention._rows(x, "q", 3, CPU)
+    attention._rows(x, "q", 3, CPU)

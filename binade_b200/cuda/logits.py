@@ -116,6 +116,8 @@ def process_logits(logits: torch.Tensor, said: TokenCounts | None = None, *, rep
         raise ValueError("out has to be float32 of the logits' shape with rows of neighbouring elements that do not overlap")
     elif overlap(out, logits) and not (out.data_ptr() == logits.data_ptr() and out.dtype == logits.dtype and (batch == 1 or out.stride(0) == logits.stride(0))):
         raise ValueError("out may be logits (float32), but not lie across them")
+    elif any(t is not None and overlap(out, t) for t in (*keep, said and said._all)):
+        raise ValueError("out may not lie among the penalties, the bias, the mask or the counts")
     refuse_gradient(out, "out")
     tokens = torch.empty(batch, dtype=torch.int64, device=dev)
     if batch:

@@ -39,3 +39,23 @@ def test_what_asks_for_a_gradient_is_refused():
             with pytest.raises(ValueError, match="gradient"):
                 call()
         process_logits(x), attention(q, q, q)
+
+
+def test_out_among_the_rules_is_refused():
+    """A block writes its piece of a row while another still reads the bias, the mask or the penalties there."""
+    from binade_b200.cuda.logits import TokenCounts, process_logits
+
+    said = TokenCounts(2, 96)
+    x, out = torch.randn((2, 96), device="cuda"), torch.zeros((2, 96), device="cuda")
+    for call in (
+        lambda: process_logits(x, bias=out, out=out),
+        lambda: process_logits(x, bias=out[1], out=out),
+        lambda: process_logits(x, said, presence=out[0, :2], out=out),
+        lambda: process_logits(x, mask=out.view(-1).view(torch.int32)[:3], out=out),
+        lambda: process_logits(x, said, presence=1.0, out=said.counts.view(torch.float32)),
+    ):
+        with pytest.raises(ValueError, match="out may not"):
+            call()
+    one = torch.randn((2, 96), device="cuda")
+    got, _ = process_logits(one, said, presence=1.0, bias=out[0], out=one)  # the logits themselves, beside the others
+    assert got is one

@@ -67,7 +67,14 @@ def _numbers(t, name: str, n: int, device, dtype=torch.int32) -> torch.Tensor | 
         raise ValueError(f"{name} has to be a tensor of {n} {'whole ' if dtype == torch.int32 else ''}numbers on cuda:{device}")
     if dtype == torch.float32:
         refuse_gradient(t, name)
+    elif t.dtype.itemsize > 4:
+        t = narrow(t)
     return t if t.dtype is dtype and t.is_contiguous() else t.to(dtype).contiguous()
+
+
+def narrow(t: torch.Tensor) -> torch.Tensor:
+    """64-bit whole numbers in 32: what lies beyond them as the nearest that they hold (a prefix of 2^40 keys is all of them)."""
+    return t.clamp(-(1 << 31), (1 << 31) - 1).to(torch.int32)
 
 
 def extent(t: torch.Tensor):

@@ -12,7 +12,7 @@ import torch
 
 from .. import _native
 from . import kernels as ck
-from .attention import overlap, refuse_gradient
+from .attention import narrow, overlap, refuse_gradient
 
 
 class TokenCounts:
@@ -47,7 +47,7 @@ class TokenCounts:
         if lengths is not None:
             if not isinstance(lengths, torch.Tensor) or lengths.device != self.device or lengths.shape != (self.batch,) or lengths.is_floating_point():
                 raise ValueError(f"lengths have to be {self.batch} whole numbers on {self.device}")
-            lengths = lengths.to(torch.int32).contiguous()
+            lengths = (narrow(lengths) if lengths.dtype.itemsize > 4 else lengths.to(torch.int32)).contiguous()
         ck._call("bn_token_counts", ck._p(tokens), int(tokens.dtype == torch.int64), tokens.stride(0), self.batch, tokens.shape[1], ck._p(lengths), self.vocab, int(prompt), ck._p(self.seen), self._all.stride(0), ck._p(self.counts), self._all.stride(0))
 
     def clear(self, row=None) -> None:

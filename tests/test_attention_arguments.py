@@ -61,3 +61,8 @@ def test_what_carries_a_tangent_is_refused():
                 bad()
         attention._rows(x, "q", 3, CPU)
     attention._rows(x, "q", 3, CPU)
+
+
+def test_whole_numbers_beyond_32_bits_do_not_wrap():
+    got = attention._numbers(torch.tensor([1 << 40, -(1 << 40), (1 << 31) - 1, 5]), "prefix", 4, CPU)
+    assert got.dtype is torch.int32 and got.tolist() == [(1 << 31) - 1, -(1 << 31), (1 << 31) - 1, 5]

@@ -143,6 +143,29 @@ def test_rows_computed_again_repeat_bit_for_bit():
         assert torch.equal(first[: T - 1], attention(q, k, v)[: T - 1])
 
 
+# ------------------------------------------------------------------------- whole numbers
+def test_whole_numbers_beyond_32_bits_do_not_wrap():
+    from binade_b200.cuda.attention import KV8Cache, attention
+
+    g = gen(75)
+    q, k, v = normal((90, 4, 64), g), normal((90, 2, 64), g), normal((90, 2, 64), g)
+    everything = torch.tensor([1 << 40], device="cuda")
+    want, bound = ref.attend(q, k, v, prefix=1000)
+    close(attention(q, k, v, prefix=everything), want, bound)
+    offsets = torch.tensor([-(1 << 40), 1 << 33], device="cuda")
+    want, bound = ref.attend(q, k, v)
+    close(attention(q, k, v, offsets), want, bound)
+    cache = KV8Cache(1, 1, 2, 64, 100, block=32)
+    cache.append(0, k[None], v[None], torch.tensor([1 << 40], device="cuda"))
+    cache.advance(torch.tensor([-(1 << 40)], device="cuda"))
+    assert cache.length.tolist() == [0]
+    cache.advance(90)
+    stored = [ref.stored(x, "int8", 32) for x in (k, v)]
+    want, bound = ref.attend(q[-1:], *stored, 89)
+    cache.advance(-1)
+    close(cache.attend(0, q[None, -1:], k[None, -1:], v[None, -1:], torch.tensor([(1 << 33) + 0], device="cuda"), prefix=everything)[0], want, bound)
+
+
 # ------------------------------------------------------------------------- strides
 def test_one_token_of_rows_with_an_odd_stride():
     """torch calls a tensor contiguous whatever the stride of a dimension of one element."""

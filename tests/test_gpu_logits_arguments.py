@@ -59,3 +59,11 @@ def test_out_among_the_rules_is_refused():
     one = torch.randn((2, 96), device="cuda")
     got, _ = process_logits(one, said, presence=1.0, bias=out[0], out=one)  # the logits themselves, beside the others
     assert got is one
+
+
+def test_lengths_beyond_32_bits_do_not_wrap():
+    from binade_b200.cuda.logits import TokenCounts
+
+    said = TokenCounts(2, 10)
+    said.add(torch.tensor([[1, 2, 3], [4, 5, 6]], device="cuda"), lengths=torch.tensor([1 << 32, -(1 << 32) + 2], device="cuda"))
+    assert said.counts.sum(1).tolist() == [3, 0]

@@ -28,7 +28,7 @@ extern "C" int bn_attention(const uint16_t *q, int64_t q_token, int64_t q_head, 
   if (D != 64 && D != 128 && D != 256) return bn::fail(BN_ERR_ARG, "bn_attention: a head has 64, 128 or 256 dimensions");
   if (!scores || (T && (!q || !k || !v || !out)) || (!offsets && docs != 1)) return bn::fail(BN_ERR_ARG, "bn_attention: null pointer, or no offsets for several documents");
   if (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out) & 15 || (q_token | q_head | k_token | k_head | v_token | v_head | o_token | o_head) & 7) return bn::fail(BN_ERR_ARG, "bn_attention: rows have to start on 16 bytes");
-  if (scores->window < 0 || scores->window > 0x3FFFFFFF || !(scores->softcap >= 0.0f)) return bn::fail(BN_ERR_ARG, "bn_attention: negative window or cap");
+  if (const char *why = bn::scores_refusal(scores)) return bn::refuse("bn_attention", why);
   if ((T > 1 && !(q_token && k_token && v_token && o_token)) || (heads > 1 && !(q_head && o_head)) || (kv_heads > 1 && !(k_head && v_head)) || (q_token | q_head | k_token | k_head | v_token | v_head) < 0) return bn::fail(BN_ERR_ARG, "bn_attention: rows have to lie apart");
   if (T == 0) return BN_OK;
   bn::PromptArgs a{q, k, v, out, q_token, q_head, k_token, k_head, v_token, v_head, o_token, o_head, offsets, prefix, scores->slopes, (int)T, (int)docs, (int)heads, (int)kv_heads, (int)scores->window, scores->causal, zero_rest, scores->scale, scores->softcap, {}, nullptr, 0, 0, 0, 0};

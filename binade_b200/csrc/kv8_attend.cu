@@ -198,14 +198,19 @@ __device__ __forceinline__ void weigh(const AttendArgs &a, float (&x)[P][MT][2][
 #pragma unroll
       for (int h = 0; h < 2; h++) {
         const float f = fmaxf(fminf(pc[p].scale * r.factor[mt][h], 3.0e38f), -3.0e38f);
+        const bool wide = !PLAIN && a.cap > WIDE_CAP;
+        if (wide) {
+#pragma unroll
+          for (int i = 0; i < 4; i++) x[p][mt][i >> 1][2 * h + (i & 1)] = capped_wide(x[p][mt][i >> 1][2 * h + (i & 1)] * f, a.cap * LOG2E);
+        }
 #pragma unroll
         for (int j = 0; j < 2; j++)
 #pragma unroll
           for (int e = 0; e < 2; e++) {
             float &v = x[p][mt][j][2 * h + e];
-            v *= f;
+            if (PLAIN || !wide) v *= f;
             if constexpr (!PLAIN) {
-              if (a.cap > 0.0f) v = capped(v, a.cap * LOG2E);
+              if (a.cap > 0.0f && !wide) v = capped(v, a.cap * LOG2E);
               v = fmaf(-r.slope[mt][h], (float)abs(r.i[mt][h] - (first + 2 * j + e)), v);
             }
           }
@@ -941,7 +946,7 @@ extern "C" int bn_kv8_attend(const bn_kv8 *c, const uint16_t *q, int64_t q_seq, 
   if (!bn::attend_sizes(c, tokens, heads)) return bn::fail(BN_ERR_ARG, "bn_kv8_attend: bad size (query heads have to be a multiple of the cache's heads)");
   if (!scores || (tokens && (!q || !out)) || !k != !v) return bn::fail(BN_ERR_ARG, "bn_kv8_attend: null pointer");
   if (((uintptr_t)q | (uintptr_t)out) & 15 || (q_seq | q_token | q_head | o_seq | o_token | o_head) & 7) return bn::fail(BN_ERR_ARG, "bn_kv8_attend: rows have to start on 16 bytes");
-  if (scores->window < 0 || scores->window > 0x3FFFFFFF || !(scores->softcap >= 0.0f)) return bn::fail(BN_ERR_ARG, "bn_kv8_attend: negative window or cap");
+  if (const char *why = bn::scores_refusal(scores)) return bn::refuse("bn_kv8_attend", why);
   if (tokens == 0) return BN_OK;
   const bool chunk = bn::chunk_wins(c, tokens, heads);
   const bn::Plan p = bn::plan_of(c, tokens, heads);

@@ -118,7 +118,7 @@ __device__ __noinline__ void attend_row(const PromptArgs &a, const Piece &p, int
 #pragma unroll
     for (int d = 16; d; d >>= 1) dot += __shfl_xor_sync(BN_FULL, dot, d);
     float s = dot * a.scale;
-    s = a.cap > 0.0f ? capped(s * (2.0f * LOG2E / a.cap), a.cap * LOG2E) : s * LOG2E;
+    s = a.cap > 0.0f ? capped_wide(s * (2.0f * LOG2E / a.cap), a.cap * LOG2E) : s * LOG2E;
     return s - slope * (float)abs(i - j);
   };
   for (int j = lo; j < hi; j++) {
@@ -299,8 +299,10 @@ __device__ __forceinline__ uint32_t bf16_pair(float lo, float hi) {
   return r;
 }
 
-// PLAIN: no cap, no bias, a positive scale. Else CAP: a cap.
-template <int D, bool PLAIN, bool CAP, int SRC>
+// PLAIN: no cap, no bias, a positive scale. Else CAP: a cap, a WIDE one beyond WIDE_CAP (a kernel of its own: beside one another
+// the two ways to cap spill 300 bytes a thread).
+constexpr int NO_CAP = 0, USUAL = 1, WIDE = 2;
+template <int D, bool PLAIN, int CAP, int SRC>
 __global__ void __launch_bounds__(Roles<SRC>::WARPS * 32, 1) prompt_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, const __grid_constant__ PromptArgs a, int group_log2, int head_groups) {
   using G = Tiles<D>;
   constexpr int NQ = G::NQ, BN = G::BN, ST = G::STAGES, TMA_WARP = Roles<SRC>::TMA_WARP, MMA_WARP = Roles<SRC>::MMA_WARP;
@@ -622,7 +624,8 @@ __global__ void __launch_bounds__(Roles<SRC>::WARPS * 32, 1) prompt_kernel(const
         for (int x = 0; x < CN; x += 2) {
           float z0, z1;
           split_f32(mul_f32x2(pair_f32(__uint_as_float(s[x]), __uint_as_float(s[x + 1])), f), z0, z1);
-          s[x] = __float_as_uint(capped(z0, a.cap * LOG2E)), s[x + 1] = __float_as_uint(capped(z1, a.cap * LOG2E));
+          s[x] = __float_as_uint(CAP == WIDE ? capped_wide(z0, a.cap * LOG2E) : capped(z0, a.cap * LOG2E));
+          s[x + 1] = __float_as_uint(CAP == WIDE ? capped_wide(z1, a.cap * LOG2E) : capped(z1, a.cap * LOG2E));
         }
       }
       if constexpr (!PLAIN) {  // s c - slope |i - j|; the bias is a line where all keys lie before the queries
@@ -805,7 +808,7 @@ inline int block_group_log2(int64_t heads, int64_t kv_heads) {
 
 template <int D, int SRC>
 int prompt_launch(const PromptArgs &a, const CUtensorMap &q_map, const CUtensorMap &k_map, const CUtensorMap &v_map, int64_t blocks, int log2, cudaStream_t stream) {
-  auto kern = a.cap > 0.0f ? prompt_kernel<D, false, true, SRC> : !a.slopes && a.scale > 0.0f ? prompt_kernel<D, true, false, SRC> : prompt_kernel<D, false, false, SRC>;
+  auto kern = a.cap > WIDE_CAP ? prompt_kernel<D, false, WIDE, SRC> : a.cap > 0.0f ? prompt_kernel<D, false, USUAL, SRC> : !a.slopes && a.scale > 0.0f ? prompt_kernel<D, true, NO_CAP, SRC> : prompt_kernel<D, false, NO_CAP, SRC>;
   const uint32_t smem = SRC == FROM_BF16 ? Tiles<D>::SMEM : Tiles<D>::SMEM_CODES;
   BN_CUDA(allow_smem(kern, smem));
   cudaLaunchConfig_t cfg{};

@@ -110,12 +110,12 @@ def _scores(dim: int, heads: int, device, scale, softcap, window, slopes, causal
     made = _score_structs.get(options) if slopes is None else None  # (one look: another thread may clear the table)
     if made is not None:
         return made, None
-    if softcap is not None and not (softcap > 0 and math.isfinite(softcap)):
-        raise ValueError("softcap has to be a positive number")
+    if softcap is not None and not 2.0**-60 <= softcap <= 2.0**60:
+        raise ValueError("softcap has to be a number in 2^-60 .. 2^60")
     if window is not None and not 1 <= window < 1 << 30:
         raise ValueError("window has to be at least 1")
-    if scale is not None and not math.isfinite(scale):
-        raise ValueError("scale has to be a finite number")
+    if scale is not None and not abs(scale) <= 3.4e38:
+        raise ValueError("scale has to be a number that fp32 holds")
     slopes = _numbers(slopes, "slopes", heads, device, torch.float32)
     made = _native.Scores(1.0 / math.sqrt(dim) if scale is None else scale, softcap or 0.0, window or 0, ck._p(slopes), int(bool(causal)))
     if slopes is None:

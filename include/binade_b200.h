@@ -285,8 +285,8 @@ int bn_swiglu(const uint16_t *gate, const uint16_t *up, int64_t n, uint16_t *h, 
  *   max(0, i - window + 1) <= j < min(L, i + window, causal ? max(i + 1, prefix) : L)   (window 0: no limit)
  * and its output is the softmax over their scores times their values. Sums are kept in fp32. */
 typedef struct bn_scores {
-  float scale;
-  float softcap;       /* 0: none */
+  float scale;         /* finite */
+  float softcap;       /* 0: none; else 2^-60 .. 2^60 */
   int64_t window;      /* 0: none */
   const float *slopes; /* [query heads] or NULL */
   int causal;

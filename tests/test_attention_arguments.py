@@ -66,3 +66,20 @@ def test_what_carries_a_tangent_is_refused():
 def test_whole_numbers_beyond_32_bits_do_not_wrap():
     got = attention._numbers(torch.tensor([1 << 40, -(1 << 40), (1 << 31) - 1, 5]), "prefix", 4, CPU)
     assert got.dtype is torch.int32 and got.tolist() == [(1 << 31) - 1, -(1 << 31), (1 << 31) - 1, 5]
+
+
+@pytest.mark.parametrize("bad", [dict(softcap=1e-50), dict(softcap=1e39), dict(softcap=2.0**61), dict(softcap=2.0**-61), dict(scale=1e39)])
+def test_caps_and_scales_that_fp32_does_not_hold_are_refused(bad):
+    with pytest.raises(ValueError):
+        attention._scores(128, 4, CPU, bad.get("scale"), bad.get("softcap"), None, None, True)
+
+
+@pytest.mark.parametrize("bad", [dict(softcap=1e-30), dict(softcap=float("inf")), dict(softcap=2.0**61), dict(scale=float("inf")), dict(scale=float("nan"))])
+def test_the_c_calls_refuse_them_too(bad):
+    from test_attention_host import attend, attention, scores
+
+    from binade_b200._native import NativeError
+
+    for call in (attention, attend):
+        with pytest.raises(NativeError, match="bad argument"):
+            call(s=scores(**bad))

@@ -143,6 +143,38 @@ def test_rows_computed_again_repeat_bit_for_bit():
         assert torch.equal(first[: T - 1], attention(q, k, v)[: T - 1])
 
 
+# ------------------------------------------------------------------------- caps
+@pytest.mark.parametrize("D,heads,kv", [(64, 4, 2), (128, 8, 2), (256, 2, 1)])
+@pytest.mark.parametrize("softcap", [2.0**-60, 1e-3, 300.0, 1000.0, 1e4, 1e6, 1e9, 2.0**60])
+def test_caps_of_all_sizes(D, heads, kv, softcap):
+    from binade_b200.cuda.attention import KV8Cache, attention
+
+    g = gen(74)
+    T = 300
+    q, k, v = normal((T, heads, D), g, 2.0), normal((T, kv, D), g, 1.5), normal((T, kv, D), g)
+    want, bound = ref.attend(q, k, v, softcap=softcap)
+    close(attention(q, k, v, softcap=softcap), want, bound)
+    stored = [ref.stored(x, "int8", 32) for x in (k, v)]
+    for new, batch in ((2, 1), (120, 6)):
+        cache = KV8Cache(1, batch, kv, D, T, block=32)
+        many = [x[None].expand(batch, -1, -1, -1).contiguous() for x in (q, k, v)]
+        cache.append(0, many[1][:, :-new], many[2][:, :-new])
+        cache.advance(T - new)
+        got = cache.attend(0, *(x[:, -new:] for x in many), softcap=softcap)
+        want, bound = ref.attend(q[-new:], *stored, T - new, softcap=softcap)
+        for b in range(batch):
+            close(got[b], want, bound)
+
+
+def test_caps_and_scales_that_fp32_does_not_hold_are_refused():
+    from binade_b200.cuda.attention import attention
+
+    x = torch.zeros((8, 4, 128), dtype=torch.bfloat16, device="cuda")
+    for bad in (dict(softcap=1e-50), dict(softcap=1e39), dict(softcap=2.0**61), dict(softcap=2.0**-61), dict(scale=1e39), dict(scale=-1e39)):
+        with pytest.raises(ValueError):
+            attention(x, x, x, **bad)
+
+
 # ------------------------------------------------------------------------- whole numbers
 def test_whole_numbers_beyond_32_bits_do_not_wrap():
     from binade_b200.cuda.attention import KV8Cache, attention

@@ -30,7 +30,7 @@ class Scores(C.Structure):
 class KV8Struct(C.Structure):
     """bn_kv8: device pointers and sizes of one layer's 8-bit key/value cache."""
 
-    _fields_ = [(n, _vp) for n in ("k", "v", "k_scale", "v_scale", "k_tail", "v_tail", "length", "side", "tickets")] + [(n, _i64) for n in ("batch", "kv_heads", "rows", "D", "max_seq")] + [("block", _int), ("kind", _int)]
+    _fields_ = [(n, _vp) for n in ("k", "v", "k_scale", "v_scale", "k_tail", "v_tail", "length", "side", "tickets")] + [(n, _i64) for n in ("batch", "kv_heads", "rows", "D", "max_seq")] + [("block", _int), ("kind", _int), ("kept", _vp)]
 
 
 class LogitRules(C.Structure):

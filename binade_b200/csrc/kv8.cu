@@ -7,7 +7,7 @@
 
 namespace bn {
 
-__device__ int g_kv8_error;  // 1: tokens were brought that the cache has no room for
+__device__ int g_kv8_error;  // 1: tokens were brought that the cache has no room for; 2: a length was asked for whose block is not held
 
 namespace {
 
@@ -31,7 +31,8 @@ __global__ void __launch_bounds__(128) append_kernel(const __grid_constant__ App
   const int64_t b = blockIdx.z;
   int held, brought;
   const bool all = kv8_tokens(c, a.counts, a.tokens, b, held, brought);
-  if (!all && rel == 0 && h == 0 && !values && threadIdx.x == 0) atomicExch(&g_kv8_error, 1);
+  if (!all && rel == 0 && h == 0 && !values && threadIdx.x == 0) atomicOr(&g_kv8_error, 1);
+  if (brought && rel == 0 && h == 0 && !values && threadIdx.x == 0) kv8_note(c, b, held, held + brought);
   const int j = held / c.block + rel;
   if (brought == 0 || j > (held + brought - 1) / c.block) return;
   const bool v = values;
@@ -43,8 +44,16 @@ __global__ void __launch_bounds__(256) advance_kernel(const __grid_constant__ bn
   if (b >= c.batch) return;
   const int held = min(max(c.length[b], 0), (int)c.max_seq);
   const int now = (int)min(max((int64_t)held + (counts ? counts[b] : n), (int64_t)0), c.max_seq);
+  if (now != held) {
+    const int block = now / c.block, slot = c.kept[2 * b] == block ? 0 : c.kept[2 * b + 1] == block ? 1 : -1;
+    if (slot < 0 && now % c.block) {  // tokens of a block that went straight to codes, or whose rows are overwritten
+      atomicOr(&g_kv8_error, 2);
+      return;
+    }
+    if (slot >= 0) c.side[b] = slot;
+    else if (block != held / c.block) c.side[b] ^= 1;
+  }
   c.length[b] = now;
-  if (now / c.block != held / c.block) c.side[b] ^= 1;
 }
 
 // Sixteen codes a thread at a time, as they lie: of keys sixteen dimensions of a token, of values four of four tokens. Tokens
@@ -136,6 +145,7 @@ extern "C" int bn_kv8_append(const bn_kv8 *c, const uint16_t *k, int64_t k_seq, 
 extern "C" int bn_kv8_advance(const bn_kv8 *c, int64_t n, const int32_t *counts, void *stream) {
   if (const char *why = bn::kv8_refusal(c)) return bn::refuse("bn_kv8_advance", why);
   if (n < -0x3FFFFFFF || n > 0x3FFFFFFF) return bn::fail(BN_ERR_ARG, "bn_kv8_advance: bad number of tokens");
+  if (!c->kept) return bn::refuse("bn_kv8_advance", "null cache array");
   bn::advance_kernel<<<(unsigned)((c->batch + 255) / 256), 256, 0, (cudaStream_t)stream>>>(*c, (int)n, counts);
   return bn::launched("advance_kernel");
 }

@@ -23,6 +23,17 @@ __device__ __forceinline__ bool kv8_tokens(const bn_kv8 &c, const int32_t *__res
 // the tokens of the call.
 __device__ __forceinline__ int kv8_slot(const bn_kv8 &c, int64_t b, int held, int j) { return (c.side[b] ^ (j != held / c.block)) & 1; }
 
+// Notes, for advance, which blocks the tail's slots hold when the tokens held .. end - 1 are there: the block open at `held`, and the
+// one open behind them or an earlier one, if its rows are still there.
+__device__ __forceinline__ void kv8_note(const bn_kv8 &c, int64_t b, int held, int end) {
+  if (!c.kept) return;
+  const int first = held / c.block, last = end / c.block, slot = c.side[b] & 1;
+  int32_t *const kept = c.kept + 2 * b;
+  kept[slot] = first;
+  if (last != first && end % c.block) kept[slot ^ 1] = last;
+  else if (kept[slot ^ 1] >= first) kept[slot ^ 1] = -1;
+}
+
 // The value of a code, without its scale.
 template <int KIND>
 __device__ __forceinline__ float kv8_code(uint32_t byte) {

@@ -572,6 +572,7 @@ __global__ void __launch_bounds__(WARPS * 32, (D == 64 && MT == 1) ? 4 : (MT * D
       }
       copies_commit();
     };
+    if (appends && kv == 0 && threadIdx.x == 0) kv8_note(cache, b, s.held, s.L);
     if (fills) append_filled<D>(a, b, kv, s.held, s.L);
 #pragma unroll
     for (int i = 0; i < S::STAGES - 1; i++) issue(tile + i, i);

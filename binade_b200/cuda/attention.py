@@ -189,12 +189,13 @@ class KV8Cache:
         self.k_scale, self.v_scale = new(rows // block, dtype=torch.float32), new(rows // block, dtype=torch.float32)
         self.k_tail, self.v_tail = new(2, block, head_dim, dtype=torch.bfloat16), new(2, block, head_dim, dtype=torch.bfloat16)
         self.length, self._side = torch.zeros(batch, dtype=torch.int32, device=self.device), torch.zeros(batch, dtype=torch.int32, device=self.device)
+        self._kept = torch.full((batch, 2), -1, dtype=torch.int32, device=self.device)
         self._tickets = torch.zeros(batch * kv_heads, dtype=torch.int32, device=self.device)
-        self._structs = [_native.KV8Struct(*(t[i].data_ptr() for t in (self.k, self.v, self.k_scale, self.v_scale, self.k_tail, self.v_tail)), self.length.data_ptr(), self._side.data_ptr(), self._tickets.data_ptr(), batch, kv_heads, rows, head_dim, max_seq, block, KINDS[kind]) for i in range(layers)]
+        self._structs = [_native.KV8Struct(*(t[i].data_ptr() for t in (self.k, self.v, self.k_scale, self.v_scale, self.k_tail, self.v_tail)), self.length.data_ptr(), self._side.data_ptr(), self._tickets.data_ptr(), batch, kv_heads, rows, head_dim, max_seq, block, KINDS[kind], self._kept.data_ptr()) for i in range(layers)]
 
     def bytes(self) -> int:
         """Device memory of the cache."""
-        return sum(t.numel() * t.element_size() for t in (self.k, self.v, self.k_scale, self.v_scale, self.k_tail, self.v_tail, self.length, self._side))
+        return sum(t.numel() * t.element_size() for t in (self.k, self.v, self.k_scale, self.v_scale, self.k_tail, self.v_tail, self.length, self._side, self._kept))
 
     def _layer(self, layer: int):
         if not 0 <= layer < self.layers:
@@ -213,7 +214,7 @@ class KV8Cache:
         """New tokens k, v [batch, tokens, kv_heads, D] bfloat16 behind what the sequences hold; counts (whole
         numbers [batch] on the device): how many of each sequence's are real, the first ones (None: all).
         `length` stays until `advance`: until then a second append writes the same places again. Tokens
-        beyond max_seq are dropped, and bn_device_status tells (bits 24..27)."""
+        beyond max_seq are dropped, and bn_device_status tells (value 1 in bits 24..27)."""
         at = self._layer(layer)
         (k, k_steps), (v, v_steps) = self._new(k, "k", self.kv_heads), self._new(v, "v", self.kv_heads)
         if k.shape != v.shape:
@@ -256,9 +257,10 @@ class KV8Cache:
 
     def advance(self, n) -> None:
         """Moves `length` on by n tokens (a number, or whole numbers [batch] on the device), within 0 .. max_seq.
-        Fewer than were appended may be kept (a draft whose end is rejected), and a sequence may go back, as
-        long as the new length lies in the block that was open before, in the one that is open behind all
-        the tokens, or on a border of blocks."""
+        Fewer than were appended may be kept (a draft whose end is rejected), and a sequence may go back. The new
+        length has to lie on a border of blocks, or in a block whose rows are still held in BF16: the one that was
+        open before the append, or the one that is open behind all its tokens. A sequence for which it does not
+        stays where it is, and bn_device_status tells (value 2 in bits 24..27)."""
         at = self._layer(0)
         counts = _numbers(n, "n", self.batch, self._index) if isinstance(n, torch.Tensor) else None
         ck._call("bn_kv8_advance", at, 0 if counts is not None else n, ck._p(counts))

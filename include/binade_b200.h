@@ -328,11 +328,12 @@ typedef struct bn_kv8 {
   uint32_t *tickets; /* [batch * kv_heads] zeros, for bn_kv8_attend, which leaves them so */
   int64_t batch, kv_heads, rows, D, max_seq;
   int block, kind;
+  int32_t *kept; /* [batch, 2] set to -1 at the start: the block whose rows each slot holds, for bn_kv8_advance (append and attend write it) */
 } bn_kv8;
 
 /* Up to `tokens` new tokens of every sequence, of which counts[b] are real (NULL: all), written behind the
  * length[b] that it holds; rows k, v (sequence, token, head) in BF16. Tokens that do not fit in max_seq are dropped, and
- * the device status says so (bits 24..27). */
+ * the device status says so (value 1 in bits 24..27). */
 int bn_kv8_append(const bn_kv8 *c, const uint16_t *k, int64_t k_seq, int64_t k_token, int64_t k_head,
                   const uint16_t *v, int64_t v_seq, int64_t v_token, int64_t v_head, int64_t tokens,
                   const int32_t *counts, void *stream);
@@ -350,8 +351,9 @@ int bn_kv8_attend(const bn_kv8 *c, const uint16_t *q, int64_t q_seq, int64_t q_t
                   int zero_rest, void *workspace, uint64_t workspace_bytes, void *stream);
 
 /* length moves on by n (counts NULL) or counts[b] tokens, within 0 .. max_seq: after the last layer of a step, by
- * all the tokens that were appended, or by fewer (a draft whose end is rejected), as long as the new length lies in the block that
- * was open before, in the one open behind all of them, or on a border of blocks. */
+ * all the tokens that were appended, or by fewer (a draft whose end is rejected), or back. The new length has to lie on a border of
+ * blocks or in a block whose rows a slot of the tail holds: the one that was open before the append, or behind all its tokens.
+ * A sequence for which it does not stays where it is, and the device status says so (value 2 in bits 24..27). */
 int bn_kv8_advance(const bn_kv8 *c, int64_t n, const int32_t *counts, void *stream);
 
 /* What the cache holds, as the values that the codes stand for: k, v [batch, kv_heads, max_seq, D] fp32,
@@ -415,7 +417,7 @@ int bn_push_gather_beside(const void *const *locals, const uint64_t *bytes, int 
 
 /* Device-side status of the calling thread's current device: 0, or non-zero once a kernel of
  * this library gave up a bounded wait or refused a launch whose shared-memory window did not
- * match (its output is then incomplete): bits 0..7 the batch-1 matvec kernels, bits 8..15 the tensor-core GEMM, bits 16..23 the peer exchange, bits 24..27 tokens that a key/value cache had no room for, bits 28..30 the attention of prompts. Every wait inside the
+ * match (its output is then incomplete): bits 0..7 the batch-1 matvec kernels, bits 8..15 the tensor-core GEMM, bits 16..23 the peer exchange, bits 24..27 a key/value cache (1: it had no room for tokens, 2: a length was asked for whose block it does not hold), bits 28..30 the attention of prompts. Every wait inside the
  * kernels is bounded, so a lost copy or an absent peer ends in this status instead of a hang.
  * Synchronises with the device. No counterpart in the reference. */
 int bn_device_status(int *status);

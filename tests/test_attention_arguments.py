@@ -83,3 +83,14 @@ def test_the_c_calls_refuse_them_too(bad):
     for call in (attention, attend):
         with pytest.raises(NativeError, match="bad argument"):
             call(s=scores(**bad))
+
+
+def test_advance_needs_to_know_which_blocks_are_held():
+    import ctypes
+
+    from test_attention_host import cache
+
+    from binade_b200 import _native
+
+    with pytest.raises(_native.NativeError, match="bad argument: bn_kv8_advance"):
+        _native.call("cuda", "bn_kv8_advance", ctypes.byref(cache(kept=None)), 1, None, None)

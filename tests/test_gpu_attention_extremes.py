@@ -221,3 +221,86 @@ def test_one_token_of_rows_with_an_odd_stride():
     out = torch.empty((1, 260), dtype=torch.bfloat16, device="cuda")[:, :256].unflatten(1, (2, 128))
     attention(x[:1], x[:1], x[:1], out=out)
     assert torch.equal(out, x[:1])
+
+
+# ------------------------------------------------------------------------- how far a cache moves on
+def test_advance_into_a_block_that_is_not_held_is_refused():
+    from binade_b200 import _native
+    from binade_b200.cuda.attention import KV8Cache
+
+    g = gen(77)
+    k, v = normal((3, 60, 1, 64), g), normal((3, 60, 1, 64), g)
+    for apart in (True, False):
+        _native.call("cuda", "bn_device_status_reset")
+        cache = KV8Cache(1, 3, 1, 64, 200, block=16)
+        cache.append(0, k[:, :15], v[:, :15])
+        cache.advance(15)
+        n = 20 if apart else 16
+        if apart:
+            cache.append(0, k[:, 15:35], v[:, 15:35])
+        else:
+            cache.attend(0, k[:, 15:31], k[:, 15:31], v[:, 15:31])
+        assert status() == 0
+        if apart:
+            cache.advance(torch.tensor([5, 17, 1], device="cuda"))  # into block 1, which went straight to codes; 2, open; a border
+            assert cache.length.tolist() == [15, 32, 16] and status() >> 24 == 2
+            _native.call("cuda", "bn_device_status_reset")
+            cache.advance(torch.tensor([n, 0, 0], device="cuda"))
+            assert cache.length.tolist() == [35, 32, 16] and status() == 0
+            got = cache.dense(0)
+            for b, L in enumerate((35, 32, 16)):
+                for x, y in zip(got, (k, v)):
+                    assert torch.equal(x[b, :, :L].transpose(0, 1), ref.stored(y[b, :L], "int8", 16).float())
+        else:
+            cache.advance(torch.tensor([5, 16, 1], device="cuda"))  # 20 and 31 lie in the open block behind 31 tokens
+            assert cache.length.tolist() == [20, 31, 16] and status() == 0
+
+
+def test_a_sequence_goes_back_as_far_as_its_rows_are_held():
+    from binade_b200 import _native
+    from binade_b200.cuda.attention import KV8Cache
+
+    _native.call("cuda", "bn_device_status_reset")
+    g = gen(78)
+    k, v, again = normal((1, 100, 2, 128), g), normal((1, 100, 2, 128), g), normal((1, 100, 2, 128), g)
+    cache = KV8Cache(2, 1, 2, 128, 200, block=32)
+    at = 0
+    for n in (20, 20, 30):  # 20, 40, 70 tokens: blocks 1 and 2 are held as they came, block 0 is codes
+        for layer in range(2):
+            cache.append(layer, k[:, at : at + n], v[:, at : at + n])
+        cache.advance(n)
+        at += n
+    cache.advance(-20)  # 50, in block 1
+    assert cache.length.item() == 50 and status() == 0
+    cache.advance(-40)  # 10, in block 0: no
+    assert cache.length.item() == 50 and status() >> 24 == 2
+    _native.call("cuda", "bn_device_status_reset")
+    for layer in range(2):
+        cache.append(layer, again[:, :70], again[:, :70])  # 120: blocks 1 and 3 are held
+    cache.advance(60)  # 110, in block 3
+    assert cache.length.item() == 110
+    cache.advance(-5)  # 105: the same
+    cache.advance(-40)  # 65, in block 2, which went straight to codes
+    assert cache.length.item() == 105 and status() >> 24 == 2
+    _native.call("cuda", "bn_device_status_reset")
+    cache.advance(-9)  # 96: a border
+    assert cache.length.item() == 96
+    cache.advance(-40)  # 56, in block 1
+    assert cache.length.item() == 56 and status() == 0
+    want = [torch.cat([x[0, :50], again[0, :6]]) for x in (k, v)]
+    for layer in range(2):
+        for got, w in zip(cache.dense(layer), want):
+            assert torch.equal(got[0, :, :56].transpose(0, 1), ref.stored(w, "int8", 32).float())
+    cache.advance(-24)  # 32, a border; then on, over what was there
+    q = normal((1, 12, 4, 128), g)
+    for layer in range(2):
+        cache.attend(layer, q, again[:, 80:92], again[:, 80:92])
+    cache.advance(7)
+    want = [torch.cat([x[0, :32], again[0, 80:87]]) for x in (k, v)]
+    assert cache.length.item() == 39 and status() == 0
+    for got, w in zip(cache.dense(1), want):
+        assert torch.equal(got[0, :, :39].transpose(0, 1), ref.stored(w, "int8", 32).float())
+    cache.length.zero_()  # the place is free: a new sequence, behind which nothing of the old one may come back
+    cache.append(0, k[:, :3], v[:, :3])
+    cache.advance(3)
+    assert cache.length.item() == 3 and status() == 0

@@ -243,7 +243,7 @@ class Decoder(nn.Module):
         """A prompt, int64 [P] on the device, through the layers in one pass -> logits [1, vocab] behind its last token; its
         keys and values go to the cache (in 8 bits; one GPU). Without `more` the cache is emptied first and the prompt's tokens
         see one another's keys as they are; with it the prompt goes behind what the cache holds, and sees what the
-        cache holds then."""
+        cache holds then (its length is read on the host, to refuse a prompt that does not fit)."""
         if self.cache is None or self.world > 1:
             raise ValueError("prefill needs a cache in 8 bits and one GPU")
         s, d, P = self.shape, self.shape.head_dim, tokens.numel()
@@ -251,6 +251,10 @@ class Decoder(nn.Module):
             raise ValueError(f"a prompt of {P} tokens, max_seq {s.max_seq}")
         if not more:
             self.reset()
+        elif not torch.cuda.is_current_stream_capturing():  # (a capture reads nothing: there the device status alone tells)
+            held = int(self.cache.length.item())
+            if held + P > s.max_seq:
+                raise ValueError(f"a prompt of {P} tokens behind {held}, max_seq {s.max_seq}")
         x = self.embed(tokens) if isinstance(self.embed, r4.R4Embedding) else self.embed.index_select(0, tokens)  # [P, hidden]
         at = torch.clamp(self.positions[:P] + self.cache.length.to(torch.int64) if more else self.positions[:P], max=s.max_seq - 1)
         cos, sin = self.cos.index_select(0, at)[:, None, :], self.sin.index_select(0, at)[:, None, :]  # [P, 1, d/2]

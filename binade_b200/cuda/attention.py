@@ -13,6 +13,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import operator
 
 import torch
 from torch.autograd import forward_ad
@@ -106,7 +107,9 @@ _score_structs: dict = {}  # bn_scores of calls without slopes, by their options
 
 def _scores(dim: int, heads: int, device, scale, softcap, window, slopes, causal):
     """The bn_scores of a call, and the slopes that it points at."""
-    options = (dim, scale, softcap, window, causal)
+    scale, softcap = None if scale is None else float(scale), None if softcap is None else float(softcap)
+    window, causal = None if window is None else operator.index(window), bool(causal)
+    options = (dim, scale, softcap, window, causal)  # (plain numbers: what a tensor holds may change)
     made = _score_structs.get(options) if slopes is None else None  # (one look: another thread may clear the table)
     if made is not None:
         return made, None
@@ -117,7 +120,7 @@ def _scores(dim: int, heads: int, device, scale, softcap, window, slopes, causal
     if scale is not None and not abs(scale) <= 3.4e38:
         raise ValueError("scale has to be a number that fp32 holds")
     slopes = _numbers(slopes, "slopes", heads, device, torch.float32)
-    made = _native.Scores(1.0 / math.sqrt(dim) if scale is None else scale, softcap or 0.0, window or 0, ck._p(slopes), int(bool(causal)))
+    made = _native.Scores(1.0 / math.sqrt(dim) if scale is None else scale, softcap or 0.0, window or 0, ck._p(slopes), int(causal))
     if slopes is None:
         if len(_score_structs) >= 64:
             _score_structs.clear()

@@ -94,3 +94,12 @@ def test_advance_needs_to_know_which_blocks_are_held():
 
     with pytest.raises(_native.NativeError, match="bad argument: bn_kv8_advance"):
         _native.call("cuda", "bn_kv8_advance", ctypes.byref(cache(kept=None)), 1, None, None)
+
+
+def test_options_are_taken_by_value():
+    """A number in a tensor may change between two calls; nothing is kept by an object's identity."""
+    scale, cap, window, causal = torch.tensor(0.5), torch.tensor(20.0), torch.tensor(7), torch.tensor(True)
+    for factor in (1, 2, 3):
+        made, _ = attention._scores(128, 4, CPU, scale, cap, window, None, causal)
+        assert (made.scale, made.softcap, made.window, made.causal) == (0.5 * factor, 20.0 * factor, 7, factor % 2)
+        scale.add_(0.5), cap.add_(20.0), causal.logical_not_()

@@ -159,7 +159,7 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets: torch.
         offsets = _numbers(offsets, "offsets", docs + 1, dev)
     prefix = _numbers(prefix, "prefix", docs, dev)
     scores, slopes = _scores(D, heads, dev, scale, softcap, window, slopes, causal)
-    y = _out(out, q, dev, q, k, v)
+    y = _out(out, q, dev, q, k, v, offsets, prefix, slopes)
     if T:
         ck._call("bn_attention", q.data_ptr(), *q_steps, k.data_ptr(), *k_steps, v.data_ptr(), *v_steps, T, heads, kv, D, ck._p(offsets), docs, ck._p(prefix), ctypes.byref(scores), y.data_ptr(), *(y.stride()[:-1] if out is None else _steps(y)), int(out is None))
     return y
@@ -242,7 +242,7 @@ class KV8Cache:
         counts = _numbers(counts, "counts", self.batch, self._index)
         prefix = _numbers(prefix, "prefix", self.batch, self._index)
         scores, slopes = _scores(self.head_dim, heads, self._index, scale, softcap, window, slopes, causal)
-        y = _out(out, q, self._index, q, k, v)
+        y = _out(out, q, self._index, q, k, v, counts, prefix, slopes)
         if k is None:
             new = (None, 0, 0, 0, None, 0, 0, 0)
         else:

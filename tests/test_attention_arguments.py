@@ -103,3 +103,11 @@ def test_options_are_taken_by_value():
         made, _ = attention._scores(128, 4, CPU, scale, cap, window, None, causal)
         assert (made.scale, made.softcap, made.window, made.causal) == (0.5 * factor, 20.0 * factor, 7, factor % 2)
         scale.add_(0.5), cap.add_(20.0), causal.logical_not_()
+
+
+def test_out_among_the_inputs_is_refused():
+    x = torch.zeros((2, 4, 64), dtype=torch.bfloat16)
+    for t in (x, x.view(torch.int32)[0, 0], x.view(torch.float32)[1, 3, :2]):
+        with pytest.raises(ValueError, match="among the inputs"):
+            attention._out(x, torch.empty_like(x), CPU, None, t)
+    assert attention._out(x, torch.empty_like(x), CPU, torch.zeros(4)) is x

@@ -317,9 +317,9 @@ __device__ __noinline__ void append_filled(const AttendArgs &a, int64_t b, int h
   __syncthreads();
 }
 
-// The open block's 16 tokens from `key0` on, in BF16. Weights go in two BF16 halves (hi + lo: 2^-17), values times 2^-23
-// with 2^23 as V's scale, so that no sum of 63 of them passes fp32. Where a value is not finite, a
-// weight of zero must not touch it: those go one by one.
+// The open block's 16 tokens from `key0` on, in BF16. Weights go in two BF16 halves (hi + lo: 2^-17), values over the power of two
+// of the largest, which is V's scale then as a code's block has one: no sum passes fp32, and none is lost beside the codes' for a
+// scale that is not theirs. Where a value is not finite, a weight of zero must not touch it: those go one by one.
 template <int D, int MT, bool PLAIN>
 __device__ void open_block(const AttendArgs &a, const uint16_t *const (&qrow)[MT][2], const OpenRows &rows, int L, int key0, const Rows<MT> &r, State<D, MT> &st) {
   const uint32_t lane = lane_id(), n = lane >> 2, c = lane & 3u;
@@ -347,7 +347,30 @@ __device__ void open_block(const AttendArgs &a, const uint16_t *const (&qrow)[MT
   Rows<MT> plain = r;  // the queries as they are: no power of two in the factor
 #pragma unroll
   for (int mt = 0; mt < MT; mt++) plain.factor[mt][0] = plain.factor[mt][1] = a.cap > 0.0f ? a.scale * (2.0f * LOG2E / a.cap) : a.scale * LOG2E;
-  const PieceOf16 piece[1] = {{key0, L, 1.0f, (float)(1 << 23), 23.0f, true}};
+  const uint16_t *v[4];
+  uint32_t most = 0;  // largest magnitudes, as pairs of 16 bits
+#pragma unroll
+  for (int i = 0; i < 4; i++) v[i] = rows.value(min(key0 + 4 * (int)c + i, L - 1));
+#pragma unroll
+  for (int t = 0; t < Shape<D, MT>::NT; t += 2)
+#pragma unroll
+    for (int i = 0; i < 4; i++) most = __vmaxu2(most, *reinterpret_cast<const uint32_t *>(v[i] + dim_of<D>(t, (int)n)) & 0x7FFF7FFFu);  // dims dim_of(t, n) and the next
+  most = __reduce_max_sync(BN_FULL, max(most & 0xFFFFu, most >> 16));
+  const bool odd = most >= 0x7F80u;
+  if (odd) {  // the largest of the others
+    most = 0;
+#pragma unroll 1
+    for (int t = 0; t < Shape<D, MT>::NT; t += 2)
+#pragma unroll 1
+      for (int i = 0; i < 4; i++) {
+        const uint32_t w = *reinterpret_cast<const uint32_t *>(v[i] + dim_of<D>(t, (int)n)), lo = w & 0x7FFFu, hi = (w >> 16) & 0x7FFFu;
+        most = max(most, max(lo < 0x7F80u ? lo : 0u, hi < 0x7F80u ? hi : 0u));
+      }
+    most = __reduce_max_sync(BN_FULL, most);
+  }
+  const int exponent = min(max((int)(most >> 7), 27), 253);  // as it stands in fp32: 2^-100 .. 2^126
+  const float vscale = __uint_as_float((uint32_t)exponent << 23), vinv = __uint_as_float((uint32_t)(254 - exponent) << 23);
+  const PieceOf16 piece[1] = {{key0, L, 1.0f, vscale, (float)(exponent - 127), true}};
   weigh<D, MT, 1, PLAIN>(a, x1, plain, st, piece);
   uint32_t hi[MT][4], lo[MT][4];
 #pragma unroll
@@ -358,27 +381,15 @@ __device__ void open_block(const AttendArgs &a, const uint16_t *const (&qrow)[MT
       hi[mt][f] = pack_bf16(p0, p1);
       lo[mt][f] = pack_bf16(p0 - __uint_as_float(hi[mt][f] << 16), p1 - __uint_as_float(hi[mt][f] & 0xFFFF0000u));
     }
-  const uint16_t *v[4];
-  bool odd = false;
-#pragma unroll
-  for (int i = 0; i < 4; i++) v[i] = rows.value(min(key0 + 4 * (int)c + i, L - 1));
-#pragma unroll
-  for (int t = 0; t < Shape<D, MT>::NT; t += 2) {
-    uint32_t w[4];  // dims dim_of(t, n) and the next
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-      w[i] = *reinterpret_cast<const uint32_t *>(v[i] + dim_of<D>(t, (int)n));
-      odd |= (w[i] & 0x7F80u) == 0x7F80u || (w[i] & 0x7F800000u) == 0x7F800000u;
-    }
-  }
-  if (!__any_sync(BN_FULL, odd)) {
+  if (!odd) {
+    const uint32_t down = (__float_as_uint(vinv) >> 16) * 0x10001u;  // 2^-exponent twice, in BF16
 #pragma unroll
     for (int t = 0; t < Shape<D, MT>::NT; t += 2) {
       uint32_t w[4];
 #pragma unroll
       for (int i = 0; i < 4; i++) {
         w[i] = *reinterpret_cast<const uint32_t *>(v[i] + dim_of<D>(t, (int)n));
-        asm("mul.rn.bf16x2 %0, %0, %1;" : "+r"(w[i]) : "r"(0x34003400u));  // 2^-23
+        asm("mul.rn.bf16x2 %0, %0, %1;" : "+r"(w[i]) : "r"(down));
       }
 #pragma unroll
       for (int e = 0; e < 2; e++) {
@@ -405,7 +416,7 @@ __device__ void open_block(const AttendArgs &a, const uint16_t *const (&qrow)[MT
 #pragma unroll
           for (int t = 0; t < Shape<D, MT>::NT; t++)
 #pragma unroll
-            for (int e = 0; e < 2; e++) st.o[mt][t][2 * h + e] = fmaf(p, bf16_to_f32(row[dim_of<D>(t, 2 * (int)c + e)]) * (1.0f / (1 << 23)), st.o[mt][t][2 * h + e]);
+            for (int e = 0; e < 2; e++) st.o[mt][t][2 * h + e] = fmaf(p, bf16_to_f32(row[dim_of<D>(t, 2 * (int)c + e)]) * vinv, st.o[mt][t][2 * h + e]);
       }
   }
 }

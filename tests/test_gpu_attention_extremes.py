@@ -89,6 +89,20 @@ def test_decode_values_from_the_smallest_to_the_largest(kind, D, heads, kv):
 
 
 @pytest.mark.parametrize("kind", ["int8", "e4m3"])
+@pytest.mark.parametrize("D,heads,kv", [(64, 4, 2), (128, 12, 1), (256, 4, 1)])
+@pytest.mark.parametrize("size", [1e-25, 1e-20, 1.0, 1e30])
+def test_decode_small_values_behind_an_open_token_without_any(D, heads, kv, kind, size):
+    """The open block takes the weight and has no values, or ones as small: stored blocks' stay beside it, however small."""
+    g = gen(79)
+    for gap in (10, 24, 40):
+        for open_size in (0.0, size, 1e-3 * size):
+            keys = torch.cat([constant(96, kv, D, 0), constant(3, kv, D, gap)])
+            values = (torch.cat([normal((96, kv, D), g).abs().float() * size, normal((3, kv, D), g).abs().float() * open_size])).to(torch.bfloat16)
+            check_decode(keys, values, heads, kind, 32, new=2)
+            check_decode(keys, values, heads, kind, 32, new=2, softcap=100.0)
+
+
+@pytest.mark.parametrize("kind", ["int8", "e4m3"])
 @pytest.mark.parametrize("D,heads,kv,L", [(64, 4, 1, 4100), (128, 4, 1, 9001), (128, 24, 1, 4100), (256, 4, 2, 4100), (128, 4, 1, 300)])
 @pytest.mark.parametrize("gap", [6.0, 12.0, 17.0, 18.0])
 def test_decode_behind_a_sink(kind, D, heads, kv, L, gap):

@@ -19,8 +19,9 @@ struct AppendArgs {
   int tokens, rel;  // tokens a sequence brings at most; blocks of the cache that those can touch
 };
 
-// A block per block of tokens, keys or values. 4 x 2000 tokens, 8 heads of 128 (49 MB): 24 us; the instructions of the
-// rounding (20 a value) come before the bytes.
+// A block per block of tokens, keys or values. 4 x 2000 tokens, 8 heads of 128 (49 MB): 23 us from DRAM, 15 where the tokens are
+// in L2. Neither bytes (7.5 us) nor instructions (10.2 M, 9 us at full issue) bound it: a block's loads, maximum, codes and stores
+// follow one another, and 2.3 rounds of blocks leave the SMs idle a third of the time.
 template <int D, int CHUNKS>
 __global__ void __launch_bounds__(128) append_kernel(const __grid_constant__ AppendArgs a) {
   const bn_kv8 &c = a.c;

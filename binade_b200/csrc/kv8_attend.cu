@@ -29,9 +29,9 @@
 // codes the block that they fill before it reads it: a decode step is one launch. Several groups of rows (more than
 // 32, or 16 with heads of 256) read what an append kernel has written.
 //
-// Measured: 64 sequences of up to 8192 tokens, 8 key heads of 128, int8, 637 MB: 171 us, 3.7 TB/s, 57 % of the copy rate;
-// one sequence of 131073, 269 MB: 68 us; one of 300: 12 us in a graph. What bounds the long ones: 64 M warp
-// instructions (410 a piece of 16 keys; 44 % of the issue slots) at 12 warps an SM, fixed-latency waits first.
+// Measured: 64 sequences of up to 8192 tokens, 8 key heads of 128, int8, 637 MB: 178 us, 3.6 TB/s, 55 % of the copy rate;
+// one sequence of 131073, 269 MB: 71 us; one of 300: 21 us a call, 12 in a graph. What bounds the long ones: 68 M warp
+// instructions (430 a piece of 16 keys; 45 % of the issue slots) at 12 warps an SM, fixed-latency waits first.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -891,8 +891,10 @@ Plan plan_of(const bn_kv8 *c, int64_t tokens, int64_t heads) {
   const int64_t most = c->batch * c->kv_heads * p.row_groups * ((c->max_seq + tile - 1) / tile + 1);
   const int64_t full = (int64_t)sm_count() * resident;
   p.blocks = (int)(most < full ? most : full);
-  // The block that finishes last reads a few parts faster than another kernel starts, many parts slower (us, 300 tokens,
-  // 6 parts at most: 12.4 / 14.4; 131073 tokens, 55 parts: 82 / 70).
+  // A kernel for the join costs a launch, the block that finishes last a chain of loads that grows with the parts. One sequence
+  // of 8 heads, here / kernel: 300 tokens, 6 parts at most, 13.5 / 15.4 us a call (the host's; 12.0 / 11.4 in a graph); in a graph
+  // 1000 tokens 13.9 / 11.9, 130000, 55 parts, 93 / 71. 64 sequences: 300 tokens 30 / 35, 10000 258 / 262. Eight blocks a head: few
+  // parts, or many heads, of which few are cut.
   p.join_here = p.row_groups == 1 && p.blocks <= 8 * c->batch * c->kv_heads;
   p.plan_bytes = ((uint64_t)(c->batch + 2) * 8 + 127) / 128 * 128;
   p.bytes = p.plan_bytes + (uint64_t)p.blocks * 2 * (16 * p.mt * (D + 3)) * 4;
@@ -924,7 +926,10 @@ int attend_kind(const AttendArgs &a, int mt, cudaStream_t s) {
 }
 
 // Whether many rows go to the other kernel (kv8_chunk.cu), which reads a sequence's keys once for 256 rows (128 with heads
-// of 256), but by one block from end to end.
+// of 256), but by one block from end to end: it wins where there are groups of 32 rows to fill the card several times over with
+// this kernel's blocks. Where the two cross depends on the lengths, which the host does not know: near 50 groups at 500 keys,
+// near 250 at 9000 and more; 100 lies between. us, this kernel / the other, 8 heads of 128 in groups of 4, by groups:
+// 500 keys 64: 36 / 26, 128: 47 / 26; 9000 keys 64: 78 / 233, 128: 130 / 243, 256: 232 / 250, 504: 438 / 269.
 bool chunk_wins(const bn_kv8 *c, int64_t tokens, int64_t heads) {
   const int64_t rows = heads / c->kv_heads * tokens, units = c->batch * c->kv_heads, per_block = c->D == 256 ? 128 : 256;
   const int64_t groups = (rows + 31) / 32, waves = (units * ((rows + per_block - 1) / per_block) + sm_count() - 1) / sm_count();

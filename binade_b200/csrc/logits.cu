@@ -52,9 +52,10 @@ __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.aligned;" ::: "memory"); }
 
 // A cluster of blocks per row: the blocks take pieces of the vocabulary in turn, four tokens a thread, and the
-// first of them joins their choices through distributed shared memory. One launch, whatever the batch: 8 us in a graph for
-// one row of 128256 (the latency of a few loads in a row), 36 us for 64 rows of 151937 fp32 (2.2 TB/s: 130 instructions a
-// quad, and the counts' second load). Quads start where the output row
+// first of them joins their choices through distributed shared memory. One launch, whatever the batch: 6 us in a graph for
+// one row of 128256 (the latency of a few loads in a row), 35 us for 64 rows of 151937 fp32 with penalties, bias and masks (2.3
+// TB/s; 12 us of bytes, 17 of instructions at full issue: a thread's ten rounds each wait for their loads, then for the
+// counts). Quads start where the output row
 // has 16-byte boundaries (rows of an odd vocabulary start anywhere); the input is read in one piece
 // where its row has them at the same places. Counts are read only where a token was said.
 template <typename T, int THREADS, int U>
@@ -188,7 +189,9 @@ extern "C" int bn_logits(const void *x, int fp32, int64_t x_row, int64_t batch, 
   constexpr int threads = 512;
   const int quads = batch <= 8 ? 2 : 1;
   bn::LogitsArgs a{x, out, token, x_row, out_row, (int)V, *rules};
-  // blocks of a row: up to 8 (the portable cluster size), 16 where the rows are few
+  // Blocks of a row: up to 8 (the portable cluster size), 16 where the rows are few; two quads a thread there, whose loads wait
+  // together. us in a graph, 128256 tokens, penalties, one quad and 8 blocks / two and 16: 1 row 9.4 / 6.8, 8 rows 9.8 / 8.3, 16
+  // rows 12.6 / 11.9, 32 rows 12.9 / 17.8, 64 rows 22 / 33.
   const int64_t need = (V + 4 * threads - 1) / (4 * threads);
   const unsigned most = batch <= 8 ? 16 : 8;
   unsigned blocks = 1;

@@ -9,8 +9,8 @@
 //   a warp copies Q, K and V tiles by TMA (128-byte swizzle) into a ring
 //   a warp issues the MMAs: for tile i in turn P_i V of the last keys, then Q_i K^T of the next, so that one
 //     tile's softmax runs beside the other's products (heads of 256: two S buffers do the same for one tile)
-//   four warps a tile do the softmax, a row a thread: S out of tensor memory, P back over it in BF16 (rounded to
-//     2^-9 of a weight; the sum takes it before that) as the second product's first operand
+//   four warps a tile do the softmax, a row a thread: S out of tensor memory, P back over it in BF16 (rounded by up
+//     to 2^-8 of a weight; the sum takes it before that) as the second product's first operand
 // m moves only when a row's maximum passes it by 8 (weights up to 2^8 are as good in BF16 and fp32): most
 // tiles leave O where it is. V is the MMA's B by columns, as it lies in memory: nothing is transposed.
 // Keys that no row of the block sees are not read. A row whose sums are not finite is computed again by one warp over its
@@ -20,9 +20,11 @@
 // fit its 8 bits) straight into the ring, the open block's tokens as they are. The scales stay apart: K's multiply
 // the scores of their 16 keys or more, V's the weights, before these are rounded.
 //
-// Measured: 8192 tokens, 32 / 8 heads of 128, causal: 477 us at full clocks, 1.15 PFLOP/s, 69 % of the measured cuBLAS
-// rate (552 us under the power cap). Tensor pipe 53 %, ex2's 53 %: a tile's S, softmax, P and O in a row are twice as long as either,
-// and two tiles are what tensor memory holds. Chunk of 2 x 500 tokens over up to 9000, int8: 265 us.
+// Measured: 8192 tokens, 32 / 8 heads of 128, causal: 552 us a call among others (under the power cap), 1.00 PFLOP/s, 60 % of
+// the measured cuBLAS rate; 481 us at full clocks. Tensor pipe 53 %, ex2's 53 %: a tile's S, softmax, P and O in a row are twice as
+// long as either, and two tiles are what tensor memory holds. Chunk of 2 x 500 tokens over up to 9000, int8: 303 us a call, 260 at
+// full clocks. 5003 tokens in 11 documents, heads of 256, cap, window: 76 us; 6001 in 7, heads of 64, bias: 58 us: blocks of a few
+// key tiles, one an SM, whose start and end nothing hides (tensor pipe 20 and 13 %, ex2's 31 and 27 %).
 //
 // Every wait is bounded: a wait that gives up sets the device status, and the block still ends.
 #pragma once

@@ -256,7 +256,7 @@ __device__ __forceinline__ void weigh(const AttendArgs &a, float (&x)[P][MT][2][
         t = fmaxf(t, __shfl_xor_sync(BN_FULL, t, 1)), u = fmaxf(u, __shfl_xor_sync(BN_FULL, u, 1));
         t = fmaxf(t, __shfl_xor_sync(BN_FULL, t, 2)), u = fmaxf(u, __shfl_xor_sync(BN_FULL, u, 2));
         t = fmaxf(t, st.m[mt][h]);
-        const float rise = t - st.m[mt][h], d = floorf(fminf(st.d[mt][h] + rise, AIM - (u - t)));  // (whole: 2^d is exact)
+        const float rise = t - st.m[mt][h], d = fminf(st.d[mt][h] + rise, floorf(AIM - (u - t)));  // (m - d stays where it is unless a p' is too large)
         const float keep = ex2(-rise), keep_o = ex2(d - st.d[mt][h] - rise);
         st.m[mt][h] = t, st.d[mt][h] = d, st.l[mt][h] *= keep;
 #pragma unroll

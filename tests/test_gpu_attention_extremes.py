@@ -116,6 +116,33 @@ def test_decode_behind_a_sink(kind, D, heads, kv, L, gap):
     check_decode(keys[order], values[order], heads, kind, 32)
 
 
+@pytest.mark.parametrize("kind", ["int8", "e4m3"])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_decode_values_beside_keys_that_rise_without_any(kind, D):
+    """Every other block has zeros for values and, for one head, a score that rises from tile to tile by less than a power of two;
+    for another head of the same warp the blocks between them rise by more. The first head's keep their bits."""
+    from binade_b200.cuda.attention import KV8Cache
+
+    g = gen(80)
+    batch, kv, L = 60, 8, 100 * 128
+    key = torch.arange(L, device="cuda")
+    zero = key // 16 % 2 == 0
+    none = torch.zeros_like(key, dtype=torch.float32)
+    halves = torch.stack([torch.where(zero, 0.9 * (key // 128), none), torch.where(zero, none, 3.6 * (key // 128))], dim=1) * math.log(2)
+    keys = halves.repeat_interleave(D // 2, 1)[:, None].expand(L, kv, D).to(torch.bfloat16)
+    values = torch.where(zero[:, None, None], torch.zeros((), device="cuda"), normal((L, kv, D), g).float().abs()).to(torch.bfloat16)
+    cache = KV8Cache(1, batch, kv, D, L + 1, kind=kind, block=16)
+    many = lambda x: x[None].expand(batch, -1, -1, -1)  # noqa: E731
+    cache.append(0, many(keys), many(values))
+    cache.advance(L)
+    q = (2 * torch.eye(2, device="cuda").repeat_interleave(D // 2, 1).repeat(kv, 1))[None, None].expand(batch, 1, 2 * kv, D).to(torch.bfloat16)
+    last = torch.zeros((1, kv, D), dtype=torch.bfloat16, device="cuda")
+    got = cache.attend(0, q, many(last), many(last), scale=1.0 / D)
+    want, bound = ref.attend(q[0], ref.stored(torch.cat([keys, last]), kind, 16), ref.stored(torch.cat([values, last]), kind, 16), L, scale=1.0 / D)
+    for b in range(batch):
+        close(got[b], want, bound)
+
+
 # ------------------------------------------------------------------------- rows that are computed again
 @pytest.mark.parametrize("D", [64, 128, 256])
 @pytest.mark.parametrize("softcap", [None, 20.0])

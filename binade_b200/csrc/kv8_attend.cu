@@ -29,7 +29,7 @@
 // codes the block that they fill before it reads it: a decode step is one launch. Several groups of rows (more than
 // 32, or 16 with heads of 256) read what an append kernel has written.
 //
-// Measured: 64 sequences of up to 8192 tokens, 8 key heads of 128, int8, 637 MB: 178 us, 3.6 TB/s, 55 % of the copy rate;
+// Measured: 64 sequences of up to 8192 tokens, 8 key heads of 128, int8, 637 MB: 179 us, 3.6 TB/s, 55 % of the copy rate;
 // one sequence of 131073, 269 MB: 71 us; one of 300: 21 us a call, 12 in a graph. What bounds the long ones: 68 M warp
 // instructions (430 a piece of 16 keys; 45 % of the issue slots) at 12 warps an SM, fixed-latency waits first.
 #include <cuda_bf16.h>

@@ -24,7 +24,7 @@ HOST_LIB = LIBDIR / "libbinade_b200_host.so"
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-lineinfo", "-O3", "-std=c++17",
-    "-Xcompiler", "-fPIC", "-shared",
+    "-Xcompiler", "-fPIC", "-shared", "--threads", "8",
 ]  # fmt: skip
 
 

@@ -4,7 +4,7 @@
   KV8Cache(layers, batch, ...)     keys and values of a batch of sequences as 8-bit codes with a scale for
                                    each block of tokens and head; append, attend, advance, dense
 
-Scores take the options that models put on them: softcap (s = cap tanh(s / cap)), slopes (a bias
+Scores take the options that models put on them: softcap (s = cap tanh(s / cap), caps from 2^-60 to 2^60), slopes (a bias
 -slope |i - j| for each query head), window (keys at a distance below it), prefix (the first keys of a document,
 seen from everywhere in it) and causal. Kernels, no gradients: tensors that ask for one are refused.
 """
